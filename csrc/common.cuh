@@ -30,6 +30,9 @@ enum : int {
   kTimeoutCellsGather = 10,   // all-reduce tail, gather step: a slice owner's result cells missing
   kTimeoutTopk = 11,      // vocabulary-parallel top-k: a rank's record never arrived
   kEpOverflow = 12,       // more rows for one expert (or one rank) than the receive slab / the grouped launch covers
+  kNoPage = 13,           // slot plan: the free pages ran out
+  kRowsOverflow = 14,     // slot plan: more new rows than the row buffers hold
+  kBadToken = 15,         // a drafted token outside the vocabulary
 };
 
 constexpr uint32_t kSpinLimit = 1u << 20;  // polls; each try_wait already suspends for a while

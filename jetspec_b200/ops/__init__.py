@@ -232,6 +232,23 @@ def paged_tree_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens,
                                     mask_bits, scale, causal)
 
 
+def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale, prefix_len,
+                            causal: bool = False, max_q: Optional[int] = None):
+    return ref.shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale, prefix_len, causal)
+
+
+def verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, sample_u, temperature=1.0, draft_temperature=None):
+    if target_logits.is_cuda:
+        return _ext().verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, sample_u, temperature, draft_temperature)
+    return ref.verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, sample_u, temperature, draft_temperature)
+
+
+def plan_slots(past_lens, counts, seq_rows, free_pages, page_size, slot_map, rows, mapped_lens=None):
+    if slot_map.is_cuda:
+        return _ext().plan_slots(past_lens, counts, seq_rows, free_pages, int(page_size), slot_map, int(rows), mapped_lens)
+    return ref.plan_slots(past_lens, counts, seq_rows, free_pages, page_size, slot_map, rows, mapped_lens)
+
+
 def lm_head_argmax(h, w):
     if _kern(h):
         from . import cuda_ext
@@ -255,7 +272,7 @@ def moe_forward(x, gate_w, w_gate_up, w_down, top_k, renorm, router_logits=None)
 
 __all__ = [
     "rmsnorm", "add_rmsnorm", "linear", "silu_mul", "qkv_postprocess", "kv_scatter",
-    "paged_tree_attention", "lm_head_argmax", "lm_head_topk_logprobs", "moe_forward",
+    "paged_tree_attention", "shared_prefix_attention", "verify_chains", "plan_slots", "lm_head_argmax", "lm_head_topk_logprobs", "moe_forward",
     "dynamic_tanh", "gelu_tanh_mul", "relu_squared", "latent_scatter", "latent_attention", "sigmoid_moe",
     "rmsnorm_f32", "linear_f32", "rotate_norm", "window_scatter", "window_attention", "delta_mix", "gated_head_norm",
     "experts_swiglu", "pool_blocks", "query_temperature", "depth_average", "xielu", "gelu_erf", "rotate", "head_gate", "retention",

@@ -181,7 +181,9 @@ STATUS_NAMES = {0: "ok", 1: "timeout waiting for a TMA stage", 2: "timeout waiti
                 9: "all-reduce tail / expert combine: partial cells never arrived",
                 10: "all-reduce tail: a slice owner's result cells never arrived",
                 11: "vocabulary-parallel top-k: a rank's record never arrived",
-                12: "expert-parallel dispatch: more rows for one expert than the grouped launch covers"}
+                12: "expert-parallel dispatch: more rows for one expert than the grouped launch covers",
+                13: "slot plan: the free pages ran out", 14: "slot plan: more new rows than the row buffers hold",
+                15: "drafted token outside the vocabulary"}
 
 
 def check_status(device) -> None:
@@ -1452,3 +1454,86 @@ def moe_forward(x, gate_w, w_gate_up, w_down, top_k: int, renorm: bool, router_l
     out.index_add_(0, tok.long(), ys.float() * row_w[:, None])
     out = out.to(x.dtype)
     return out if residual is None else residual.add_(out)
+
+
+# ------------------------------------------------------------------ a batched serving step
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _ints(device, **tensors) -> None:
+    """Index tensors of a serving op: contiguous int32 on its device."""
+    for name, t in tensors.items():
+        _need(t.dtype == torch.int32 and t.device == device and t.is_contiguous(), f"{name}: expected a contiguous int32 tensor on {device}")
+
+
+def _elsewhere(device) -> bool:
+    """Whether ``device`` is not the current one (kernels launch on the current device's stream)."""
+    return device.index is not None and device.index != (_cur_device() if _cur_device is not None else torch.cuda.current_device())
+
+
+def plan_slots(past_lens, counts, seq_rows, free_pages, page_size: int, slot_map, rows: int, mapped_lens=None):
+    """See :func:`jetspec_b200.ops.reference.plan_slots` for the contract."""
+    dev = slot_map.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return plan_slots(past_lens, counts, seq_rows, free_pages, page_size, slot_map, rows, mapped_lens)
+    mapped = past_lens if mapped_lens is None else mapped_lens
+    _ints(dev, past_lens=past_lens, counts=counts, seq_rows=seq_rows, free_pages=free_pages, slot_map=slot_map, mapped_lens=mapped)
+    B, (max_seqs, max_len) = past_lens.numel(), slot_map.shape
+    _need(counts.numel() == seq_rows.numel() == mapped.numel() == B, "past_lens, counts, seq_rows and mapped_lens differ in length")
+    _need(B <= 65535 and page_size >= 1 and rows >= 0, f"plan_slots(B={B}, page_size={page_size}, rows={rows})")
+    # blocks a request: enough to fill the SMs, a couple of thousand positions each
+    chunks = max(1, min(4 * SM_COUNT // max(1, B), max_len // 2048))
+    cu_q, cu_pages, positions, slots = torch.empty(2 * (B + 1) + 2 * rows, dtype=torch.int32, device=dev).split((B + 1, B + 1, rows, rows))
+    lib = load()
+    _check(lib.js_slot_plan(_p(past_lens), _p(counts), _p(mapped), _p(seq_rows), _p(free_pages), _p(slot_map), _p(cu_q), _p(cu_pages),
+                            _p(positions), _p(slots), _p(status_word(dev)), B, free_pages.numel(), page_size, max_seqs, max_len, rows,
+                            chunks, _stream()), "js_slot_plan")
+    return cu_q, positions, slots, cu_pages
+
+
+def _temperatures(t, B: int, device, name: str) -> tuple:
+    """Pointer to a temperature per sequence, or null and the one that holds for all."""
+    if torch.is_tensor(t):
+        _need(t.dtype == torch.float32 and t.device == device and t.is_contiguous() and t.numel() == B, f"{name}: expected a number or {B} fp32 values on {device}")
+        return _p(t), ctypes.c_double(0.0)
+    _need(t >= 0.0, f"{name}={t}")
+    return None, ctypes.c_double(t)
+
+
+def verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, sample_u, temperature=1.0, draft_temperature=None):
+    """See :func:`jetspec_b200.ops.reference.verify_chains` for the contract.  Logits in fp32 or bf16 (other types are converted), any row
+    stride."""
+    dev = target_logits.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, sample_u, temperature, draft_temperature)
+    B, D = cu_drafts.numel() - 1, drafts.numel()
+    _need(target_logits.dim() == 2 and draft_logits.dim() == 2 and draft_logits.device == dev, "logits: expected matrices on one device")
+    V = target_logits.shape[1]
+    _need(B >= 0 and V >= 1 and draft_logits.shape == (D, V) and target_logits.shape[0] == D + B,
+          f"{D} drafts of {B} sequences: target_logits {tuple(target_logits.shape)}, draft_logits {tuple(draft_logits.shape)}")
+    if target_logits.dtype != draft_logits.dtype or target_logits.dtype not in (torch.float32, torch.bfloat16):
+        target_logits, draft_logits = target_logits.float(), draft_logits.float()
+    if target_logits.stride(1) != 1:
+        target_logits = target_logits.contiguous()
+    if draft_logits.stride(1) != 1:
+        draft_logits = draft_logits.contiguous()
+    _ints(dev, drafts=drafts, cu_drafts=cu_drafts)
+    for name, u, n in (("accept_u", accept_u, D), ("sample_u", sample_u, B)):
+        _need(u.dtype == torch.float32 and u.device == dev and u.is_contiguous() and u.numel() == n, f"{name}: expected {n} fp32 values on {dev}")
+    temp = _temperatures(temperature, B, dev, "temperature")
+    draft_temp = temp if draft_temperature is None else _temperatures(draft_temperature, B, dev, "draft_temperature")
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    token = torch.empty(B, dtype=torch.int64, device=dev)
+    # few rows are cut into chunks so that two CTAs are on every SM
+    chunks = max(1, min(2 * SM_COUNT // max(1, D + B), V // 2048))
+    ws = torch.empty((2 * D + B) * chunks * 4 + B, dtype=torch.int32, device=dev)
+    lib = load()
+    _check(lib.js_chain_verify(_p(target_logits), ctypes.c_longlong(target_logits.stride(0)), _p(draft_logits), ctypes.c_longlong(draft_logits.stride(0)),
+                               int(target_logits.dtype == torch.bfloat16), _p(drafts), _p(cu_drafts), _p(accept_u), _p(sample_u), *temp,
+                               *draft_temp, _p(ws), _p(ws[ws.numel() - B:]), _p(accepted), _p(token), _p(status_word(dev)), B, D, V, chunks,
+                               2 * SM_COUNT, _stream()), "js_chain_verify")
+    return accepted, token

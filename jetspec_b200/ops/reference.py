@@ -329,6 +329,131 @@ def sample(logits: torch.Tensor, temperature: float = 0.0, generator=None) -> to
 
 
 # --------------------------------------------------------------------------
+# a batched serving step: shared prefix, chain verification, slot planning
+# --------------------------------------------------------------------------
+def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor, slot_map: torch.Tensor,
+                            seq_rows: torch.Tensor, cu_q: torch.Tensor, past_lens: torch.Tensor, mask_bits: Optional[torch.Tensor],
+                            scale: float, prefix_len: int, causal: bool = False) -> torch.Tensor:
+    """:func:`paged_tree_attention` of a batch whose sequences share their first ``prefix_len`` positions.
+
+    Every ``past_lens[b] >= prefix_len``, and the rows ``seq_rows`` of the slot map hold the same slots up to there; the prefix is
+    read through the first of them.  Rows behind the last sequence (``cu_q[-1]`` and on) are zero.
+    """
+    rows = slot_map.clone()
+    if seq_rows.numel():
+        r = seq_rows.long()
+        rows[r, :prefix_len] = slot_map[r[0], :prefix_len]
+    out = paged_tree_attention(q, k_pool, v_pool, rows, seq_rows, cu_q, past_lens, mask_bits, scale, causal)
+    out[int(cu_q[-1]):] = 0
+    return out
+
+
+GREEDY_BELOW = 1e-5      # temperatures below it mean the most likely token
+
+
+def chain_probabilities(logits: torch.Tensor, temperature: float) -> torch.Tensor:
+    """fp64 ``softmax(logits / T)`` of one row; a point mass at the lowest most likely index for ``T < 1e-5``; zeros where no logit
+    is above -inf."""
+    x = logits.double()
+    top = x.max()
+    if not bool(top > -math.inf):
+        return torch.zeros_like(x)
+    if temperature < GREEDY_BELOW:
+        return (torch.arange(x.numel(), device=x.device) == x.argmax()).double()
+    x = ((x - top) / temperature).exp()
+    return x / x.sum()
+
+
+def verify_chains(target_logits: torch.Tensor, draft_logits: torch.Tensor, drafts: torch.Tensor, cu_drafts: torch.Tensor,
+                  accept_u: torch.Tensor, sample_u: torch.Tensor, temperature=1.0, draft_temperature=None):
+    """Verify drafted chains against the target's probabilities, from given random numbers.
+
+    Sequence ``b`` of ``B`` drafted ``n_b`` tokens, ``drafts[cu_drafts[b]:cu_drafts[b + 1]]``, drawn from ``q = softmax(draft_logits /
+    draft_temperature)`` (a row each).  ``target_logits (D + B, V)`` holds ``n_b + 1`` rows a sequence, back to back: the target's
+    ``p = softmax(target_logits / temperature)`` at every draft's place and behind the last one.  Draft ``i`` is accepted when all
+    before it were and ``accept_u[i] * q_i(x_i) < p_i(x_i)``.  The next token is drawn by inverse CDF with ``sample_u[b]``: from
+    the last row when every draft was accepted, else from ``max(p - q, 0)`` at the first one that was not; the tokens kept are
+    then distributed like the target's own.  ``temperature`` and ``draft_temperature`` (default: the same) are numbers or ``(B,)``
+    tensors; below 1e-5 they mean the lowest most likely token.  The rows of a sequence behind its first rejection do not matter.
+
+    A row without any logit above -inf accepts nothing; its next token is -1.  Where rounding leaves nothing of ``max(p - q, 0)``
+    the target's most likely token is taken.  Returns ``(accepted (B,) int32, next token (B,) int64)``.
+    """
+    B = cu_drafts.numel() - 1
+    cu = cu_drafts.tolist()
+    each = lambda t, b: float(t[b]) if torch.is_tensor(t) else float(t)
+    draft_temperature = temperature if draft_temperature is None else draft_temperature
+    accepted, tokens = [], []
+    V = target_logits.shape[-1]
+    for b in range(B):
+        n, kept, weight = cu[b + 1] - cu[b], 0, None
+        t, td = each(temperature, b), each(draft_temperature, b)
+        for i in range(n):
+            p = chain_probabilities(target_logits[cu[b] + b + i], t)
+            q = chain_probabilities(draft_logits[cu[b] + i], td)
+            x = int(drafts[cu[b] + i])
+            if not (0 <= x < V and bool(accept_u[cu[b] + i].double() * q[x] < p[x])):
+                weight = (p - q).clamp_min(0)
+                break
+            kept += 1
+        row = target_logits[cu[b] + b + kept].double()
+        if weight is None:
+            weight = chain_probabilities(row, t)
+        run = weight.cumsum(0)
+        if not bool(row.max() > -math.inf):
+            token = -1
+        elif t < GREEDY_BELOW or not bool(run[-1] > 0):
+            token = int(row.argmax())
+        else:
+            token = min(int((run <= sample_u[b].double() * run[-1]).sum()), int(weight.nonzero()[-1]))
+        accepted.append(kept)
+        tokens.append(token)
+    dev = target_logits.device
+    return torch.tensor(accepted, dtype=torch.int32, device=dev), torch.tensor(tokens, dtype=torch.int64, device=dev)
+
+
+def plan_slots(past_lens: torch.Tensor, counts: torch.Tensor, seq_rows: torch.Tensor, free_pages: torch.Tensor, page_size: int,
+               slot_map: torch.Tensor, rows: int, mapped_lens: Optional[torch.Tensor] = None):
+    """Grant pages to the requests of a batch and lay out the rows of its next forward.
+
+    Request ``b`` (slot-map row ``seq_rows[b]``, a row of its own) has ``past_lens[b]`` committed positions and gets ``counts[b]`` new
+    ones; whole pages of ``page_size`` slots cover its first ``mapped_lens[b]`` positions (default: ``past_lens``).  The pages it lacks
+    come off ``free_pages`` in order, request after request, and their slots are written to ``slot_map (max_seqs, max_len)``.
+    Returns ``(cu_q (B + 1,), positions (rows,), slots (rows,), cu_pages (B + 1,))``, int32: offsets of the new rows, position and
+    slot of each, and offsets of the pages taken (``cu_pages[-1]`` in all).  Rows behind the last request have position 0 and
+    slot -1.  A slot is -1 too where the free pages ran out, a position is past the slot map, or a slot-map row is out of range or an
+    earlier request's; the kernel then also sets the device's status word (:func:`jetspec_b200.ops.cuda_ext.check_status`).
+    """
+    B, (max_seqs, max_len), dev = past_lens.numel(), slot_map.shape, slot_map.device
+    past, count = past_lens.long().clamp_min(0), counts.long().clamp_min(0)
+    held = -(-(past_lens if mapped_lens is None else mapped_lens).long().clamp_min(0) // page_size)
+    need = (-(-(past + count) // page_size) - held).clamp_min(0)
+    offsets = lambda n: torch.cat((n.new_zeros(1), n.cumsum(0)))
+    cu_q, cu_pages = offsets(count), offsets(need)
+    row = seq_rows.long()
+    known = (row[:, None] == row[None, :]).tril(-1).any(1)
+    sound = (row >= 0) & (row < max_seqs) & ~known
+    pages = torch.cat((free_pages.long(), free_pages.new_full((1,), -1).long()))
+
+    def granted(b, pos):
+        page = pages[(cu_pages[b] + pos // page_size - held[b]).clamp(0, pages.numel() - 1)]
+        return torch.where(page < 0, -1, page * page_size + pos % page_size)
+
+    b = torch.repeat_interleave(torch.arange(B, device=dev), need * page_size)
+    pos = held[b] * page_size + torch.arange(b.numel(), device=dev) - (cu_pages * page_size)[b]
+    keep = (pos < max_len) & sound[b]
+    b, pos = b[keep], pos[keep]
+    slot_map[row[b], pos] = granted(b, pos).to(slot_map.dtype)
+    positions, slots = (torch.full((rows,), v, dtype=torch.int32, device=dev) for v in (0, -1))
+    b = torch.repeat_interleave(torch.arange(B, device=dev), count)[:rows]
+    pos = past[b] + torch.arange(b.numel(), device=dev) - cu_q[b]
+    positions[:b.numel()] = pos.to(torch.int32)
+    ok = (pos < max_len) & sound[b]
+    slots[:b.numel()] = torch.where(ok, slot_map[torch.where(ok, row[b], 0), torch.where(ok, pos, 0)], -1) if b.numel() else slots[:0]
+    return cu_q.to(torch.int32), positions, slots, cu_pages.to(torch.int32)
+
+
+# --------------------------------------------------------------------------
 # window attention, gated delta rules, table-routed experts
 # --------------------------------------------------------------------------
 def rmsnorm_f32(x: torch.Tensor, weight: torch.Tensor, eps: float) -> torch.Tensor:

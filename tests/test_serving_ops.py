@@ -1,0 +1,290 @@
+"""Operators of a batched serving step: slot planning, attention behind a shared prefix, verification of drafted chains.
+
+On the CPU the PyTorch implementations against plain loops; on the GPU the kernels against them, in 64 bits where they compute.
+"""
+import math
+import random
+
+import pytest
+import torch
+
+from jetspec_b200 import ops
+from jetspec_b200.ops import reference as ref
+
+gpu = pytest.mark.gpu
+I32 = torch.int32
+
+
+@pytest.fixture
+def clean():
+    """The device's status word is clear before and after."""
+    from jetspec_b200.ops import cuda_ext
+    cuda_ext.check_status("cuda")
+    yield cuda_ext
+    cuda_ext.check_status("cuda")
+
+
+def i32(*v, device="cpu"):
+    return torch.tensor(v, dtype=I32, device=device)
+
+
+# ------------------------------------------------------------------ slot planning
+def plan_by_loops(past, counts, rows, free, page, slot_map, T, mapped):
+    """The contract of ``plan_slots``, request by request."""
+    free, out, taken, cu_q, cu_p = list(free), [], set(), [0], [0]
+    slot_map = [list(r) for r in slot_map]
+    max_len = len(slot_map[0])
+    for p, c, r, m in zip(past, counts, rows, mapped):
+        sound = 0 <= r < len(slot_map) and r not in taken
+        taken.add(r)
+        held, want = -(-m // page), -(-(p + c) // page)
+        pages = {j: free.pop(0) if free else -1 for j in range(held, want)}
+        slot = lambda pos: -1 if pages[pos // page] < 0 else pages[pos // page] * page + pos % page
+        for pos in range(held * page, want * page):
+            if sound and pos < max_len:
+                slot_map[r][pos] = slot(pos)
+        for pos in range(p, p + c):
+            out.append((pos, -1 if not sound or pos >= max_len else slot_map[r][pos]))
+        cu_q.append(cu_q[-1] + c)
+        cu_p.append(cu_p[-1] + max(0, want - held))
+    out = (out + [(0, -1)] * T)[:T]
+    return cu_q, [o[0] for o in out], [o[1] for o in out], cu_p, slot_map
+
+
+def plan_case(seed, B, page, max_len, count, window=0, short=0, extra_rows=0, device="cpu"):
+    """Requests of mixed lengths on random pages; ``short``: how many pages are missing."""
+    r = random.Random(seed)
+    past = [r.randint(0, max(0, max_len - count - page)) for _ in range(B)]
+    counts = [r.choice([0, 1, count, r.randint(0, count)]) for _ in range(B)]
+    mapped = [min(p + r.choice([0, window]), max_len) for p in past]
+    seqs = B + 2
+    need = sum(max(0, -(-(p + c) // page) - -(-m // page)) for p, c, m in zip(past, counts, mapped))
+    ids = list(range(need + seqs))
+    r.shuffle(ids)
+    g = torch.Generator().manual_seed(seed)
+    slot_map = torch.randint(0, 1000, (seqs, max_len), generator=g, dtype=I32)
+    rows = r.sample(range(seqs), B)
+    t = lambda v: torch.tensor(v, dtype=I32, device=device)
+    return dict(past_lens=t(past), counts=t(counts), seq_rows=t(rows), free_pages=t(ids[:max(0, need - short)]), page_size=page,
+                slot_map=slot_map.to(device), rows=sum(counts) + extra_rows, mapped_lens=t(mapped))
+
+
+PLANS = [  # B, page, max_len, count, window, missing pages, rows too many (below 0: too few)
+    (1, 16, 64, 1, 0, 0, 0), (1, 16, 64, 40, 0, 0, 3), (7, 16, 200, 33, 20, 0, 5), (16, 1, 50, 9, 3, 0, 0), (33, 5, 121, 60, 7, 0, 1),
+    (9, 64, 512, 130, 0, 0, 0), (5, 16, 160, 50, 0, 4, 2), (300, 16, 96, 20, 16, 0, 7), (6, 128, 100, 30, 0, 0, 4),
+]
+
+
+def run_plan(fn, case):
+    c = dict(case)
+    slot_map = c["slot_map"].clone()
+    out = fn(c["past_lens"], c["counts"], c["seq_rows"], c["free_pages"], c["page_size"], slot_map, c["rows"], c["mapped_lens"])
+    return [o.tolist() for o in out] + [slot_map.tolist()]
+
+
+def plan_expected(case):
+    c = {k: v.tolist() if torch.is_tensor(v) else v for k, v in case.items()}
+    return list(plan_by_loops(c["past_lens"], c["counts"], c["seq_rows"], c["free_pages"], c["page_size"], c["slot_map"], c["rows"],
+                              c["mapped_lens"]))
+
+
+@pytest.mark.parametrize("plan", PLANS)
+def test_plan_slots_by_loops(plan):
+    B, page, max_len, count, window, short, more = plan
+    case = plan_case(B + page, B, page, max_len, count, window, short, more)
+    assert run_plan(ops.plan_slots, case) == plan_expected(case)
+
+
+def odd_plans(device="cpu"):
+    """Calls with something wrong in them, and what the status word says: (case, status)."""
+    def case(past, counts, rows, free, page, max_len, T, seqs=3):
+        t = lambda v: torch.tensor(v, dtype=I32, device=device)
+        return dict(past_lens=t(past), counts=t(counts), seq_rows=t(rows), free_pages=t(free), page_size=page,
+                    slot_map=torch.arange(seqs * max_len, dtype=I32, device=device).view(seqs, max_len) + 500, rows=T, mapped_lens=t(past))
+    return [
+        (case([5, 9], [4, 4], [1, 1], [3, 4], 4, 32, 8), 5),          # the same slot-map row twice: the second gets nothing
+        (case([5, 9], [4, 4], [1, 7], [3, 4], 4, 32, 8), 5),          # a row out of range
+        (case([5, 9], [4, 4], [-1, 0], [3, 4], 4, 32, 8), 5),
+        (case([30, 2], [6, 1], [0, 1], [3, 4], 4, 32, 7), 5),         # positions past the slot map
+        (case([4, 4], [4, 4], [0, 1], [3], 4, 32, 8), 13),            # too few pages
+        (case([4, 4], [4, 4], [0, 1], [], 4, 32, 8), 13),
+        (case([4, 4], [4, 4], [0, 1], [3, 4], 4, 32, 6), 14),         # too few rows
+    ]
+
+
+def test_plan_slots_with_something_wrong():
+    for case, _ in odd_plans():
+        assert run_plan(ops.plan_slots, case) == plan_expected(case)
+
+
+def test_plan_slots_of_nothing():
+    for device in ["cpu"] + ["cuda"] * torch.cuda.is_available():
+        e = torch.empty(0, dtype=I32, device=device)
+        slot_map = torch.full((2, 8), 7, dtype=I32, device=device)
+        cu_q, positions, slots, cu_pages = ops.plan_slots(e, e, e, e, 4, slot_map, 3)
+        assert cu_q.tolist() == [0] and cu_pages.tolist() == [0] and positions.tolist() == [0] * 3 and slots.tolist() == [-1] * 3
+        assert [o.numel() for o in ops.plan_slots(e, e, e, e, 4, slot_map, 0)] == [1, 0, 0, 1] and bool((slot_map == 7).all())
+
+
+@gpu
+@pytest.mark.parametrize("plan", PLANS + [(3, 16, 70000, 66000, 0, 0, 11), (1000, 16, 300, 40, 0, 0, 0)])
+def test_plan_slots_kernel(clean, plan):
+    B, page, max_len, count, window, short, more = plan
+    case = plan_case(B + page, B, page, max_len, count, window, short, more, device="cuda")
+    cpu = {k: v.cpu() if torch.is_tensor(v) else v for k, v in case.items()}
+    assert run_plan(ops.plan_slots, case) == run_plan(ref.plan_slots, cpu)
+    if short:
+        with pytest.raises(RuntimeError, match="free pages ran out"):
+            clean.check_status("cuda")
+
+
+@gpu
+def test_plan_slots_kernel_with_something_wrong(clean):
+    for (case, status), (cpu, _) in zip(odd_plans("cuda"), odd_plans()):
+        assert run_plan(ops.plan_slots, case) == run_plan(ref.plan_slots, cpu)
+        with pytest.raises(RuntimeError, match=f"status {status}"):
+            clean.check_status("cuda")
+
+
+def kernel_refuses(call, *words):
+    with pytest.raises(ValueError, match="|".join(words)):
+        call()
+
+
+def test_plan_slots_refusals():
+    from jetspec_b200.ops import cuda_ext
+    z, m = i32(0, 0), torch.zeros(2, 8, dtype=I32)
+    plan = lambda **kw: cuda_ext.plan_slots(**{**dict(past_lens=z, counts=z, seq_rows=z, free_pages=z, page_size=4, slot_map=m, rows=2), **kw})
+    kernel_refuses(lambda: plan(past_lens=z.long()), "past_lens")
+    kernel_refuses(lambda: plan(free_pages=i32(1, 2, 3, 4)[::2]), "free_pages")
+    kernel_refuses(lambda: plan(slot_map=torch.zeros(8, 2, dtype=I32).t()), "slot_map")
+    kernel_refuses(lambda: plan(counts=i32(0)), "length")
+    kernel_refuses(lambda: plan(mapped_lens=i32(0)), "length")
+    kernel_refuses(lambda: plan(page_size=0), "page_size")
+    kernel_refuses(lambda: plan(rows=-1), "rows")
+
+
+# ------------------------------------------------------------------ verification of chains
+def chains(seed, lens, V, dtype=torch.float32, spread=3.0, shift=0.75, device="cpu"):
+    g = torch.Generator().manual_seed(seed)
+    D, B = sum(lens), len(lens)
+    draft = (torch.randn(D, V, generator=g) * spread).to(dtype)
+    target = torch.randn(D + B, V, generator=g) * spread
+    seq = torch.repeat_interleave(torch.arange(B), torch.tensor(lens, dtype=torch.long))
+    at = torch.arange(D) + seq
+    target[at] = draft.float() + shift * target[at] / spread
+    drafts = torch.multinomial(draft.float().softmax(-1), 1, generator=g).view(-1).to(I32) if D else torch.zeros(0, dtype=I32)
+    cu = torch.tensor([0] + torch.tensor(lens, dtype=torch.long).cumsum(0).tolist(), dtype=I32)
+    out = dict(target_logits=target.to(dtype), draft_logits=draft, drafts=drafts, cu_drafts=cu, accept_u=torch.rand(D, generator=g),
+               sample_u=torch.rand(B, generator=g))
+    return {k: v.to(device) for k, v in out.items()}
+
+
+def test_verify_chains_keeps_the_targets_distribution():
+    """20000 chains of two drafts over 6 tokens: the first token kept is distributed like the target's first row, and the second, after
+    an accepted first, like the target's second row.  Bounds: 4.5 standard deviations of a share of n draws."""
+    n, V = 20000, 6
+    one = chains(0, [2], V, spread=1.0, shift=1.5)
+    g = torch.Generator().manual_seed(1)
+    q, p = one["draft_logits"].softmax(-1), one["target_logits"].softmax(-1)
+    drafts = torch.stack([torch.multinomial(q[i], n, replacement=True, generator=g) for i in range(2)], 1)
+    kept, token = ref.verify_chains(one["target_logits"].repeat(n, 1), one["draft_logits"].repeat(n, 1), drafts.reshape(-1).to(I32),
+                                    torch.arange(n + 1, dtype=I32) * 2, torch.rand(2 * n, generator=g), torch.rand(n, generator=g))
+    first = torch.where(kept > 0, drafts[:, 0], token)
+    second = torch.where(kept > 1, drafts[:, 1], token)[kept > 0]
+    for got, want in ((first, p[0]), (second, p[1])):
+        share = torch.bincount(got, minlength=V) / got.numel()
+        assert bool(((share - want).abs() <= 4.5 * (want * (1 - want) / got.numel()).sqrt()).all())
+    assert 0.2 < float((kept > 0).double().mean()) < 0.95
+
+
+def test_verify_chains_by_hand():
+    """Point masses and empty rows, where every number is known."""
+    inf = math.inf
+    row = lambda *p: torch.tensor([math.log(x) if x else -inf for x in p])
+    call = lambda target, draft, x, u, v, **kw: tuple(int(t) for t in ops.verify_chains(
+        torch.stack(target), torch.stack(draft), i32(*x), i32(0, len(x)), torch.tensor(u), torch.tensor([v]), **kw))
+    p, q = row(.5, .25, .25), row(.25, .5, .25)
+    assert call([p, p], [q], [1], [.49], .0) == (1, 0)                # u q < p: .49 * .5 < .25; then the first of the last row
+    assert call([p, p], [q], [1], [.51], .9) == (0, 0)                # only token 0 is in the difference
+    assert call([p, row(0, 0, 1)], [q], [1], [.4], .9) == (1, 2)
+    assert call([row(0, .5, .5), p], [q], [0], [.0], .0) == (0, 2)    # the target gives the draft nothing: 0 < 0 is false; .25 is left at 2
+    empty = row(0, 0, 0)
+    assert call([empty, p], [q], [1], [.0], .5) == (0, -1)            # a row whose mask leaves nothing
+    assert call([p, empty], [q], [0], [.5], .5) == (1, -1)
+    assert call([p, p], [empty], [2], [.9], .3) == (1, 0)             # the draft's row says nothing: whatever the target can say is kept
+    assert call([p, p], [q], [1], [.9], .7, temperature=0.0) == (0, 0)
+    assert call([p, p], [p], [0], [.9], .7, temperature=0.0) == (1, 0)
+    assert call([p, row(.25, .375, .375)], [p], [0], [.9], .7, temperature=0.0) == (1, 1)      # equal: the lowest index
+    assert call([p, p], [p], [0], [.6], .4, draft_temperature=0.0) == (0, 1)      # drafted for certain, .6 >= .5: without token 0
+    assert call([p, p], [q], [7], [.0], .0) == (0, 0)                 # no such token
+
+
+CHAINS = [([3], 151936, torch.float32), ([0], 1000, torch.float32), ([1], 1, torch.float32), ([2, 0, 5, 1], 7, torch.bfloat16),
+          ([4] * 20, 32001, torch.float32), ([6, 3, 0, 8, 2], 151936, torch.bfloat16), ([1, 2] * 150, 515, torch.float32),
+          ([40], 4099, torch.bfloat16), (list(range(17)), 50001, torch.float32), ([700, 1], 33, torch.float32)]
+
+
+@gpu
+@pytest.mark.parametrize("lens,V,dtype", CHAINS)
+def test_verify_chains_kernel(clean, lens, V, dtype):
+    c = chains(len(lens) + V, lens, V, dtype)
+    dev = {k: v.cuda() for k, v in c.items()}
+    hot = 0.5 + torch.rand(len(lens), generator=torch.Generator().manual_seed(3))
+    cold = hot.clone()
+    cold[::2] = 0.0
+    for kw in (dict(), dict(temperature=0.7), dict(temperature=hot, draft_temperature=1.0), dict(temperature=cold), dict(temperature=0.0),
+               dict(draft_temperature=0.0)):
+        want = ref.verify_chains(**c, **kw)
+        got = ops.verify_chains(**dev, **{k: v.cuda() if torch.is_tensor(v) else v for k, v in kw.items()})
+        assert got[0].tolist() == want[0].tolist() and got[1].tolist() == want[1].tolist()
+        assert got[0].dtype == I32 and got[1].dtype == torch.int64
+
+
+@gpu
+def test_verify_chains_kernel_masked_and_strided(clean):
+    """Vocabularies cut down to a few tokens (-inf elsewhere), empty rows, views of wider matrices, rows off 16-byte boundaries, drafts
+    with the same token again, numbers at the ends of [0, 1)."""
+    for V, dtype in ((1000, torch.float32), (1003, torch.bfloat16), (9001, torch.float16)):
+        c = chains(V, [5, 1, 0, 7, 3, 2], V, dtype)
+        g = torch.Generator().manual_seed(9)
+        keep = torch.rand(1, V, generator=g) < 0.02
+        keep[0, c["drafts"].long()[::2]] = True
+        for name in ("target_logits", "draft_logits"):
+            c[name] = c[name].masked_fill(~keep, -math.inf)
+        c["target_logits"][3] = -math.inf
+        c["draft_logits"][9] = -math.inf
+        c["drafts"][6:10] = c["drafts"][6]
+        c["accept_u"][0], c["accept_u"][6], c["sample_u"][0], c["sample_u"][1] = 0.0, 1 - 2 ** -24, 0.0, 1 - 2 ** -24
+        want = ref.verify_chains(**c)
+        dev = {k: v.cuda() for k, v in c.items()}
+        wide = {k: torch.full((dev[k].shape[0], V + 5), math.nan, dtype=dtype, device="cuda") for k in ("target_logits", "draft_logits")}
+        for k, w in wide.items():
+            w[:, 3:V + 3] = dev[k]
+            dev[k] = w[:, 3:V + 3]
+        got = ops.verify_chains(**dev)
+        assert got[0].tolist() == want[0].tolist() and got[1].tolist() == want[1].tolist()
+
+
+@gpu
+def test_verify_chains_kernel_bad_token(clean):
+    c = chains(5, [3, 2], 100, device="cuda")
+    c["drafts"][0], c["drafts"][4], c["accept_u"] = -1, 100, c["accept_u"] * 0
+    accepted, token = ops.verify_chains(**c)
+    assert accepted.tolist()[0] == 0 and accepted.tolist()[1] == 1 and bool((token >= 0).all() & (token < 100).all())
+    with pytest.raises(RuntimeError, match="outside the vocabulary"):
+        clean.check_status("cuda")
+
+
+def test_verify_chains_refusals():
+    from jetspec_b200.ops import cuda_ext
+    c = chains(0, [2, 1], 9)
+    call = lambda **kw: cuda_ext.verify_chains(**{**c, **kw})
+    kernel_refuses(lambda: call(target_logits=c["target_logits"][:4]), "drafts of")
+    kernel_refuses(lambda: call(draft_logits=c["draft_logits"][:, :8]), "drafts of")
+    kernel_refuses(lambda: call(drafts=c["drafts"].long()), "drafts")
+    kernel_refuses(lambda: call(accept_u=c["accept_u"].double()), "accept_u")
+    kernel_refuses(lambda: call(sample_u=c["sample_u"][:1]), "sample_u")
+    kernel_refuses(lambda: call(temperature=-1.0), "temperature")
+    kernel_refuses(lambda: call(temperature=torch.ones(3)), "temperature")
+    kernel_refuses(lambda: call(draft_temperature=torch.ones(2, dtype=torch.float64)), "draft_temperature")
