@@ -1,0 +1,728 @@
+// Attention of a batch whose sequences share a long prefix (tcgen05, head_dim 128), over the slot-addressed pool.
+//
+// Softmax over a union of key sets: with (m, l, O) = (maximum, sum of 2^(s - m), sum of 2^(s - m) v) of each set, the union has
+// m = max m_i, l = sum l_i 2^(m_i - m), O = sum O_i 2^(m_i - m), output O / l.  So the shared prefix [0, P) is attended by the rows
+// of ALL sequences together (128 rows a tile whatever sequences they are from, its keys read once), every sequence attends to its
+// own keys [P, L), and the parts are joined.  Where every sequence's rows fill tiles of their own there is nothing to gain by that, and a
+// sequence's rows take both ranges in one go.
+//
+// Work is a line of units, a unit being 128 keys for a pair of row tiles: items (pair of tiles, KV head) one after the other, an
+// item's units in key order.  Every CTA takes an equal piece of the line, so lengths, which only the device knows, balance by
+// themselves; where a piece begins or ends inside an item its parts go through a workspace and attn_shared_merge_kernel.
+//
+// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warp 8 issues the MMAs, warps 9-12 load K and V by TMA (boxes of 16 rows where
+// slots follow one another, gathers of four rows where not), warps 13-14 load Q.  A job is one row tile against 128 keys; jobs alternate between the
+// groups: the two tiles of a pair on the same keys, or, for a single tile, every other block of keys.  Scores (128 columns) and
+// output (128 columns) of both groups fill the 512 columns of tensor memory; probabilities overwrite the scores as bf16 and are the second
+// MMA's A operand there.  Every wait is bounded (status word).
+#include "gemm_common.cuh"
+
+#include <math.h>
+
+namespace js {
+
+constexpr int SD = 128;              // head dim
+constexpr int SROWS = 128;           // rows of a tile
+constexpr int SKEYS = 128;           // keys of a unit
+constexpr int SSLOTS = 5;            // ring of K and V tiles, in turn
+constexpr int kSTile = 128 * 256;    // bytes of a K, V or Q tile: 2 halves x 128 rows x 128 B
+constexpr int SWARPS = 15, STHREADS = 32 * SWARPS;
+constexpr int kSharedSmem = (2 + SSLOTS) * kSTile + 512 + 1024;
+
+struct SharedAttn {
+  const __nv_bfloat16* q;      // (T, Hq, 128), ldq elements between tokens
+  const int *slot_map, *seq_rows, *cu_q, *past_lens, *mask_bits;
+  __nv_bfloat16* out;          // (T, Hq * 128)
+  int* plan;                   // units in all; of every item its first unit
+  float *po, *so;              // partial outputs of prefix and sequence segments: (segment, side, row, 128)
+  float2 *pml, *sml;           // their (maximum, sum): (segment, side, row)
+  int* status;
+  long long ldq;
+  int B, T, Hq, Hkv, S, max_seqs, max_len, W, causal, G, npt, ctas;
+  int prefix;                  // keys of the prefix items (0: none)
+  int first_key;               // where the sequences' own items begin
+  int prefix_items, seq_items, seq_rows_kept;      // bounds on item numbers; rows of a sequence segment's tile that the workspace holds
+  float scale_log2;
+};
+
+struct SharedMaps {
+  CUtensorMap k16, v16;        // boxes of 16 rows x 64 columns
+  CUtensorMap k1, v1;          // boxes of one row, for gathers
+};
+
+JS_DEVICE int sa_wait(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t* gave_up) {
+  return mbar_wait_warp(bar, parity, status, code, gave_up);
+}
+
+// ---------------------------------------------------------------- the line of units
+struct SaSeq { int q_begin, n, past, first, end, row; };      // rows, committed keys, key range, slot-map row
+JS_DEVICE SaSeq sa_seq(const SharedAttn& p, int b) {
+  SaSeq s;
+  if (b < 0) {                 // the prefix, for the rows of all sequences
+    s.q_begin = 0;
+    s.n = max(0, min(p.cu_q[p.B], p.T));
+    s.past = s.end = p.prefix;
+    s.first = 0;
+    s.row = p.seq_rows[0];
+  } else {
+    s.q_begin = min(max(0, p.cu_q[b]), p.T);
+    s.n = max(0, min(p.cu_q[b + 1], p.T) - s.q_begin);
+    s.past = min(max(0, p.past_lens[b]), p.max_len);
+    s.end = min(s.past + s.n, p.max_len);
+    s.first = p.first_key;
+    s.row = p.seq_rows[b];
+  }
+  return s;
+}
+// keys a pair of tiles sees end here
+JS_DEVICE int sa_end(const SharedAttn& p, const SaSeq& s, int b, int pair) {
+  return b >= 0 && p.causal ? min(s.end, s.past + (pair + 1) * 2 * p.npt) : s.end;
+}
+JS_DEVICE int sa_units(const SharedAttn& p, const SaSeq& s, int b, int pair) {
+  return max(0, sa_end(p, s, b, pair) - s.first + SKEYS - 1) / SKEYS;
+}
+JS_DEVICE int sa_pairs(const SharedAttn& p, const SaSeq& s) { return (s.n + 2 * p.npt - 1) / (2 * p.npt); }
+JS_DEVICE int sa_total(const SharedAttn& p, int b) {       // units of one head
+  const SaSeq s = sa_seq(p, b);
+  const int pairs = sa_pairs(p, s);
+  if (b < 0 || !p.causal) return pairs * sa_units(p, s, b, 0);
+  int n = 0;
+  for (int i = 0; i < pairs; ++i) n += sa_units(p, s, b, i);
+  return n;
+}
+// Item numbers grow along the line (with gaps): a sequence starts behind the pairs of all rows before it.
+JS_DEVICE int sa_item(const SharedAttn& p, const SaSeq& s, int b, int pair, int h) {
+  return (b < 0 ? pair : p.prefix_items / p.Hkv + s.q_begin / (2 * p.npt) + b + pair) * p.Hkv + h;
+}
+// The line is cut into as many pieces as there are CTAs, none of them empty: with fewer units than CTAs the last CTAs have none.
+JS_DEVICE int sa_cta(const SharedAttn& p, int unit, int total) {
+  return static_cast<int>((static_cast<long long>(unit + 1) * min(p.ctas, total) - 1) / total);
+}
+JS_DEVICE int sa_start(const SharedAttn& p, int cta, int total) {
+  const int pieces = min(p.ctas, total);
+  return cta >= pieces ? total : static_cast<int>(static_cast<long long>(total) * cta / pieces);
+}
+
+// A CTA's piece of the line, item by item; every role walks it for itself.
+struct SaWalk {
+  int b, pair, h, t, left;     // next unit, units left
+  int parity;                  // group of the next job
+  SaSeq s;
+  int units, nt;               // of the item; of them in this segment, from t
+  int group0;                  // the group of the segment's first job
+  bool two;                    // both tiles of the pair have rows
+};
+JS_DEVICE void sa_begin(const SharedAttn& p, SaWalk& w) { if (w.left > 0) w.s = sa_seq(p, w.b); }
+// the next segment; t has been moved behind it when the call after this one is made
+JS_DEVICE bool sa_next(const SharedAttn& p, SaWalk& w) {
+  if (w.left <= 0) return false;
+  for (;;) {
+    w.units = sa_units(p, w.s, w.b, w.pair);
+    if (w.pair < sa_pairs(p, w.s) && w.t < w.units) break;
+    w.t = 0;
+    if (w.units == 0 || ++w.h == p.Hkv) {
+      w.h = 0;
+      ++w.pair;
+    }
+    while (w.pair >= sa_pairs(p, w.s)) {
+      w.pair = 0;
+      if (++w.b >= p.B) return false;
+      w.s = sa_seq(p, w.b);
+    }
+  }
+  w.nt = min(w.left, w.units - w.t);
+  w.two = w.s.n - w.pair * 2 * p.npt > p.npt;
+  w.group0 = w.parity;
+  return true;
+}
+JS_DEVICE void sa_done(SaWalk& w) {
+  w.left -= w.nt;
+  w.t += w.nt;
+  if (!w.two) w.parity ^= w.nt & 1;
+}
+
+JS_DEVICE void sa_mma_tmem_a(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(d), "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+JS_DEVICE void sa_tmem_st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+JS_DEVICE void sa_tmem_st32(uint32_t taddr, const uint32_t* r) {
+  sa_tmem_st16(taddr, r);
+  sa_tmem_st16(taddr + 16, r + 16);
+}
+JS_DEVICE void sa_tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+JS_DEVICE float sa_exp2(float x) {      // denormal results flush to zero; exp2(-inf) = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+JS_DEVICE void sa_cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
+JS_DEVICE void sa_tma_box(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y) : "memory");
+}
+JS_DEVICE void sa_tma_rows(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y0, int y1, int y2, int y3) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(y0), "r"(y1), "r"(y2), "r"(y3) : "memory");
+}
+// MN-major operand stored as two 64-column halves of 128-byte rows, 128-byte swizzle; the halves `half_stride` bytes apart
+JS_DEVICE uint64_t sa_desc_mn(uint32_t smem_addr, uint32_t half_stride) {
+  uint64_t d = 0;
+  d |= static_cast<uint64_t>((smem_addr & 0x3FFFF) >> 4);
+  d |= static_cast<uint64_t>(half_stride >> 4) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+// Keys [k, k + 32) that a row sees, bit by bit: all committed ones, and new ones by the causal rule or the row's ancestor bits
+JS_DEVICE uint32_t sa_visible(const SharedAttn& p, const SaSeq& s, bool prefix, int end, int node, const int* bits, int k) {
+  const int j = k - s.past;                                    // place of the first among the new rows
+  uint32_t v = j <= -32 ? 0xffffffffu : j < 0 ? (1u << -j) - 1u : 0u;
+  if (!prefix && j > -32) {
+    if (p.causal) {
+      const int c = node - j;
+      if (c >= 31) v = 0xffffffffu; else if (c >= 0) v |= (1u << (c + 1)) - 1u;
+    } else {
+      auto word = [&](int i) { return i >= 0 && i < p.W ? static_cast<uint32_t>(bits[i]) : 0u; };
+      if (j < 0) v |= word(0) << -j;
+      else v = __funnelshift_r(word(j >> 5), word((j >> 5) + 1), j & 31);
+    }
+  }
+  const int left = end - k;                                    // keys at or past the end do not exist
+  if (left < 32) v &= left <= 0 ? 0u : (1u << left) - 1u;
+  return v;
+}
+
+__global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAttn p, const __grid_constant__ SharedMaps maps) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sQ = smem, *sKV = smem + 2 * kSTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + SSLOTS * kSTile);
+  uint64_t *kv_full = bars, *kv_empty = bars + SSLOTS;                        // a slot of the ring
+  uint64_t *q_full = bars + 2 * SSLOTS, *q_empty = q_full + 2;                // a Q buffer
+  uint64_t *s_full = q_empty + 2, *p_full = s_full + 2, *o_full = p_full + 2; // a group
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint32_t* gave_up_words = tmem_slot + 1;
+  int* start = reinterpret_cast<int*>(gave_up_words + 16);                    // the first unit: b, pair, h, t; units in all; scan scratch
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t* gave_up = gave_up_words + warp;
+
+  pdl_launch_dependents();
+  pdl_wait();
+
+  // ---- this CTA's piece of the line
+  if (tid == 0) {
+    for (int s = 0; s < SSLOTS; ++s) { mbar_init(&kv_full[s], 4); mbar_init(&kv_empty[s], 1); }
+    for (int g = 0; g < 2; ++g) {
+      mbar_init(&q_full[g], 64);
+      mbar_init(&q_empty[g], 1);
+      mbar_init(&s_full[g], 1);
+      mbar_init(&p_full[g], 128);
+      mbar_init(&o_full[g], 1);
+    }
+    for (int w = 0; w < 16; ++w) gave_up_words[w] = 0;
+    fence_barrier_init();
+  }
+  int* scan = start + 8;                        // a total per warp
+  const int prefix_units = p.prefix > 0 ? sa_total(p, -1) * p.Hkv : 0;
+  int mine = 0;
+  for (int b = tid; b < p.B; b += STHREADS) mine += sa_total(p, b) * p.Hkv;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) scan[warp] = mine;
+  __syncthreads();
+  int total = prefix_units;
+  for (int w = 0; w < SWARPS; ++w) total += scan[w];
+  const int u0 = sa_start(p, blockIdx.x, total), u1 = sa_start(p, blockIdx.x + 1, total);
+  if (u0 < prefix_units) {
+    if (tid == 0) {
+      const SaSeq s = sa_seq(p, -1);
+      const int units = sa_units(p, s, -1, 0);
+      start[0] = -1;
+      start[1] = u0 / units / p.Hkv;
+      start[2] = u0 / units % p.Hkv;
+      start[3] = u0 % units;
+    }
+  } else if (u0 < u1) {
+    int run = prefix_units;
+    for (int base = 0; base < p.B; base += STHREADS) {
+      const int b = base + tid, v = b < p.B ? sa_total(p, b) * p.Hkv : 0;
+      int inc = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int other = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += other;
+      }
+      __syncthreads();
+      if (lane == 31) scan[warp] = inc;
+      __syncthreads();
+      int before = run + inc - v;
+      for (int w = 0; w < SWARPS; ++w) {
+        if (w < warp) before += scan[w];
+        run += scan[w];
+      }
+      if (u0 >= before && u0 < before + v) {
+        const SaSeq s = sa_seq(p, b);
+        int pair = 0, at = u0 - before;
+        while (at >= sa_units(p, s, b, pair) * p.Hkv) at -= sa_units(p, s, b, pair++) * p.Hkv;
+        const int units = sa_units(p, s, b, pair);
+        start[0] = b;
+        start[1] = pair;
+        start[2] = at / units;
+        start[3] = at % units;
+      }
+    }
+  }
+  if (warp == 8) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0 && blockIdx.x == 0) p.plan[0] = total;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  SaWalk w;
+  w.left = u1 - u0;
+  if (w.left > 0) {
+    w.b = start[0];
+    w.pair = start[1];
+    w.h = start[2];
+    w.t = start[3];
+  }
+  w.parity = 0;
+  sa_begin(p, w);
+
+  if (warp >= 13) {
+    // ================================================================ Q loaders; the first of them notes where items begin
+    const int lt = tid - 13 * 32;
+    int uses = 0;                               // Q buffers filled so far: buffer uses % 2
+    int unit = u0;
+    bool ok = true;
+    while (ok && sa_next(p, w)) {
+      if (lt == 0 && w.t == 0) p.plan[1 + sa_item(p, w.s, w.b, w.pair, w.h)] = unit;
+      unit += w.nt;
+      for (int side = 0; side < (w.two ? 2 : 1) && ok; ++side, ++uses) {
+        const int buf = uses & 1;
+        ok = sa_wait(&q_empty[buf], ((uses >> 1) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
+        if (!ok) break;
+        const uint32_t dst = smem_u32(sQ + buf * kSTile);
+        const int node0 = (w.pair * 2 + side) * p.npt;
+        for (int c = lt; c < SROWS * 16; c += 64) {
+          const int r = c >> 4, ch = c & 15, tok = r / p.G, node = node0 + tok;
+          const bool valid = tok < p.npt && node < w.s.n;
+          const __nv_bfloat16* src = p.q + (valid ? static_cast<long long>(w.s.q_begin + node) * p.ldq + (w.h * p.G + r % p.G) * SD + ch * 8 : 0);
+          sa_cp_async16(dst + (ch >> 3) * (SROWS * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, valid);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async();
+        mbar_arrive(&q_full[buf]);
+      }
+      sa_done(w);
+    }
+  } else if (warp >= 9) {
+    // ================================================================ K/V loaders: 32 keys of every tile each
+    const int lw = warp - 9;
+    int n = 0;                                  // ring slots used so far
+    bool ok = true;
+    while (ok && sa_next(p, w)) {
+      const bool known = w.s.row >= 0 && w.s.row < p.max_seqs;
+      if (!known) report(p.status, kBadSlot);
+      const int* slots = p.slot_map + static_cast<size_t>(known ? w.s.row : 0) * p.max_len;
+      const int end = sa_end(p, w.s, w.b, w.pair), row0 = w.h * p.S;
+      auto slot_at = [&](int i) { return __ldg(slots + min(w.s.first + (w.t + i) * SKEYS + 32 * lw + lane, end - 1)); };      // keys past the end repeat the last one (no row sees them)
+      int next = slot_at(0);
+      for (int i = 0; i < w.nt && ok; ++i) {
+        int slot = next;
+        if (i + 1 < w.nt) next = slot_at(i + 1);
+        if (slot < 0 || slot >= p.S) { report(p.status, kBadSlot); slot = 0; }
+        const int first = __shfl_sync(0xffffffffu, slot, lane & 16);
+        const uint32_t in_row = __ballot_sync(0xffffffffu, slot == first + (lane & 15));
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv, ++n) {
+          const int s = n % SSLOTS;
+          ok = sa_wait(&kv_empty[s], ((n / SSLOTS) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
+          if (!ok) break;
+          const CUtensorMap *box = kv ? &maps.v16 : &maps.k16, *one = kv ? &maps.v1 : &maps.k1;
+          if (elect_one()) mbar_expect_tx(&kv_full[s], 32 * 256);
+          __syncwarp();
+#pragma unroll
+          for (int part = 0; part < 2; ++part) {
+            const uint32_t dst = smem_u32(sKV + s * kSTile) + (32 * lw + 16 * part) * 128;
+            if (((in_row >> (16 * part)) & 0xffffu) == 0xffffu) {
+              const int y = row0 + __shfl_sync(0xffffffffu, slot, 16 * part);
+              if (elect_one()) {
+                sa_tma_box(dst, box, &kv_full[s], 0, y);
+                sa_tma_box(dst + SKEYS * 128, box, &kv_full[s], 64, y);
+              }
+            } else {
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                int y[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) y[e] = row0 + __shfl_sync(0xffffffffu, slot, 16 * part + 4 * g + e);
+                if (elect_one()) {
+                  sa_tma_rows(dst + g * 512, one, &kv_full[s], 0, y[0], y[1], y[2], y[3]);
+                  sa_tma_rows(dst + g * 512 + SKEYS * 128, one, &kv_full[s], 64, y[0], y[1], y[2], y[3]);
+                }
+                __syncwarp();
+              }
+            }
+            __syncwarp();
+          }
+        }
+      }
+      sa_done(w);
+    }
+  } else if (warp == 8) {
+    // ================================================================ MMA issuer: QK of job n + 2 goes behind PV of job n
+    constexpr uint32_t idesc_qk = umma_idesc_bf16(SROWS, SKEYS), idesc_pv = umma_idesc_bf16(SROWS, SD) | (1u << 16);
+    const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ)), k_desc = umma_desc_sw128(smem_u32(sKV)), v_desc = sa_desc_mn(smem_u32(sKV), SKEYS * 128);
+    struct Cursor { SaWalk w; int job, tile0, q0; bool more; };      // job within the segment; K/V tiles and Q buffers before it
+    auto open = [&](Cursor& c) { c.job = 0; c.more = sa_next(p, c.w); };
+    auto step = [&](Cursor& c) {                                      // behind the current job
+      if (++c.job < c.w.nt * (c.w.two ? 2 : 1)) return;
+      c.tile0 += c.w.nt;
+      c.q0 += c.w.two ? 2 : 1;
+      sa_done(c.w);
+      open(c);
+    };
+    auto tile_of = [&](const Cursor& c) { return c.tile0 + (c.w.two ? c.job >> 1 : c.job); };
+    Cursor qk{w, 0, 0, 0, false}, pv{w, 0, 0, 0, false};
+    open(qk);
+    open(pv);
+    int nq = 0, np = 0;                         // jobs issued
+    bool ok = true;
+    auto issue_qk = [&] {
+      const int jobs = qk.w.nt * (qk.w.two ? 2 : 1), side = qk.w.two ? qk.job & 1 : 0, use = qk.q0 + side, buf = use & 1, g = nq & 1;
+      if (qk.job <= side && !sa_wait(&q_full[buf], (use >> 1) & 1, p.status, kTimeoutFull, gave_up)) return false;
+      const int n = 2 * tile_of(qk), s = n % SSLOTS;
+      if (!sa_wait(&kv_full[s], (n / SSLOTS) & 1, p.status, kTimeoutFull, gave_up)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t a = q_desc + static_cast<uint64_t>(buf * (kSTile >> 4)), b = k_desc + static_cast<uint64_t>(s * (kSTile >> 4));
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_f16(tmem + g * SKEYS, a + (k >> 2) * (SROWS * 128 >> 4) + 2 * (k & 3), b + (k >> 2) * (SKEYS * 128 >> 4) + 2 * (k & 3), idesc_qk, k != 0);
+        if (!qk.w.two || side == 1) umma_commit(&kv_empty[s]);
+        if (qk.job + (qk.w.two ? 2 : 1) >= jobs) umma_commit(&q_empty[buf]);
+        umma_commit(&s_full[g]);
+      }
+      __syncwarp();
+      ++nq;
+      step(qk);
+      return true;
+    };
+    auto issue_pv = [&] {
+      const int jobs = pv.w.nt * (pv.w.two ? 2 : 1), g = np & 1, n = 2 * tile_of(pv) + 1, s = n % SSLOTS;
+      if (!sa_wait(&kv_full[s], (n / SSLOTS) & 1, p.status, kTimeoutFull, gave_up)) return false;
+      if (!sa_wait(&p_full[g], (np >> 1) & 1, p.status, kTimeoutAccum, gave_up)) return false;
+      tc_fence_after();
+      if (elect_one()) {
+        const uint64_t b = v_desc + static_cast<uint64_t>(s * (kSTile >> 4));
+#pragma unroll
+        for (int k = 0; k < SKEYS / 16; ++k)
+          sa_mma_tmem_a(tmem + 256 + g * SD, tmem + g * SKEYS + k * 8, b + k * (2048 >> 4), idesc_pv, k != 0 || pv.job >= 2);
+        if (!pv.w.two || (pv.job & 1)) umma_commit(&kv_empty[s]);
+        if (pv.job + 2 >= jobs) umma_commit(&o_full[g]);
+      }
+      __syncwarp();
+      ++np;
+      step(pv);
+      return true;
+    };
+    while (ok && qk.more && nq < 2) ok = issue_qk();
+    while (ok && pv.more) {
+      ok = issue_pv();
+      if (ok && qk.more) ok = issue_qk();
+    }
+  } else {
+    // ================================================================ softmax and epilogue: one row a thread
+    const int g = warp >> 2, row = (warp & 3) * 32 + lane, tok = row / p.G, sub = row % p.G;
+    const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + t_lane + g * SKEYS, to = tmem + t_lane + 256 + g * SD;
+    int jobs_done = 0, segs_done = 0;           // of this group: phases of its barriers
+    bool ok = true;
+    while (ok && sa_next(p, w)) {
+      const bool prefix = w.b < 0;
+      const int rel = g ^ w.group0, side = w.two ? rel : 0;
+      const int node = (w.pair * 2 + side) * p.npt + tok, head = w.h * p.G + sub;
+      const bool valid = tok < p.npt && node < w.s.n;
+      const int end = sa_end(p, w.s, w.b, w.pair);
+      const int* bits = !p.causal && valid && !prefix ? p.mask_bits + static_cast<size_t>(w.s.q_begin + node) * p.W : nullptr;
+      float m_run = -INFINITY, l_run = 0.f;
+      int jobs = 0;
+      for (int i = w.two ? 0 : rel; i < w.nt && ok; i += w.two ? 1 : 2, ++jobs, ++jobs_done) {
+        const int k0 = w.s.first + (w.t + i) * SKEYS;
+        uint32_t vis[4] = {0u, 0u, 0u, 0u};
+        const bool all = k0 + SKEYS <= min(w.s.past, end);      // the same for all rows of the item
+        if (!all && valid) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) vis[c] = sa_visible(p, w.s, prefix, end, node, bits, k0 + 32 * c);
+        }
+        ok = sa_wait(&s_full[g], jobs_done & 1, p.status, kTimeoutAccum, gave_up);
+        if (!ok) break;
+        tc_fence_after();
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t sr[32];
+          tmem_ld_32x32(ts + 32 * c, sr);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            mx4[j & 3] = fmaxf(mx4[j & 3], all || ((vis[c] >> j) & 1u) ? __uint_as_float(sr[j]) : -INFINITY);
+        }
+        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+        // integer running maximum in the log2 domain: probabilities are exact powers of two apart whatever the pieces
+        const float m_new = fmaxf(m_run, ceilf(mx)), m_safe = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = exp2f(m_run - m_safe);
+        m_run = m_new;
+        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          uint32_t sr[32], pr[16];
+          tmem_ld_32x32(ts + 32 * c, sr);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float p0 = sa_exp2(fmaf(__uint_as_float(sr[j]), p.scale_log2, -m_safe)), p1 = sa_exp2(fmaf(__uint_as_float(sr[j + 1]), p.scale_log2, -m_safe));
+            if (!all) {
+              if (!((vis[c] >> j) & 1u)) p0 = 0.f;
+              if (!((vis[c] >> (j + 1)) & 1u)) p1 = 0.f;
+            }
+            sum4[(j >> 1) & 3] += p0 + p1;
+            const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);      // the MMA's operand: bf16, the sum keeps fp32
+            pr[j >> 1] = *reinterpret_cast<const uint32_t*>(&v);
+          }
+          sa_tmem_st16(ts + 16 * c, pr);        // over scores that are read already
+        }
+        l_run = l_run * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+        // every earlier PV of this group ended before these scores did
+        if (__any_sync(0xffffffffu, jobs > 0 && alpha != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < SD; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(to + c, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            sa_tmem_st32(to + c, o);
+          }
+        }
+        sa_tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[g]);
+      }
+      if (!ok) break;
+      // ---- the segment's result: the output where this CTA saw all keys of the rows, else a part
+      const int item = sa_item(p, w.s, w.b, w.pair, w.h);
+      const bool direct = w.two && w.nt == w.units && !prefix && p.prefix == 0;
+      const int rows = prefix ? SROWS : p.seq_rows_kept;
+      const size_t seg = static_cast<size_t>(blockIdx.x) + (prefix ? item : item - p.prefix_items);
+      const size_t at = (seg * 2 + rel) * rows + row;
+      if (jobs > 0) {
+        ok = sa_wait(&o_full[g], segs_done & 1, p.status, kTimeoutAccum, gave_up);
+        if (!ok) break;
+        ++segs_done;
+        tc_fence_after();
+        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+#pragma unroll 1
+        for (int c = 0; c < SD; c += 32) {
+          uint32_t o[32];
+          tmem_ld_32x32(to + c, o);
+          tmem_ld_wait();
+          if (!valid) continue;
+          if (direct) {
+            uint4 pk[4];
+            __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(pk);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o2[j] = __floats2bfloat162_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
+            uint4* dst = reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(w.s.q_begin + node) * p.Hq + head) * SD + c);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[j] = pk[j];
+          } else if (row < rows) {
+            float4* dst = reinterpret_cast<float4*>((prefix ? p.po : p.so) + at * SD + c);
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+          }
+        }
+      }
+      if (valid && !direct) {
+        if (row < rows) (prefix ? p.pml : p.sml)[at] = make_float2(m_run, l_run);
+        else report(p.status, kRowsOverflow);   // more rows in a sequence than the caller's bound
+      }
+      sa_done(w);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Joins the parts of a row: a warp each (token, head), four columns a lane.
+__global__ void __launch_bounds__(256) attn_shared_merge_kernel(const SharedAttn p) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const int at = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+  if (at >= p.T * p.Hq) return;
+  const int t = at / p.Hq, head = at % p.Hq, h = head / p.G, sub = head % p.G;
+  int b = -1;                                  // sequences that begin at or before the token, the last of them that has it
+  for (int base = 0; base < p.B; base += 32) {
+    const bool before = base + lane < p.B && p.cu_q[base + lane] <= t;
+    const unsigned some = __ballot_sync(0xffffffffu, before);
+    b += __popc(some);
+    if (some != 0xffffffffu) break;
+  }
+  __nv_bfloat16* out = p.out + static_cast<size_t>(at) * SD + lane * 4;
+  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+  const int total = p.plan[0];
+  auto join = [&](const float* o, const float2* ml, size_t row) {
+    const float2 v = ml[row];
+    if (v.y == 0.f) return;                    // no visible key (the part's output may be unwritten)
+    const float m_new = fmaxf(m, v.x), safe = m_new == -INFINITY ? 0.f : m_new;      // NaN scores leave a sum without a maximum
+    const float old = exp2f(m - safe), add = exp2f(v.x - safe);
+    const float4 x = *reinterpret_cast<const float4*>(o + row * SD + lane * 4);
+    acc[0] = acc[0] * old + x.x * add;
+    acc[1] = acc[1] * old + x.y * add;
+    acc[2] = acc[2] * old + x.z * add;
+    acc[3] = acc[3] * old + x.w * add;
+    l = l * old + v.y * add;
+    m = m_new;
+  };
+  bool done = false;
+  for (int part = p.prefix > 0 ? 0 : 1; part < 2 && b >= 0; ++part) {
+    const int seq = part == 0 ? -1 : b;
+    const SaSeq s = sa_seq(p, seq);
+    const int node = t - s.q_begin, tile = node / p.npt, pair = tile >> 1;
+    if (node < 0 || node >= s.n) continue;     // behind the last sequence
+    const int units = sa_units(p, s, seq, pair);
+    if (units == 0) continue;
+    const int item = sa_item(p, s, seq, pair, h), u = p.plan[1 + item];
+    const int c0 = sa_cta(p, u, total), c1 = sa_cta(p, u + units - 1, total);
+    const bool two = s.n - pair * 2 * p.npt > p.npt;
+    if (two && c0 == c1 && part == 1 && p.prefix == 0) { done = true; break; }
+    const int rows = part == 0 ? SROWS : p.seq_rows_kept, row = (node - tile * p.npt) * p.G + sub;
+    if (row >= rows) continue;
+    for (int c = c0; c <= c1; ++c) {
+      const size_t seg = (static_cast<size_t>(c) + (part == 0 ? item : item - p.prefix_items)) * 2;
+      for (int side = two ? tile & 1 : 0; side < (two ? (tile & 1) + 1 : 2); ++side)
+        join(part == 0 ? p.po : p.so, part == 0 ? p.pml : p.sml, (seg + side) * rows + row);
+    }
+  }
+  if (done) return;                            // written by its CTA
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
+  *reinterpret_cast<__nv_bfloat162*>(out + 2) = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+}
+
+static long long shared_round(long long bytes) { return (bytes + 255) / 256 * 256; }
+
+// What a launch lays out in its workspace; returns the bytes.
+static long long shared_layout(SharedAttn* p, uint8_t* ws, int max_q) {
+  const int pair_rows = 2 * p->npt;
+  p->prefix_items = p->prefix > 0 ? (p->T + pair_rows - 1) / pair_rows * p->Hkv : 0;
+  p->seq_items = (p->T / pair_rows + p->B + 1) * p->Hkv;
+  p->seq_rows_kept = max_q >= p->npt ? SROWS : max_q * p->G;
+  const long long prefix_rows = p->prefix > 0 ? 2ll * SROWS * (p->ctas + p->prefix_items) : 0;
+  const long long rows = 2ll * p->seq_rows_kept * (p->ctas + p->seq_items);
+  long long at = 0;
+  auto take = [&](long long bytes) { uint8_t* r = ws + at; at += shared_round(bytes); return r; };
+  p->plan = reinterpret_cast<int*>(take(4ll * (1 + p->prefix_items + p->seq_items)));
+  p->pml = reinterpret_cast<float2*>(take(8 * prefix_rows));
+  p->sml = reinterpret_cast<float2*>(take(8 * rows));
+  p->po = reinterpret_cast<float*>(take(4 * SD * prefix_rows));
+  p->so = reinterpret_cast<float*>(take(4 * SD * rows));
+  return at;
+}
+
+// Attending to the prefix for all rows together pays where sequences leave much of their own tiles empty.
+static bool shared_pays(int B, int T, int max_q, int G, int npt) {
+  (void)G;
+  const long long own = static_cast<long long>(B) * ((max_q + npt - 1) / npt), together = (T + npt - 1) / npt;
+  return 4 * together <= 3 * own;
+}
+
+static int shared_setup(SharedAttn* p, int max_q, int prefix_len, int ctas) {
+  if (p->B < 0 || p->T < 0 || p->Hkv < 1 || p->Hq < 1 || p->Hq % p->Hkv || prefix_len < 0 || prefix_len > p->max_len || max_q < 1 || ctas < 1) return -10;
+  p->G = p->Hq / p->Hkv;
+  if (p->G > SROWS) return -11;
+  p->npt = SROWS / p->G;
+  p->ctas = ctas;
+  const bool shared = prefix_len > 0 && shared_pays(p->B, p->T, max_q, p->G, p->npt);
+  p->prefix = shared ? prefix_len : 0;
+  p->first_key = shared ? prefix_len : 0;
+  return 0;
+}
+
+}  // namespace js
+
+// Bytes of workspace that js_shared_attention wants for these sizes; negative: refused.
+extern "C" long long js_shared_attention_ws(int B, int T, int Hq, int Hkv, int max_len, int prefix_len, int max_q, int ctas) {
+  using namespace js;
+  SharedAttn p{};
+  p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.max_len = max_len;
+  const int rc = shared_setup(&p, max_q, prefix_len, ctas);
+  return rc != 0 ? rc : shared_layout(&p, nullptr, max_q);
+}
+
+// q (T, Hq, 128) bf16, ldq elements between tokens; pools (Hkv, S, 128); slot_map (max_seqs, max_len); seq_rows, past_lens (B); cu_q (B + 1);
+// mask_bits (T, W), or null when causal; out (T, Hq * 128).  Positions [0, prefix_len) hold the same slots in all rows of the slot map that
+// are named; max_q bounds a sequence's rows.  ws: js_shared_attention_ws bytes.
+extern "C" int js_shared_attention(const void* q, long long ldq, const void* k_pool, const void* v_pool, const int* slot_map, const int* seq_rows,
+                                   const int* cu_q, const int* past_lens, const int* mask_bits, void* out, void* ws, long long ws_bytes,
+                                   int* status, int B, int T, int Hq, int Hkv, int S, int max_seqs, int max_len, int W, int causal, float scale,
+                                   int prefix_len, int max_q, int ctas, cudaStream_t stream) {
+  using namespace js;
+  if (T == 0 || B == 0) return 0;
+  SharedAttn p{};
+  p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.max_len = max_len;
+  if (const int rc = shared_setup(&p, max_q, prefix_len, ctas)) return rc;
+  if (ldq % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15)) return -12;
+  if (!causal && (mask_bits == nullptr || W < 1)) return -13;
+  if (!(scale > 0.f) || S < 1 || max_seqs < 1) return -10;
+  if (shared_layout(&p, reinterpret_cast<uint8_t*>(ws), max_q) > ws_bytes) return -14;
+  p.q = reinterpret_cast<const __nv_bfloat16*>(q);
+  p.ldq = ldq;
+  p.slot_map = slot_map; p.seq_rows = seq_rows; p.cu_q = cu_q; p.past_lens = past_lens; p.mask_bits = mask_bits;
+  p.out = reinterpret_cast<__nv_bfloat16*>(out);
+  p.status = status;
+  p.S = S; p.max_seqs = max_seqs; p.W = W; p.causal = causal;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  SharedMaps maps;
+  const uint64_t rows = static_cast<uint64_t>(Hkv) * S;
+  if (rows >= (1ull << 31) || make_map(&maps.k16, k_pool, rows, SD, SD, 16) || make_map(&maps.v16, v_pool, rows, SD, SD, 16) ||
+      make_map(&maps.k1, k_pool, rows, SD, SD, 1) || make_map(&maps.v1, v_pool, rows, SD, SD, 1)) return -15;
+  static int configured[kMaxDevicesCached] = {};
+  if (ensure_dyn_smem(attn_shared_kernel, kSharedSmem, configured) != 0) return -3;
+  attn_shared_kernel<<<ctas, STHREADS, kSharedSmem, stream>>>(p, maps);
+  if (cudaGetLastError() != cudaSuccess) return -4;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((T * Hq + 7) / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attn_shared_merge_kernel, p) == cudaSuccess ? 0 : -5;
+}

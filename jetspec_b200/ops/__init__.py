@@ -234,6 +234,9 @@ def paged_tree_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens,
 
 def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale, prefix_len,
                             causal: bool = False, max_q: Optional[int] = None):
+    if _kern(q) and q.shape[-1] == 128 and q.shape[1] // k_pool.shape[0] <= 128:
+        return _ext().shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, float(scale),
+                                              int(prefix_len), bool(causal), int(max_q if max_q is not None else q.shape[0]))
     return ref.shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale, prefix_len, causal)
 
 

@@ -182,7 +182,7 @@ STATUS_NAMES = {0: "ok", 1: "timeout waiting for a TMA stage", 2: "timeout waiti
                 10: "all-reduce tail: a slice owner's result cells never arrived",
                 11: "vocabulary-parallel top-k: a rank's record never arrived",
                 12: "expert-parallel dispatch: more rows for one expert than the grouped launch covers",
-                13: "slot plan: the free pages ran out", 14: "slot plan: more new rows than the row buffers hold",
+                13: "slot plan: the free pages ran out", 14: "more new rows than the caller's bound",
                 15: "drafted token outside the vocabulary"}
 
 
@@ -1457,6 +1457,59 @@ def moe_forward(x, gate_w, w_gate_up, w_down, top_k: int, renorm: bool, router_l
 
 
 # ------------------------------------------------------------------ a batched serving step
+def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale: float, prefix_len: int,
+                            causal: bool, max_q: int, out: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None):
+    """See :func:`jetspec_b200.ops.reference.shared_prefix_attention` for the contract.  bf16, heads of 128; ``max_q`` bounds a sequence's
+    rows; ``q`` may be a view whose tokens lie further apart.  ``ws`` (uint8, :func:`shared_prefix_workspace` bytes) and ``out`` keep a
+    captured launch's buffers outside; a workspace serves one launch at a time."""
+    dev = q.device
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale, prefix_len, causal, max_q,
+                                           out, ws)
+    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == 128, f"q {tuple(q.shape)} {q.dtype}: expected (T, Hq, 128) in bf16")
+    T, Hq, _ = q.shape
+    _need(k_pool.dim() == 3 and k_pool.shape == v_pool.shape and k_pool.shape[2] == 128 and k_pool.dtype == v_pool.dtype == torch.bfloat16
+          and k_pool.is_contiguous() and v_pool.is_contiguous() and k_pool.device == v_pool.device == dev,
+          "pools: expected contiguous bf16 (Hkv, S, 128) tensors on the queries' device")
+    Hkv, S, _ = k_pool.shape
+    _need(Hkv >= 1 and S >= 1 and Hq >= 1 and Hq % Hkv == 0 and Hq // Hkv <= 128 and Hkv * S < 2 ** 31, f"{Hq} query and {Hkv} KV heads over {S} slots")
+    causal = bool(causal)
+    _ints(dev, slot_map=slot_map, seq_rows=seq_rows, cu_q=cu_q, past_lens=past_lens, **({} if causal or mask_bits is None else {"mask_bits": mask_bits}))
+    B, (max_seqs, max_len) = seq_rows.numel(), slot_map.shape
+    _need(cu_q.numel() == B + 1 and past_lens.numel() == B and max_seqs >= 1, f"{B} sequences: cu_q {cu_q.numel()}, past_lens {past_lens.numel()}")
+    _need(causal or (mask_bits is not None and mask_bits.dim() == 2 and mask_bits.shape[0] == T and mask_bits.shape[1] >= 1),
+          "mask_bits: a row of words for every query is needed without the causal rule")
+    _need(0 <= prefix_len <= max_len and max_q >= 1 and scale > 0.0, f"prefix_len={prefix_len}, max_q={max_q}, scale={scale}")
+    if q.stride(2) != 1 or q.stride(1) != 128 or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    if out is None:
+        out = torch.empty(T, Hq * 128, dtype=q.dtype, device=dev)
+    _need(out.shape == (T, Hq * 128) and out.dtype == q.dtype and out.is_contiguous() and out.device == dev and out.data_ptr() % 16 == 0,
+          "out: expected a contiguous (T, Hq * 128) bf16 tensor")
+    if T == 0 or B == 0:
+        return out.zero_()
+    need = shared_prefix_workspace(B, T, Hq, Hkv, max_len, prefix_len, max_q)
+    if ws is None:
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    _need(ws.dtype == torch.uint8 and ws.is_contiguous() and ws.device == dev and ws.numel() >= need and ws.data_ptr() % 16 == 0,
+          f"ws: expected {need} bytes on {dev}")
+    _check(load().js_shared_attention(
+        _p(q), ctypes.c_longlong(q.stride(0)), _p(k_pool), _p(v_pool), _p(slot_map), _p(seq_rows), _p(cu_q), _p(past_lens), _p(mask_bits), _p(out),
+        _p(ws), ctypes.c_longlong(ws.numel()), _p(status_word(dev)), B, T, Hq, Hkv, S, max_seqs, max_len,
+        0 if causal else mask_bits.shape[1], int(causal), ctypes.c_float(scale), prefix_len, max_q, SM_COUNT, _stream()), "js_shared_attention")
+    return out
+
+
+def shared_prefix_workspace(B: int, T: int, Hq: int, Hkv: int, max_len: int, prefix_len: int, max_q: int) -> int:
+    """Bytes of workspace that :func:`shared_prefix_attention` wants for these sizes."""
+    fn = load().js_shared_attention_ws
+    fn.restype = ctypes.c_longlong
+    n = fn(B, T, Hq, Hkv, max_len, prefix_len, max_q, SM_COUNT)
+    _check(min(n, 0), "js_shared_attention_ws")
+    return n
+
+
 def _need(ok: bool, what: str) -> None:
     if not ok:
         raise ValueError(what)

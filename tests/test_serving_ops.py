@@ -288,3 +288,124 @@ def test_verify_chains_refusals():
     kernel_refuses(lambda: call(temperature=-1.0), "temperature")
     kernel_refuses(lambda: call(temperature=torch.ones(3)), "temperature")
     kernel_refuses(lambda: call(draft_temperature=torch.ones(2, dtype=torch.float64)), "draft_temperature")
+
+
+# ------------------------------------------------------------------ attention behind a shared prefix
+def tree_bits(counts, gen, words):
+    """Ancestor bits of random trees; some rows see nothing of their tree, not even themselves."""
+    rows = []
+    for n in counts:
+        seen = torch.zeros(n, n, dtype=torch.bool)
+        for i in range(n):
+            if i:
+                seen[i] = seen[int(torch.randint(max(0, i - 7), i, (1,), generator=gen))]
+            seen[i, i] = True
+        seen[torch.rand(n, generator=gen) < 0.1] = False
+        rows.append(ref.pack_ancestor_bits(seen, words))
+    return torch.cat(rows) if rows else torch.zeros(0, words, dtype=I32)
+
+
+def attention_case(seed, heads, kv_heads, prefix, behind, counts, causal, page=16, dim=128, dtype=torch.bfloat16, device="cpu",
+                   more_rows=0, slack=2.0):
+    """A pool of random pages whose first ``prefix`` positions all sequences share; slots that no position uses hold NaN."""
+    g = torch.Generator().manual_seed(seed)
+    B, T = len(counts), sum(counts) + more_rows
+    most = prefix + max(b + c for b, c in zip(behind, counts)) + page
+    columns, whole, shared = -(-most // page), prefix // page, -(-prefix // page)
+    pages = torch.randperm(int(slack * (shared + B * columns)) + 1, generator=g)
+    table = torch.empty(B, columns, dtype=torch.long)
+    table[:, :whole] = pages[:whole]
+    table[:, whole:] = pages[shared:shared + B * (columns - whole)].view(B, columns - whole)
+    pos = torch.arange(columns * page)
+    slot_map = table[:, pos // page] * page + pos % page
+    slot_map[:, :prefix] = pages[pos[:prefix] // page] * page + pos[:prefix] % page
+    for b in range(0, B, 2):          # a committed path trades slots inside a sequence
+        n = prefix + behind[b]
+        slot_map[b, prefix:n] = slot_map[b, prefix:n][torch.randperm(behind[b], generator=g)]
+    S = pages.numel() * page
+    used = torch.zeros(S, dtype=torch.bool)
+    for b in range(B):
+        used[slot_map[b, :prefix + behind[b] + counts[b]]] = True
+    make = lambda *s: torch.randn(*s, generator=g).to(dtype)
+    pools = [make(kv_heads, S, dim) for _ in "kv"]
+    for x in pools:
+        x[:, ~used] = math.nan
+    spare = torch.full((1, slot_map.shape[1]), S + 5)
+    words = max(1, -(-max(counts) // 32)) + 1
+    bits = None
+    if not causal:
+        bits = torch.cat((tree_bits(counts, g, words), torch.full((more_rows, words), -1, dtype=I32)))
+    out = dict(q=make(T, heads, dim) * 1.5, k_pool=pools[0], v_pool=pools[1], slot_map=torch.cat((spare, slot_map)).to(I32),
+               seq_rows=torch.arange(1, B + 1).to(I32), cu_q=torch.tensor([0] + torch.tensor(counts).cumsum(0).tolist(), dtype=I32),
+               past_lens=torch.tensor([prefix + b for b in behind], dtype=I32), mask_bits=bits, scale=dim ** -0.5, prefix_len=prefix, causal=causal)
+    return {k: v.to(device) if torch.is_tensor(v) else v for k, v in out.items()}
+
+
+def attention_exact(c):
+    """The definition in 64 bits; rows that see no key, and rows behind the last sequence, are zero."""
+    q, hkv = c["q"].double(), c["k_pool"].shape[0]
+    T, hq, dim = q.shape
+    out = torch.zeros(T, hq, dim, dtype=torch.float64, device=q.device)
+    cu, past = c["cu_q"].tolist(), c["past_lens"].tolist()
+    for b, row in enumerate(c["seq_rows"].tolist()):
+        s, e = cu[b], cu[b + 1]
+        slots = c["slot_map"][row, :past[b] + e - s].long()
+        for i in range(s, e):
+            own = torch.arange(e - s, device=q.device) <= i - s if c["causal"] else ref.unpack_ancestor_bits(c["mask_bits"][i:i + 1], e - s)[0]
+            keys = slots[torch.cat((torch.ones(past[b], dtype=torch.bool, device=q.device), own))]
+            if keys.numel():
+                k, v = (c[x][:, keys].double().repeat_interleave(hq // hkv, 0) for x in ("k_pool", "v_pool"))
+                out[i] = torch.einsum("hl,hld->hd", torch.softmax(torch.einsum("hd,hld->hl", q[i], k) * c["scale"], -1), v)
+    return out.view(T, hq * dim)
+
+
+def attend(c, **kw):
+    return ops.shared_prefix_attention(c["q"], c["k_pool"], c["v_pool"], c["slot_map"], c["seq_rows"], c["cu_q"], c["past_lens"], c["mask_bits"],
+                                       c["scale"], c["prefix_len"], causal=c["causal"], **kw)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("prefix,behind,counts", [(20, [0, 5, 3], [4, 1, 7]), (0, [0, 2], [3, 1]), (1, [0], [1]), (17, [2, 0, 0], [1, 0, 2])])
+def test_shared_prefix_attention_by_definition(causal, prefix, behind, counts):
+    c = attention_case(prefix, 4, 2, prefix, behind, counts, causal, page=4, dim=16, dtype=torch.float32, more_rows=2)
+    assert torch.allclose(attend(c).double(), attention_exact(c), atol=1e-5)
+    c["slot_map"][2:, :prefix] = 10 ** 6          # the prefix is read through the first sequence's row alone
+    assert torch.allclose(attend(c).double(), attention_exact({**c, "slot_map": torch.cat((c["slot_map"][:2], torch.cat(
+        (c["slot_map"][1:2, :prefix].expand(len(counts) - 1, prefix), c["slot_map"][2:, prefix:]), 1)))}), atol=1e-5)
+
+
+# Rounding: probabilities become bf16 ahead of the second product (half a step is 2^-8 of each; they add up at random, and never to more than
+# 2^-8 of the largest |v|, below 6 here, whatever the weights), the result once more (2^-8 of itself).  Sums and scores are fp32.
+def attention_close(got, want, v_max=6.0):
+    err = (got.double() - want).abs()
+    assert bool((err <= 2 ** -8 * (v_max + want.abs())).all()), float(err.max())
+    assert float(err.norm()) <= 5e-3 * float(want.norm()) + 1e-9
+
+
+ATTENTION = [  # query heads, KV heads, prefix, committed behind it, new rows
+    (32, 8, 1024, [3, 40, 17, 0], [1, 1, 1, 1]),
+    (32, 8, 1000, [i * 7 % 90 for i in range(40)], [1] * 40),
+    (8, 8, 300, [5], [1]),
+    (16, 2, 130, [0, 1, 400], [16, 17, 15]),
+    (12, 4, 257, [10, 0, 33], [40, 90, 3]),
+    (10, 2, 77, [0, 200], [25, 26]),
+    (64, 4, 128, [100, 3, 0, 9, 50], [8, 9, 1, 0, 30]),
+    (4, 1, 1, [0, 0], [33, 1]),
+    (32, 4, 0, [0, 130, 700], [70, 1, 128]),
+    (2, 1, 5000, [0, 1], [2, 1]),
+    (128, 1, 200, [7, 300], [3, 1]),
+    (32, 8, 500, [20, 30, 0], [130, 0, 64]),
+    (16, 8, 2000, [100] * 12, [3, 1, 2] * 4),
+    (8, 1, 40, [9], [300]),
+]
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads,kv,prefix,behind,counts", ATTENTION)
+def test_shared_prefix_attention_kernel(clean, heads, kv, prefix, behind, counts, causal):
+    c = attention_case(prefix + heads, heads, kv, prefix, behind, counts, causal, device="cuda", more_rows=3)
+    want = attention_exact(c)
+    got = attend(c, max_q=max(1, max(counts)))
+    attention_close(got, want)
+    attention_close(attend(c), want)      # without a bound on the rows
