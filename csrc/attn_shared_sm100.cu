@@ -10,14 +10,15 @@
 // item's units in key order.  Every CTA takes an equal piece of the line, so lengths, which only the device knows, balance by
 // themselves; where a piece begins or ends inside an item its parts go through a workspace and attn_shared_merge_kernel.
 //
-// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warp 8 issues the MMAs, warps 9-12 load K and V by TMA (boxes of 16 rows where
-// slots follow one another, gathers of four rows where not), warps 13-14 load Q.  A job is one row tile against 128 keys; jobs alternate between the
+// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warp 8 issues the MMAs, warps 9-10 load K and V by TMA (boxes of 16 rows where
+// slots follow one another, gathers of four rows where not), warp 11 loads Q.  A job is one row tile against 128 keys; jobs alternate between the
 // groups: the two tiles of a pair on the same keys, or, for a single tile, every other block of keys.  Scores (128 columns) and
 // output (128 columns) of both groups fill the 512 columns of tensor memory; probabilities overwrite the scores as bf16 and are the second
 // MMA's A operand there.  Every wait is bounded (status word).
 #include "gemm_common.cuh"
 
 #include <math.h>
+#include <algorithm>
 
 namespace js {
 
@@ -26,7 +27,7 @@ constexpr int SROWS = 128;           // rows of a tile
 constexpr int SKEYS = 128;           // keys of a unit
 constexpr int SSLOTS = 5;            // ring of K and V tiles, in turn
 constexpr int kSTile = 128 * 256;    // bytes of a K, V or Q tile: 2 halves x 128 rows x 128 B
-constexpr int SWARPS = 15, STHREADS = 32 * SWARPS;
+constexpr int SWARPS = 12, STHREADS = 32 * SWARPS;      // 168 registers a thread
 constexpr int kSharedSmem = (2 + SSLOTS) * kSTile + 512 + 1024;
 
 struct SharedAttn {
@@ -48,6 +49,7 @@ struct SharedAttn {
 struct SharedMaps {
   CUtensorMap k16, v16;        // boxes of 16 rows x 64 columns
   CUtensorMap k1, v1;          // boxes of one row, for gathers
+  CUtensorMap q;               // boxes of npt tokens x G heads x 64 columns
 };
 
 JS_DEVICE int sa_wait(uint64_t* bar, uint32_t parity, int* status, int code, uint32_t* gave_up) {
@@ -163,8 +165,27 @@ JS_DEVICE float sa_exp2(float x) {      // denormal results flush to zero; exp2(
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-JS_DEVICE void sa_cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+// two fp32 in a register pair: half as many instructions
+JS_DEVICE uint64_t sa_pack(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+JS_DEVICE void sa_unpack(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+JS_DEVICE uint64_t sa_fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+JS_DEVICE uint64_t sa_add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+JS_DEVICE void sa_tma_heads(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int head, int token) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(bar)), "r"(x), "r"(head), "r"(token) : "memory");
 }
 JS_DEVICE void sa_tma_box(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int y) {
   asm volatile(
@@ -225,9 +246,9 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
 
   // ---- this CTA's piece of the line
   if (tid == 0) {
-    for (int s = 0; s < SSLOTS; ++s) { mbar_init(&kv_full[s], 4); mbar_init(&kv_empty[s], 1); }
+    for (int s = 0; s < SSLOTS; ++s) { mbar_init(&kv_full[s], 2); mbar_init(&kv_empty[s], 1); }
     for (int g = 0; g < 2; ++g) {
-      mbar_init(&q_full[g], 64);
+      mbar_init(&q_full[g], 1);
       mbar_init(&q_empty[g], 1);
       mbar_init(&s_full[g], 1);
       mbar_init(&p_full[g], 128);
@@ -237,15 +258,36 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     fence_barrier_init();
   }
   int* scan = start + 8;                        // a total per warp
+  volatile int* segs = start + 8 + SWARPS;      // the MMA warp's
   const int prefix_units = p.prefix > 0 ? sa_total(p, -1) * p.Hkv : 0;
-  int mine = 0;
-  for (int b = tid; b < p.B; b += STHREADS) mine += sa_total(p, b) * p.Hkv;
+  // units of the sequences ahead of this thread's (of every 384), and of all of them
+  auto ahead = [&](int value, int& all) {
+    int inc = value;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) scan[warp] = mine;
-  __syncthreads();
-  int total = prefix_units;
-  for (int w = 0; w < SWARPS; ++w) total += scan[w];
+    for (int o = 1; o < 32; o <<= 1) {
+      const int other = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += other;
+    }
+    __syncthreads();
+    if (lane == 31) scan[warp] = inc;
+    __syncthreads();
+    int before = inc - value;
+    all = 0;
+    for (int i = 0; i < SWARPS; ++i) {
+      if (i < warp) before += scan[i];
+      all += scan[i];
+    }
+    return before;
+  };
+  const int mine = tid < p.B ? sa_total(p, tid) * p.Hkv : 0;
+  int total;
+  const int mine_ahead = ahead(mine, total);
+  for (int base = STHREADS; base < p.B; base += STHREADS) {
+    int all;
+    ahead(base + tid < p.B ? sa_total(p, base + tid) * p.Hkv : 0, all);
+    total += all;
+  }
+  total += prefix_units;
   const int u0 = sa_start(p, blockIdx.x, total), u1 = sa_start(p, blockIdx.x + 1, total);
   if (u0 < prefix_units) {
     if (tid == 0) {
@@ -259,21 +301,14 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   } else if (u0 < u1) {
     int run = prefix_units;
     for (int base = 0; base < p.B; base += STHREADS) {
-      const int b = base + tid, v = b < p.B ? sa_total(p, b) * p.Hkv : 0;
-      int inc = v;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int other = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += other;
+      const int b = base + tid;
+      int v = mine, before = mine_ahead, all = 0;
+      if (p.B > STHREADS) {
+        v = b < p.B ? sa_total(p, b) * p.Hkv : 0;
+        before = ahead(v, all);
       }
-      __syncthreads();
-      if (lane == 31) scan[warp] = inc;
-      __syncthreads();
-      int before = run + inc - v;
-      for (int w = 0; w < SWARPS; ++w) {
-        if (w < warp) before += scan[w];
-        run += scan[w];
-      }
+      before += run;
+      run += all;
       if (u0 >= before && u0 < before + v) {
         const SaSeq s = sa_seq(p, b);
         int pair = 0, at = u0 - before;
@@ -306,35 +341,33 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   w.parity = 0;
   sa_begin(p, w);
 
-  if (warp >= 13) {
-    // ================================================================ Q loaders; the first of them notes where items begin
-    const int lt = tid - 13 * 32;
+  if (warp == 11) {
+    // ================================================================ Q loader; it notes where items begin
     int uses = 0;                               // Q buffers filled so far: buffer uses % 2
     int unit = u0;
     bool ok = true;
     while (ok && sa_next(p, w)) {
-      if (lt == 0 && w.t == 0) p.plan[1 + sa_item(p, w.s, w.b, w.pair, w.h)] = unit;
+      if (lane == 0 && w.t == 0) p.plan[1 + sa_item(p, w.s, w.b, w.pair, w.h)] = unit;
       unit += w.nt;
       for (int side = 0; side < (w.two ? 2 : 1) && ok; ++side, ++uses) {
         const int buf = uses & 1;
         ok = sa_wait(&q_empty[buf], ((uses >> 1) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
         if (!ok) break;
-        const uint32_t dst = smem_u32(sQ + buf * kSTile);
-        const int node0 = (w.pair * 2 + side) * p.npt;
-        for (int c = lt; c < SROWS * 16; c += 64) {
-          const int r = c >> 4, ch = c & 15, tok = r / p.G, node = node0 + tok;
-          const bool valid = tok < p.npt && node < w.s.n;
-          const __nv_bfloat16* src = p.q + (valid ? static_cast<long long>(w.s.q_begin + node) * p.ldq + (w.h * p.G + r % p.G) * SD + ch * 8 : 0);
-          sa_cp_async16(dst + (ch >> 3) * (SROWS * 128) + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, valid);
+        // A box holds the G heads of npt tokens.  Those behind the sequence's last one are another's or zero: a row's scores and output
+        // are its own, and nobody reads these.
+        if (elect_one()) {
+          mbar_expect_tx(&q_full[buf], p.npt * p.G * SD * 2);
+          const uint32_t dst = smem_u32(sQ + buf * kSTile);
+          const int token = w.s.q_begin + (w.pair * 2 + side) * p.npt;
+          sa_tma_heads(dst, &maps.q, &q_full[buf], 0, w.h * p.G, token);
+          sa_tma_heads(dst + SROWS * 128, &maps.q, &q_full[buf], 64, w.h * p.G, token);
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async();
-        mbar_arrive(&q_full[buf]);
+        __syncwarp();
       }
       sa_done(w);
     }
   } else if (warp >= 9) {
-    // ================================================================ K/V loaders: 32 keys of every tile each
+    // ================================================================ K/V loaders: 64 keys of every tile each
     const int lw = warp - 9;
     int n = 0;                                  // ring slots used so far
     bool ok = true;
@@ -343,27 +376,50 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       if (!known) report(p.status, kBadSlot);
       const int* slots = p.slot_map + static_cast<size_t>(known ? w.s.row : 0) * p.max_len;
       const int end = sa_end(p, w.s, w.b, w.pair), row0 = w.h * p.S;
-      auto slot_at = [&](int i) { return __ldg(slots + min(w.s.first + (w.t + i) * SKEYS + 32 * lw + lane, end - 1)); };      // keys past the end repeat the last one (no row sees them)
-      int next = slot_at(0);
+      auto slot_at = [&](int i, int part) {     // keys past the end repeat the last one (no row sees them)
+        return __ldg(slots + min(w.s.first + (w.t + i) * SKEYS + 64 * lw + 32 * part + lane, end - 1));
+      };
+      int next[2] = {slot_at(0, 0), slot_at(0, 1)};
       for (int i = 0; i < w.nt && ok; ++i) {
-        int slot = next;
-        if (i + 1 < w.nt) next = slot_at(i + 1);
-        if (slot < 0 || slot >= p.S) { report(p.status, kBadSlot); slot = 0; }
-        const int first = __shfl_sync(0xffffffffu, slot, lane & 16);
-        const uint32_t in_row = __ballot_sync(0xffffffffu, slot == first + (lane & 15));
+        int slot[2];
+        uint32_t in_row[2];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          slot[part] = next[part];
+          if (i + 1 < w.nt) next[part] = slot_at(i + 1, part);
+          if (slot[part] < 0 || slot[part] >= p.S) { report(p.status, kBadSlot); slot[part] = 0; }
+          const int first = __shfl_sync(0xffffffffu, slot[part], lane & 16);
+          in_row[part] = __ballot_sync(0xffffffffu, slot[part] == first + (lane & 15));
+        }
+        int page[4];
+#pragma unroll
+        for (int part = 0; part < 4; ++part) page[part] = row0 + __shfl_sync(0xffffffffu, slot[part >> 1], 16 * (part & 1));
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv, ++n) {
           const int s = n % SSLOTS;
           ok = sa_wait(&kv_empty[s], ((n / SSLOTS) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
           if (!ok) break;
           const CUtensorMap *box = kv ? &maps.v16 : &maps.k16, *one = kv ? &maps.v1 : &maps.k1;
-          if (elect_one()) mbar_expect_tx(&kv_full[s], 32 * 256);
+          if (elect_one()) mbar_expect_tx(&kv_full[s], 64 * 256);
           __syncwarp();
+          if ((in_row[0] & in_row[1]) == 0xffffffffu) {        // four pages
+            const uint32_t dst = smem_u32(sKV + s * kSTile) + 64 * lw * 128;
+            if (elect_one()) {
 #pragma unroll
-          for (int part = 0; part < 2; ++part) {
-            const uint32_t dst = smem_u32(sKV + s * kSTile) + (32 * lw + 16 * part) * 128;
-            if (((in_row >> (16 * part)) & 0xffffu) == 0xffffu) {
-              const int y = row0 + __shfl_sync(0xffffffffu, slot, 16 * part);
+              for (int part = 0; part < 4; ++part) {
+                sa_tma_box(dst + part * 2048, box, &kv_full[s], 0, page[part]);
+                sa_tma_box(dst + part * 2048 + SKEYS * 128, box, &kv_full[s], 64, page[part]);
+              }
+            }
+            __syncwarp();
+            continue;
+          }
+#pragma unroll 1
+          for (int part = 0; part < 4; ++part) {
+            const uint32_t dst = smem_u32(sKV + s * kSTile) + (64 * lw + 16 * part) * 128;
+            const int mine = part < 2 ? slot[0] : slot[1];
+            if ((((part < 2 ? in_row[0] : in_row[1]) >> (16 * (part & 1))) & 0xffffu) == 0xffffu) {
+              const int y = row0 + __shfl_sync(0xffffffffu, mine, 16 * (part & 1));
               if (elect_one()) {
                 sa_tma_box(dst, box, &kv_full[s], 0, y);
                 sa_tma_box(dst + SKEYS * 128, box, &kv_full[s], 64, y);
@@ -373,7 +429,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
               for (int g = 0; g < 4; ++g) {
                 int y[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = row0 + __shfl_sync(0xffffffffu, slot, 16 * part + 4 * g + e);
+                for (int e = 0; e < 4; ++e) y[e] = row0 + __shfl_sync(0xffffffffu, mine, 16 * (part & 1) + 4 * g + e);
                 if (elect_one()) {
                   sa_tma_rows(dst + g * 512, one, &kv_full[s], 0, y[0], y[1], y[2], y[3]);
                   sa_tma_rows(dst + g * 512 + SKEYS * 128, one, &kv_full[s], 64, y[0], y[1], y[2], y[3]);
@@ -391,23 +447,38 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     // ================================================================ MMA issuer: QK of job n + 2 goes behind PV of job n
     constexpr uint32_t idesc_qk = umma_idesc_bf16(SROWS, SKEYS), idesc_pv = umma_idesc_bf16(SROWS, SD) | (1u << 16);
     const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ)), k_desc = umma_desc_sw128(smem_u32(sKV)), v_desc = sa_desc_mn(smem_u32(sKV), SKEYS * 128);
-    struct Cursor { SaWalk w; int job, tile0, q0; bool more; };      // job within the segment; K/V tiles and Q buffers before it
-    auto open = [&](Cursor& c) { c.job = 0; c.more = sa_next(p, c.w); };
-    auto step = [&](Cursor& c) {                                      // behind the current job
-      if (++c.job < c.w.nt * (c.w.two ? 2 : 1)) return;
-      c.tile0 += c.w.nt;
-      c.q0 += c.w.two ? 2 : 1;
-      sa_done(c.w);
+    // PV follows QK by two jobs, so by three segments at most: their lengths wait in a ring (this warp writes and reads it)
+    struct Cursor { int job, nt, tile0, q0; bool two, more; };       // job within the segment, its length; K/V tiles and Q buffers before it
+    int wrote = 0, read = 0;
+    auto open_qk = [&](Cursor& c) {
+      c.job = 0;
+      c.more = sa_next(p, w);
+      if (c.more) { c.nt = w.nt; c.two = w.two; }
+      if (lane == 0) segs[wrote & 3] = c.more ? 2 * c.nt + c.two : 0;
+      ++wrote;
+      __syncwarp();
+    };
+    auto open_pv = [&](Cursor& c) {
+      const int v = segs[read++ & 3];
+      c.job = 0;
+      c.more = v != 0;
+      c.nt = v >> 1;
+      c.two = v & 1;
+    };
+    auto step = [&](Cursor& c, auto open) {                           // behind the current job
+      if (++c.job < (c.two ? 2 * c.nt : c.nt)) return;
+      c.tile0 += c.nt;
+      c.q0 += c.two ? 2 : 1;
       open(c);
     };
-    auto tile_of = [&](const Cursor& c) { return c.tile0 + (c.w.two ? c.job >> 1 : c.job); };
-    Cursor qk{w, 0, 0, 0, false}, pv{w, 0, 0, 0, false};
-    open(qk);
-    open(pv);
+    auto tile_of = [&](const Cursor& c) { return c.tile0 + (c.two ? c.job >> 1 : c.job); };
+    Cursor qk{0, 0, 0, 0, false, false}, pv{0, 0, 0, 0, false, false};
+    open_qk(qk);
+    open_pv(pv);
     int nq = 0, np = 0;                         // jobs issued
     bool ok = true;
     auto issue_qk = [&] {
-      const int jobs = qk.w.nt * (qk.w.two ? 2 : 1), side = qk.w.two ? qk.job & 1 : 0, use = qk.q0 + side, buf = use & 1, g = nq & 1;
+      const int jobs = qk.two ? 2 * qk.nt : qk.nt, side = qk.two ? qk.job & 1 : 0, use = qk.q0 + side, buf = use & 1, g = nq & 1;
       if (qk.job <= side && !sa_wait(&q_full[buf], (use >> 1) & 1, p.status, kTimeoutFull, gave_up)) return false;
       const int n = 2 * tile_of(qk), s = n % SSLOTS;
       if (!sa_wait(&kv_full[s], (n / SSLOTS) & 1, p.status, kTimeoutFull, gave_up)) return false;
@@ -417,17 +488,17 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           umma_f16(tmem + g * SKEYS, a + (k >> 2) * (SROWS * 128 >> 4) + 2 * (k & 3), b + (k >> 2) * (SKEYS * 128 >> 4) + 2 * (k & 3), idesc_qk, k != 0);
-        if (!qk.w.two || side == 1) umma_commit(&kv_empty[s]);
-        if (qk.job + (qk.w.two ? 2 : 1) >= jobs) umma_commit(&q_empty[buf]);
+        if (!qk.two || side == 1) umma_commit(&kv_empty[s]);
+        if (qk.job + (qk.two ? 2 : 1) >= jobs) umma_commit(&q_empty[buf]);
         umma_commit(&s_full[g]);
       }
       __syncwarp();
       ++nq;
-      step(qk);
+      step(qk, [&](Cursor& c) { sa_done(w); open_qk(c); });
       return true;
     };
     auto issue_pv = [&] {
-      const int jobs = pv.w.nt * (pv.w.two ? 2 : 1), g = np & 1, n = 2 * tile_of(pv) + 1, s = n % SSLOTS;
+      const int jobs = pv.two ? 2 * pv.nt : pv.nt, g = np & 1, n = 2 * tile_of(pv) + 1, s = n % SSLOTS;
       if (!sa_wait(&kv_full[s], (n / SSLOTS) & 1, p.status, kTimeoutFull, gave_up)) return false;
       if (!sa_wait(&p_full[g], (np >> 1) & 1, p.status, kTimeoutAccum, gave_up)) return false;
       tc_fence_after();
@@ -436,12 +507,12 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
 #pragma unroll
         for (int k = 0; k < SKEYS / 16; ++k)
           sa_mma_tmem_a(tmem + 256 + g * SD, tmem + g * SKEYS + k * 8, b + k * (2048 >> 4), idesc_pv, k != 0 || pv.job >= 2);
-        if (!pv.w.two || (pv.job & 1)) umma_commit(&kv_empty[s]);
+        if (!pv.two || (pv.job & 1)) umma_commit(&kv_empty[s]);
         if (pv.job + 2 >= jobs) umma_commit(&o_full[g]);
       }
       __syncwarp();
       ++np;
-      step(pv);
+      step(pv, open_pv);
       return true;
     };
     while (ok && qk.more && nq < 2) ok = issue_qk();
@@ -465,54 +536,74 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const int* bits = !p.causal && valid && !prefix ? p.mask_bits + static_cast<size_t>(w.s.q_begin + node) * p.W : nullptr;
       float m_run = -INFINITY, l_run = 0.f;
       int jobs = 0;
+      const bool busy = __any_sync(0xffffffffu, valid);      // a warp without rows only keeps the barriers going
       for (int i = w.two ? 0 : rel; i < w.nt && ok; i += w.two ? 1 : 2, ++jobs, ++jobs_done) {
         const int k0 = w.s.first + (w.t + i) * SKEYS;
-        uint32_t vis[4] = {0u, 0u, 0u, 0u};
-        const bool all = k0 + SKEYS <= min(w.s.past, end);      // the same for all rows of the item
-        if (!all && valid) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) vis[c] = sa_visible(p, w.s, prefix, end, node, bits, k0 + 32 * c);
-        }
+        const bool all = k0 + SKEYS <= min(w.s.past, end);      // every row of the item sees the whole block
         ok = sa_wait(&s_full[g], jobs_done & 1, p.status, kTimeoutAccum, gave_up);
         if (!ok) break;
         tc_fence_after();
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t sr[32];
-          tmem_ld_32x32(ts + 32 * c, sr);
-          tmem_ld_wait();
+        if (!busy) {
+          tc_fence_before();
+          mbar_arrive(&p_full[g]);
+          continue;
+        }
+        // The scores are read twice, 32 columns ahead of the arithmetic: holding all 128 takes more registers than 384 threads have.
+        // The loops stay short, since launches of a few blocks run every instruction from a cold cache.
+        auto columns = [&](auto use) {
+          uint32_t a[32], b[32];
+          tmem_ld_32x32(ts, a);
+#pragma unroll 1
+          for (int c = 0; c < SKEYS; c += 64) {
+            tmem_ld_wait();
+            tmem_ld_32x32(ts + c + 32, b);
+            use(c, a);
+            tmem_ld_wait();
+            if (c == 0) tmem_ld_32x32(ts + 64, a);
+            use(c + 32, b);
+          }
+        };
+        auto hide = [&](int c, uint32_t* sr) {          // scores of keys the row does not see
+          const uint32_t see = valid ? sa_visible(p, w.s, prefix, end, node, bits, k0 + c) : 0u;
 #pragma unroll
           for (int j = 0; j < 32; ++j)
-            mx4[j & 3] = fmaxf(mx4[j & 3], all || ((vis[c] >> j) & 1u) ? __uint_as_float(sr[j]) : -INFINITY);
-        }
+            if (!((see >> j) & 1u)) sr[j] = 0xff800000u;      // -inf
+        };
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        columns([&](int c, uint32_t* sr) {
+          if (!all) hide(c, sr);
+#pragma unroll
+          for (int j = 0; j < 32; j += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(sr[j + 2 * e])), __uint_as_float(sr[j + 2 * e + 1]));
+        });
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
         // integer running maximum in the log2 domain: probabilities are exact powers of two apart whatever the pieces
         const float m_new = fmaxf(m_run, ceilf(mx)), m_safe = m_new == -INFINITY ? 0.f : m_new;
         const float alpha = exp2f(m_run - m_safe);
         m_run = m_new;
-        float sum4[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = sa_pack(p.scale_log2, p.scale_log2), shift2 = sa_pack(-m_safe, -m_safe);
+        uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
+        columns([&](int c, uint32_t* sr) {
+          if (!all) hide(c, sr);
+          uint32_t pr[16];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          uint32_t sr[32], pr[16];
-          tmem_ld_32x32(ts + 32 * c, sr);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float p0 = sa_exp2(fmaf(__uint_as_float(sr[j]), p.scale_log2, -m_safe)), p1 = sa_exp2(fmaf(__uint_as_float(sr[j + 1]), p.scale_log2, -m_safe));
-            if (!all) {
-              if (!((vis[c] >> j) & 1u)) p0 = 0.f;
-              if (!((vis[c] >> (j + 1)) & 1u)) p1 = 0.f;
-            }
-            sum4[(j >> 1) & 3] += p0 + p1;
+          for (int j = 0; j < 16; ++j) {
+            float p0, p1;
+            sa_unpack(sa_fma2(sa_pack(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), scale2, shift2), p0, p1);
+            p0 = sa_exp2(p0);
+            p1 = sa_exp2(p1);
+            sum2[j & 3] = sa_add2(sum2[j & 3], sa_pack(p0, p1));
             const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);      // the MMA's operand: bf16, the sum keeps fp32
-            pr[j >> 1] = *reinterpret_cast<const uint32_t*>(&v);
+            pr[j] = *reinterpret_cast<const uint32_t*>(&v);
           }
-          sa_tmem_st16(ts + 16 * c, pr);        // over scores that are read already
-        }
-        l_run = l_run * alpha + ((sum4[0] + sum4[1]) + (sum4[2] + sum4[3]));
+          sa_tmem_st16(ts + c / 2, pr);         // over scores that are read already
+        });
+        float sum_lo, sum_hi;
+        sa_unpack(sa_add2(sa_add2(sum2[0], sum2[1]), sa_add2(sum2[2], sum2[3])), sum_lo, sum_hi);
+        l_run = l_run * alpha + (sum_lo + sum_hi);
         // every earlier PV of this group ended before these scores did
-        if (__any_sync(0xffffffffu, jobs > 0 && alpha != 1.f)) {
+        if (__any_sync(0xffffffffu, valid && jobs > 0 && alpha != 1.f)) {
 #pragma unroll 1
           for (int c = 0; c < SD; c += 32) {
             uint32_t o[32];
@@ -541,7 +632,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         tc_fence_after();
         const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
 #pragma unroll 1
-        for (int c = 0; c < SD; c += 32) {
+        for (int c = 0; busy && c < SD; c += 32) {
           uint32_t o[32];
           tmem_ld_32x32(to + c, o);
           tmem_ld_wait();
@@ -578,60 +669,110 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   }
 }
 
-// Joins the parts of a row: a warp each (token, head), four columns a lane.
-__global__ void __launch_bounds__(256) attn_shared_merge_kernel(const SharedAttn p) {
+// Joins the parts of the rows of a tile: a block takes up to kMergeRows rows of one head, a warp a row at a time, four columns a lane.
+constexpr int kMergeRows = 32, kMergeWarps = 8;
+__global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(const SharedAttn p) {
   pdl_launch_dependents();
   pdl_wait();
-  const int at = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (at >= p.T * p.Hq) return;
-  const int t = at / p.Hq, head = at % p.Hq, h = head / p.G, sub = head % p.G;
-  int b = -1;                                  // sequences that begin at or before the token, the last of them that has it
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, row0 = blockIdx.z * kMergeRows;
+  {                                            // rows behind the last sequence are zero
+    const int first = max(0, min(p.cu_q[p.B], p.T));
+    uint4* out = reinterpret_cast<uint4*>(p.out + static_cast<size_t>(first) * p.Hq * SD);
+    const size_t n = static_cast<size_t>(p.T - first) * p.Hq * SD / 8, blocks = static_cast<size_t>(gridDim.x) * gridDim.y * gridDim.z;
+    const size_t block = (static_cast<size_t>(blockIdx.z) * gridDim.y + h) * gridDim.x + blockIdx.x;
+    for (size_t i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) out[i] = make_uint4(0u, 0u, 0u, 0u);
+  }
+  // tiles are numbered like pairs: those of a sequence start behind the tiles of all rows before it
+  int b = -1;                                  // the last sequence that starts at or before this tile
   for (int base = 0; base < p.B; base += 32) {
-    const bool before = base + lane < p.B && p.cu_q[base + lane] <= t;
-    const unsigned some = __ballot_sync(0xffffffffu, before);
+    const unsigned some = __ballot_sync(0xffffffffu, base + lane < p.B && min(max(p.cu_q[base + lane], 0), p.T) / p.npt + base + lane <= static_cast<int>(blockIdx.x));
     b += __popc(some);
     if (some != 0xffffffffu) break;
   }
-  __nv_bfloat16* out = p.out + static_cast<size_t>(at) * SD + lane * 4;
-  float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-  const int total = p.plan[0];
-  auto join = [&](const float* o, const float2* ml, size_t row) {
-    const float2 v = ml[row];
-    if (v.y == 0.f) return;                    // no visible key (the part's output may be unwritten)
-    const float m_new = fmaxf(m, v.x), safe = m_new == -INFINITY ? 0.f : m_new;      // NaN scores leave a sum without a maximum
-    const float old = exp2f(m - safe), add = exp2f(v.x - safe);
-    const float4 x = *reinterpret_cast<const float4*>(o + row * SD + lane * 4);
-    acc[0] = acc[0] * old + x.x * add;
-    acc[1] = acc[1] * old + x.y * add;
-    acc[2] = acc[2] * old + x.z * add;
-    acc[3] = acc[3] * old + x.w * add;
-    l = l * old + v.y * add;
-    m = m_new;
-  };
-  bool done = false;
-  for (int part = p.prefix > 0 ? 0 : 1; part < 2 && b >= 0; ++part) {
-    const int seq = part == 0 ? -1 : b;
-    const SaSeq s = sa_seq(p, seq);
-    const int node = t - s.q_begin, tile = node / p.npt, pair = tile >> 1;
-    if (node < 0 || node >= s.n) continue;     // behind the last sequence
-    const int units = sa_units(p, s, seq, pair);
-    if (units == 0) continue;
-    const int item = sa_item(p, s, seq, pair, h), u = p.plan[1 + item];
-    const int c0 = sa_cta(p, u, total), c1 = sa_cta(p, u + units - 1, total);
-    const bool two = s.n - pair * 2 * p.npt > p.npt;
-    if (two && c0 == c1 && part == 1 && p.prefix == 0) { done = true; break; }
-    const int rows = part == 0 ? SROWS : p.seq_rows_kept, row = (node - tile * p.npt) * p.G + sub;
-    if (row >= rows) continue;
-    for (int c = c0; c <= c1; ++c) {
-      const size_t seg = (static_cast<size_t>(c) + (part == 0 ? item : item - p.prefix_items)) * 2;
-      for (int side = two ? tile & 1 : 0; side < (two ? (tile & 1) + 1 : 2); ++side)
-        join(part == 0 ? p.po : p.so, part == 0 ? p.pml : p.sml, (seg + side) * rows + row);
-    }
+  if (b < 0) return;
+  const SaSeq s = sa_seq(p, b);
+  const int tile = blockIdx.x - (s.q_begin / p.npt + b), node0 = tile * p.npt;
+  const int rows = min(p.npt, s.n - node0) * p.G;
+  if (rows <= row0) return;
+  const int total = p.plan[0], pair = tile >> 1, units = sa_units(p, s, b, pair);
+  const bool two = s.n - pair * 2 * p.npt > p.npt;
+  int c0 = 0, own = 0, item = 0;               // first CTA and number of CTAs with a part of the sequence's own keys
+  if (units > 0) {
+    item = sa_item(p, s, b, pair, h);
+    const int u = p.plan[1 + item];
+    c0 = sa_cta(p, u, total);
+    own = sa_cta(p, u + units - 1, total) - c0 + 1;
+    item -= p.prefix_items;
   }
-  if (done) return;                            // written by its CTA
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
-  *reinterpret_cast<__nv_bfloat162*>(out + 2) = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+  if (own == 1 && two && p.prefix == 0) return;       // written by its CTA
+  const SaSeq all = p.prefix > 0 ? sa_seq(p, -1) : s;
+  const int all_units = p.prefix > 0 ? sa_units(p, all, -1, 0) : 0;
+  const int own_parts = two ? own : 2 * own;
+  for (int row = row0 + warp; row < min(rows, row0 + kMergeRows); row += kMergeWarps) {
+    const int tok = row / p.G, t = s.q_begin + node0 + tok, head = h * p.G + row - tok * p.G;
+    int pc0 = 0, shared_parts = 0, p_item = 0, p_row = 0;
+    bool p_two = false;
+    if (all_units > 0) {
+      const int p_tile = t / p.npt, p_pair = p_tile >> 1;
+      p_item = sa_item(p, all, -1, p_pair, h);
+      const int u = (p_pair * p.Hkv + h) * all_units;
+      pc0 = sa_cta(p, u, total);
+      p_two = all.n - p_pair * 2 * p.npt > p.npt;
+      shared_parts = (sa_cta(p, u + all_units - 1, total) - pc0 + 1) * (p_two ? 1 : 2);
+      p_row = (t - p_tile * p.npt) * p.G + row - tok * p.G + (p_two ? (p_tile & 1) * SROWS : 0);
+    }
+    const int parts = shared_parts + own_parts;
+    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int base = 0; base < parts; base += 32) {
+      // a part a lane: where it lies, its maximum and sum
+      const int k = base + lane;
+      const float* at = nullptr;
+      float2 ml = make_float2(-INFINITY, 0.f);
+      if (k < shared_parts) {
+        const size_t r = (static_cast<size_t>(pc0 + (p_two ? k : k >> 1) + p_item) * 2 + (p_two ? 0 : k & 1)) * SROWS + p_row;
+        ml = p.pml[r];
+        at = p.po + r * SD;
+      } else if (k < parts && row < p.seq_rows_kept) {
+        const int j = k - shared_parts;
+        const size_t r = (static_cast<size_t>(c0 + (two ? j : j >> 1) + item) * 2 + (two ? tile & 1 : j & 1)) * p.seq_rows_kept + row;
+        ml = p.sml[r];
+        at = p.so + r * SD;
+      }
+      if (ml.y == 0.f) ml.x = -INFINITY;       // no visible key: the part's output may be unwritten
+      const float m_new = fmaxf(m, warp_max(ml.x)), safe = m_new == -INFINITY ? 0.f : m_new;      // NaN scores leave a sum without a maximum
+      const float old = exp2f(m - safe), add = ml.y == 0.f ? 0.f : exp2f(ml.x - safe);
+      m = m_new;
+      l = l * old + warp_sum(ml.y * add);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[j] *= old;
+      const int here = min(32, parts - base);
+#pragma unroll 4
+      for (int j = 0; j < here; ++j) {
+        const float f = __shfl_sync(0xffffffffu, add, j);
+        const unsigned long long from = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), j);
+        const bool use = __shfl_sync(0xffffffffu, ml.y, j) != 0.f;
+        const float4 x = use ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        acc[0] = fmaf(x.x, f, acc[0]);
+        acc[1] = fmaf(x.y, f, acc[1]);
+        acc[2] = fmaf(x.z, f, acc[2]);
+        acc[3] = fmaf(x.w, f, acc[3]);
+      }
+    }
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    __nv_bfloat16* out = p.out + (static_cast<size_t>(t) * p.Hq + head) * SD + lane * 4;
+    *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
+    *reinterpret_cast<__nv_bfloat162*>(out + 2) = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+  }
+}
+
+// Queries as (tokens, heads, 128), tokens ldq elements apart
+static int make_head_map(CUtensorMap* m, const void* q, int T, int Hq, long long ldq, int npt, int G) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return -1;
+  cuuint64_t dims[3] = {SD, static_cast<cuuint64_t>(Hq), static_cast<cuuint64_t>(T)}, strides[2] = {SD * 2, static_cast<cuuint64_t>(ldq) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(G), static_cast<cuuint32_t>(npt)}, step[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -2;
 }
 
 static long long shared_round(long long bytes) { return (bytes + 255) / 256 * 256; }
@@ -654,10 +795,10 @@ static long long shared_layout(SharedAttn* p, uint8_t* ws, int max_q) {
   return at;
 }
 
-// Attending to the prefix for all rows together pays where sequences leave much of their own tiles empty.
-static bool shared_pays(int B, int T, int max_q, int G, int npt) {
-  (void)G;
-  const long long own = static_cast<long long>(B) * ((max_q + npt - 1) / npt), together = (T + npt - 1) / npt;
+// Attending to the prefix for all rows together pays where sequences leave much of their own tiles empty: tiles of all rows together
+// against those of B sequences, whose last ones are half full on average.
+static bool shared_pays(int B, int T, int npt) {
+  const long long together = T, own = std::max(static_cast<long long>(B) * npt, T + static_cast<long long>(B) * npt / 2);
   return 4 * together <= 3 * own;
 }
 
@@ -667,9 +808,8 @@ static int shared_setup(SharedAttn* p, int max_q, int prefix_len, int ctas) {
   if (p->G > SROWS) return -11;
   p->npt = SROWS / p->G;
   p->ctas = ctas;
-  const bool shared = prefix_len > 0 && shared_pays(p->B, p->T, max_q, p->G, p->npt);
-  p->prefix = shared ? prefix_len : 0;
-  p->first_key = shared ? prefix_len : 0;
+  // The sequences' own items begin at a multiple of 16 positions, where pages do, so that their keys load in boxes.
+  p->prefix = p->first_key = shared_pays(p->B, p->T, p->npt) ? prefix_len / 16 * 16 : 0;
   return 0;
 }
 
@@ -710,14 +850,15 @@ extern "C" int js_shared_attention(const void* q, long long ldq, const void* k_p
   SharedMaps maps;
   const uint64_t rows = static_cast<uint64_t>(Hkv) * S;
   if (rows >= (1ull << 31) || make_map(&maps.k16, k_pool, rows, SD, SD, 16) || make_map(&maps.v16, v_pool, rows, SD, SD, 16) ||
-      make_map(&maps.k1, k_pool, rows, SD, SD, 1) || make_map(&maps.v1, v_pool, rows, SD, SD, 1)) return -15;
+      make_map(&maps.k1, k_pool, rows, SD, SD, 1) || make_map(&maps.v1, v_pool, rows, SD, SD, 1) ||
+      make_head_map(&maps.q, q, T, Hq, ldq, p.npt, p.G)) return -15;
   static int configured[kMaxDevicesCached] = {};
   if (ensure_dyn_smem(attn_shared_kernel, kSharedSmem, configured) != 0) return -3;
   attn_shared_kernel<<<ctas, STHREADS, kSharedSmem, stream>>>(p, maps);
   if (cudaGetLastError() != cudaSuccess) return -4;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((T * Hq + 7) / 8);
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(T / p.npt + B, Hkv, (p.seq_rows_kept + kMergeRows - 1) / kMergeRows);
+  cfg.blockDim = dim3(32 * kMergeWarps);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -336,14 +336,10 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
                             scale: float, prefix_len: int, causal: bool = False) -> torch.Tensor:
     """:func:`paged_tree_attention` of a batch whose sequences share their first ``prefix_len`` positions.
 
-    Every ``past_lens[b] >= prefix_len``, and the rows ``seq_rows`` of the slot map hold the same slots up to there; the prefix is
-    read through the first of them.  Rows behind the last sequence (``cu_q[-1]`` and on) are zero.
+    Every ``past_lens[b] >= prefix_len``, and the rows ``seq_rows`` of the slot map hold the same slots up to there (the kernel reads the
+    prefix through the first of them).  Rows behind the last sequence (``cu_q[-1]`` and on) are zero.
     """
-    rows = slot_map.clone()
-    if seq_rows.numel():
-        r = seq_rows.long()
-        rows[r, :prefix_len] = slot_map[r[0], :prefix_len]
-    out = paged_tree_attention(q, k_pool, v_pool, rows, seq_rows, cu_q, past_lens, mask_bits, scale, causal)
+    out = paged_tree_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale, causal)
     out[int(cu_q[-1]):] = 0
     return out
 
