@@ -155,6 +155,13 @@ JS_DEVICE void sa_tmem_st16(uint32_t taddr, const uint32_t* r) {
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
 }
+JS_DEVICE void sa_tmem_ld16(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr) : "memory");
+}
 JS_DEVICE void sa_tmem_st32(uint32_t taddr, const uint32_t* r) {
   sa_tmem_st16(taddr, r);
   sa_tmem_st16(taddr + 16, r + 16);
@@ -234,8 +241,9 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + SSLOTS * kSTile);
   uint64_t *kv_full = bars, *kv_empty = bars + SSLOTS;                        // a slot of the ring
   uint64_t *q_full = bars + 2 * SSLOTS, *q_empty = q_full + 2;                // a Q buffer
-  uint64_t *s_full = q_empty + 2, *p_full = s_full + 2, *o_full = p_full + 2; // a group
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_full + 2);
+  uint64_t *s_full = q_empty + 2, *o_full = s_full + 2; // a group
+  uint64_t* p_full = o_full + 2;                                              // half the keys of a group's job
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 4);
   uint32_t* gave_up_words = tmem_slot + 1;
   int* start = reinterpret_cast<int*>(gave_up_words + 16);                    // the first unit: b, pair, h, t; units in all; scan scratch
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -251,7 +259,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       mbar_init(&q_full[g], 1);
       mbar_init(&q_empty[g], 1);
       mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[g], 128);
+      mbar_init(&p_full[2 * g], 128);
+      mbar_init(&p_full[2 * g + 1], 128);
       mbar_init(&o_full[g], 1);
     }
     for (int w = 0; w < 16; ++w) gave_up_words[w] = 0;
@@ -500,13 +509,19 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     auto issue_pv = [&] {
       const int jobs = pv.two ? 2 * pv.nt : pv.nt, g = np & 1, n = 2 * tile_of(pv) + 1, s = n % SSLOTS;
       if (!sa_wait(&kv_full[s], (n / SSLOTS) & 1, p.status, kTimeoutFull, gave_up)) return false;
-      if (!sa_wait(&p_full[g], (np >> 1) & 1, p.status, kTimeoutAccum, gave_up)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t b = v_desc + static_cast<uint64_t>(s * (kSTile >> 4));
+      const uint64_t b = v_desc + static_cast<uint64_t>(s * (kSTile >> 4));
 #pragma unroll
-        for (int k = 0; k < SKEYS / 16; ++k)
-          sa_mma_tmem_a(tmem + 256 + g * SD, tmem + g * SKEYS + k * 8, b + k * (2048 >> 4), idesc_pv, k != 0 || pv.job >= 2);
+      for (int half = 1; half >= 0; --half) {        // the second half of the keys is weighed first
+        if (!sa_wait(&p_full[2 * g + half], (np >> 1) & 1, p.status, kTimeoutAccum, gave_up)) return false;
+        tc_fence_after();
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 4 * half; k < 4 * half + 4; ++k)
+            sa_mma_tmem_a(tmem + 256 + g * SD, tmem + g * SKEYS + k * 8, b + k * (2048 >> 4), idesc_pv, k != 4 || pv.job >= 2);
+        }
+        __syncwarp();
+      }
+      if (elect_one()) {
         if (!pv.two || (pv.job & 1)) umma_commit(&kv_empty[s]);
         if (pv.job + 2 >= jobs) umma_commit(&o_full[g]);
       }
@@ -545,38 +560,52 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         tc_fence_after();
         if (!busy) {
           tc_fence_before();
-          mbar_arrive(&p_full[g]);
+          mbar_arrive(&p_full[2 * g]);
+          mbar_arrive(&p_full[2 * g + 1]);
           continue;
         }
-        // The scores are read twice, 32 columns ahead of the arithmetic: holding all 128 takes more registers than 384 threads have.
-        // The loops stay short, since launches of a few blocks run every instruction from a cold cache.
-        auto columns = [&](auto use) {
-          uint32_t a[32], b[32];
-          tmem_ld_32x32(ts, a);
-#pragma unroll 1
-          for (int c = 0; c < SKEYS; c += 64) {
-            tmem_ld_wait();
-            tmem_ld_32x32(ts + c + 32, b);
-            use(c, a);
-            tmem_ld_wait();
-            if (c == 0) tmem_ld_32x32(ts + 64, a);
-            use(c + 32, b);
+        // The halves of the scores pass through registers in the order 0, 1 for the maximum and 1, 0 for the exponentials: half 1 stays,
+        // half 0 is read again behind its back.  All 128 columns at once, and what becomes of them, take more than 168 registers.
+        uint32_t s0[64], s1[64];
+        auto load = [&](int half, uint32_t* sr) {
+          tmem_ld_32x32(ts + 64 * half, sr);
+          tmem_ld_32x32(ts + 64 * half + 32, sr + 32);
+        };
+        auto hide = [&](int half, uint32_t* sr) {       // scores of keys the row does not see
+#pragma unroll
+          for (int c = 0; c < 64; c += 32) {
+            const uint32_t see = valid ? sa_visible(p, w.s, prefix, end, node, bits, k0 + 64 * half + c) : 0u;
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (!((see >> j) & 1u)) sr[c + j] = 0xff800000u;      // -inf
           }
         };
-        auto hide = [&](int c, uint32_t* sr) {          // scores of keys the row does not see
-          const uint32_t see = valid ? sa_visible(p, w.s, prefix, end, node, bits, k0 + c) : 0u;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (!((see >> j) & 1u)) sr[j] = 0xff800000u;      // -inf
-        };
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        columns([&](int c, uint32_t* sr) {
-          if (!all) hide(c, sr);
+        auto top = [&](const uint32_t* sr) {
 #pragma unroll
-          for (int j = 0; j < 32; j += 8)
+          for (int j = 0; j < 64; j += 8)
 #pragma unroll
             for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(sr[j + 2 * e])), __uint_as_float(sr[j + 2 * e + 1]));
-        });
+        };
+        auto landed = [&](uint32_t* sr) {       // and nothing of it is used before this point
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 64; ++j) asm volatile("" : "+r"(sr[j]));
+        };
+        load(0, s0);
+        landed(s0);
+        load(1, s1);
+        if (!all) hide(0, s0);
+        top(s0);
+        landed(s1);
+        if (!all) {
+          sa_tmem_st32(ts, s0);                 // for the second look
+          sa_tmem_st32(ts + 32, s0 + 32);
+          hide(1, s1);
+          sa_tmem_st_wait();
+        }
+        top(s1);
+        load(0, s0);
         const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
         // integer running maximum in the log2 domain: probabilities are exact powers of two apart whatever the pieces
         const float m_new = fmaxf(m_run, ceilf(mx)), m_safe = m_new == -INFINITY ? 0.f : m_new;
@@ -584,9 +613,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         m_run = m_new;
         const uint64_t scale2 = sa_pack(p.scale_log2, p.scale_log2), shift2 = sa_pack(-m_safe, -m_safe);
         uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
-        columns([&](int c, uint32_t* sr) {
-          if (!all) hide(c, sr);
-          uint32_t pr[16];
+        auto weigh = [&](const uint32_t* sr, uint32_t* pr) {      // 32 scores
 #pragma unroll
           for (int j = 0; j < 16; ++j) {
             float p0, p1;
@@ -597,26 +624,39 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
             const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);      // the MMA's operand: bf16, the sum keeps fp32
             pr[j] = *reinterpret_cast<const uint32_t*>(&v);
           }
-          sa_tmem_st16(ts + c / 2, pr);         // over scores that are read already
-        });
-        float sum_lo, sum_hi;
-        sa_unpack(sa_add2(sa_add2(sum2[0], sum2[1]), sa_add2(sum2[2], sum2[3])), sum_lo, sum_hi);
-        l_run = l_run * alpha + (sum_lo + sum_hi);
+        };
+        auto publish = [&](int half) {
+          sa_tmem_st_wait();
+          tc_fence_before();
+          mbar_arrive(&p_full[2 * g + half]);
+        };
+        uint32_t pr[16];
+        weigh(s1, pr);
+        landed(s0);                             // half 0 is in registers: probabilities may take its place
         // every earlier PV of this group ended before these scores did
         if (__any_sync(0xffffffffu, valid && jobs > 0 && alpha != 1.f)) {
 #pragma unroll 1
-          for (int c = 0; c < SD; c += 32) {
-            uint32_t o[32];
-            tmem_ld_32x32(to + c, o);
+          for (int c = 0; c < SD; c += 16) {
+            uint32_t o[16];
+            sa_tmem_ld16(to + c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            sa_tmem_st32(to + c, o);
+            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            sa_tmem_st16(to + c, o);
           }
         }
-        sa_tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_full[g]);
+        sa_tmem_st16(ts + 32, pr);
+        weigh(s1 + 32, pr);
+        sa_tmem_st16(ts + 48, pr);
+        publish(1);
+        weigh(s0, pr);
+        sa_tmem_st16(ts, pr);
+        weigh(s0 + 32, pr);
+        sa_tmem_st16(ts + 16, pr);
+        publish(0);
+        float sum_lo, sum_hi;
+        sa_unpack(sa_add2(sa_add2(sum2[0], sum2[1]), sa_add2(sum2[2], sum2[3])), sum_lo, sum_hi);
+        l_run = l_run * alpha + (sum_lo + sum_hi);
       }
       if (!ok) break;
       // ---- the segment's result: the output where this CTA saw all keys of the rows, else a part
