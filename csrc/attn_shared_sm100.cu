@@ -6,15 +6,15 @@
 // own keys [P, L), and the parts are joined.  Where every sequence's rows fill tiles of their own there is nothing to gain by that, and a
 // sequence's rows take both ranges in one go.
 //
-// Work is a line of units, a unit being 128 keys for a pair of row tiles: items (pair of tiles, KV head) one after the other, an
+// Work is a line of units, a unit being 80 keys for a pair of row tiles: items (pair of tiles, KV head) one after the other, an
 // item's units in key order.  Every CTA takes an equal piece of the line, so lengths, which only the device knows, balance by
 // themselves; where a piece begins or ends inside an item its parts go through a workspace and attn_shared_merge_kernel.
 //
-// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warp 8 issues the MMAs, warps 9-10 load K and V by TMA (boxes of 16 rows where
-// slots follow one another, gathers of four rows where not), warp 11 loads Q.  A job is one row tile against 128 keys; jobs alternate between the
-// groups: the two tiles of a pair on the same keys, or, for a single tile, every other block of keys.  Scores (128 columns) and
-// output (128 columns) of both groups fill the 512 columns of tensor memory; probabilities overwrite the scores as bf16 and are the second
-// MMA's A operand there.  Every wait is bounded (status word).
+// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warps 8 and 12 issue the MMAs of either product, warps 9 and 10 load K and V by
+// TMA (boxes of 16 rows where slots follow one another, gathers of four rows where not), warp 11 loads Q.  A job is one row tile against 80 keys; jobs alternate between the
+// groups: the two tiles of a pair on the same keys, or, for a single tile, every other block of keys.  Tensor memory holds
+// scores (80 columns), probabilities as bf16 (40; the second MMA's A operand) and output (128) of both groups, so that a group's next scores
+// are there while it weighs its last ones.  Every wait is bounded (status word).
 #include "gemm_common.cuh"
 
 #include <math.h>
@@ -24,11 +24,12 @@ namespace js {
 
 constexpr int SD = 128;              // head dim
 constexpr int SROWS = 128;           // rows of a tile
-constexpr int SKEYS = 128;           // keys of a unit
-constexpr int SSLOTS = 5;            // ring of K and V tiles, in turn
-constexpr int kSTile = 128 * 256;    // bytes of a K, V or Q tile: 2 halves x 128 rows x 128 B
-constexpr int SWARPS = 12, STHREADS = 32 * SWARPS;      // 168 registers a thread
-constexpr int kSharedSmem = (2 + SSLOTS) * kSTile + 512 + 1024;
+constexpr int SKEYS = 80;            // keys of a unit: scores (80 columns) and probabilities (40) of a group fit 128 columns side by side
+constexpr int SSLOTS = 8;            // ring of K and V tiles, in turn
+constexpr int kQTile = SROWS * 256, kKTile = SKEYS * 256;      // bytes of a Q, K or V tile: 2 halves x rows x 128 B
+constexpr int SWARPS = 13, STHREADS = 32 * SWARPS;      // 152 registers a thread
+constexpr int kSharedSmem = 2 * kQTile + SSLOTS * kKTile + 512;
+constexpr int kColP = SKEYS, kColO = 256;      // tensor memory: scores of group g from column 128 g, its probabilities behind them, its output from 256 + 128 g
 
 struct SharedAttn {
   const __nv_bfloat16* q;      // (T, Hq, 128), ldq elements between tokens
@@ -162,6 +163,10 @@ JS_DEVICE void sa_tmem_ld16(uint32_t taddr, uint32_t* r) {
         "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(taddr) : "memory");
 }
+JS_DEVICE void sa_tmem_st8(uint32_t taddr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
 JS_DEVICE void sa_tmem_st32(uint32_t taddr, const uint32_t* r) {
   sa_tmem_st16(taddr, r);
   sa_tmem_st16(taddr + 16, r + 16);
@@ -171,6 +176,11 @@ JS_DEVICE float sa_exp2(float x) {      // denormal results flush to zero; exp2(
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+JS_DEVICE float sa_max3(float a, float b, float c) {      // NaN if one is: a row with a NaN score stays NaN
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 // two fp32 in a register pair: half as many instructions
 JS_DEVICE uint64_t sa_pack(float lo, float hi) {
@@ -235,15 +245,13 @@ JS_DEVICE uint32_t sa_visible(const SharedAttn& p, const SaSeq& s, bool prefix, 
 }
 
 __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAttn p, const __grid_constant__ SharedMaps maps) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t *sQ = smem, *sKV = smem + 2 * kSTile;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + SSLOTS * kSTile);
+  extern __shared__ __align__(1024) uint8_t smem[];        // swizzled tiles begin at multiples of 1024
+  uint8_t *sQ = smem, *sKV = smem + 2 * kQTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + SSLOTS * kKTile);
   uint64_t *kv_full = bars, *kv_empty = bars + SSLOTS;                        // a slot of the ring
   uint64_t *q_full = bars + 2 * SSLOTS, *q_empty = q_full + 2;                // a Q buffer
-  uint64_t *s_full = q_empty + 2, *o_full = s_full + 2; // a group
-  uint64_t* p_full = o_full + 2;                                              // half the keys of a group's job
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(p_full + 4);
+  uint64_t *s_full = q_empty + 2, *s_read = s_full + 2, *p_full = s_read + 2, *pv_done = p_full + 2;      // a group
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 2);
   uint32_t* gave_up_words = tmem_slot + 1;
   int* start = reinterpret_cast<int*>(gave_up_words + 16);                    // the first unit: b, pair, h, t; units in all; scan scratch
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -254,22 +262,21 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
 
   // ---- this CTA's piece of the line
   if (tid == 0) {
-    for (int s = 0; s < SSLOTS; ++s) { mbar_init(&kv_full[s], 2); mbar_init(&kv_empty[s], 1); }
+    for (int s = 0; s < SSLOTS; ++s) { mbar_init(&kv_full[s], 1); mbar_init(&kv_empty[s], 1); }
     for (int g = 0; g < 2; ++g) {
       mbar_init(&q_full[g], 1);
       mbar_init(&q_empty[g], 1);
       mbar_init(&s_full[g], 1);
-      mbar_init(&p_full[2 * g], 128);
-      mbar_init(&p_full[2 * g + 1], 128);
-      mbar_init(&o_full[g], 1);
+      mbar_init(&s_read[g], 128);
+      mbar_init(&p_full[g], 128);
+      mbar_init(&pv_done[g], 1);
     }
     for (int w = 0; w < 16; ++w) gave_up_words[w] = 0;
     fence_barrier_init();
   }
   int* scan = start + 8;                        // a total per warp
-  volatile int* segs = start + 8 + SWARPS;      // the MMA warp's
   const int prefix_units = p.prefix > 0 ? sa_total(p, -1) * p.Hkv : 0;
-  // units of the sequences ahead of this thread's (of every 384), and of all of them
+  // units of the sequences ahead of this thread's (of every 416), and of all of them
   auto ahead = [&](int value, int& all) {
     int inc = value;
 #pragma unroll
@@ -366,7 +373,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         // are its own, and nobody reads these.
         if (elect_one()) {
           mbar_expect_tx(&q_full[buf], p.npt * p.G * SD * 2);
-          const uint32_t dst = smem_u32(sQ + buf * kSTile);
+          const uint32_t dst = smem_u32(sQ + buf * kQTile);
           const int token = w.s.q_begin + (w.pair * 2 + side) * p.npt;
           sa_tma_heads(dst, &maps.q, &q_full[buf], 0, w.h * p.G, token);
           sa_tma_heads(dst + SROWS * 128, &maps.q, &q_full[buf], 64, w.h * p.G, token);
@@ -375,10 +382,11 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       }
       sa_done(w);
     }
-  } else if (warp >= 9) {
-    // ================================================================ K/V loaders: 64 keys of every tile each
-    const int lw = warp - 9;
-    int n = 0;                                  // ring slots used so far
+  } else if (warp == 9 || warp == 10) {
+    // ================================================================ loaders: warp 9 takes the K tiles, warp 10 the V tiles
+    const bool values = warp == 10;
+    const CUtensorMap *box = values ? &maps.v16 : &maps.k16, *one = values ? &maps.v1 : &maps.k1;
+    int n = values;                             // ring slots used so far
     bool ok = true;
     while (ok && sa_next(p, w)) {
       const bool known = w.s.row >= 0 && w.s.row < p.max_seqs;
@@ -386,161 +394,116 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const int* slots = p.slot_map + static_cast<size_t>(known ? w.s.row : 0) * p.max_len;
       const int end = sa_end(p, w.s, w.b, w.pair), row0 = w.h * p.S;
       auto slot_at = [&](int i, int part) {     // keys past the end repeat the last one (no row sees them)
-        return __ldg(slots + min(w.s.first + (w.t + i) * SKEYS + 64 * lw + 32 * part + lane, end - 1));
+        return __ldg(slots + min(w.s.first + (w.t + i) * SKEYS + 32 * part + lane, end - 1));
       };
-      int next[2] = {slot_at(0, 0), slot_at(0, 1)};
-      for (int i = 0; i < w.nt && ok; ++i) {
-        int slot[2];
-        uint32_t in_row[2];
+      int next[3] = {slot_at(0, 0), slot_at(0, 1), slot_at(0, 2)};
+      for (int i = 0; i < w.nt; ++i, n += 2) {
+        int slot[3], page[6];
+        uint32_t in_row = 0xffffffffu;
 #pragma unroll
-        for (int part = 0; part < 2; ++part) {
+        for (int part = 0; part < 3; ++part) {
           slot[part] = next[part];
           if (i + 1 < w.nt) next[part] = slot_at(i + 1, part);
           if (slot[part] < 0 || slot[part] >= p.S) { report(p.status, kBadSlot); slot[part] = 0; }
           const int first = __shfl_sync(0xffffffffu, slot[part], lane & 16);
-          in_row[part] = __ballot_sync(0xffffffffu, slot[part] == first + (lane & 15));
+          uint32_t seen = __ballot_sync(0xffffffffu, slot[part] == first + (lane & 15));
+          if (part == 2) seen |= 0xffff0000u;   // the tile ends after 16 of these
+          in_row &= seen;
+          page[2 * part] = row0 + __shfl_sync(0xffffffffu, slot[part], 0);
+          page[2 * part + 1] = row0 + __shfl_sync(0xffffffffu, slot[part], 16);
         }
-        int page[4];
+        const int s = n % SSLOTS;
+        ok = sa_wait(&kv_empty[s], ((n / SSLOTS) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
+        if (!ok) break;
+        const uint32_t dst = smem_u32(sKV + s * kKTile);
+        if (elect_one()) {
+          mbar_expect_tx(&kv_full[s], kKTile);
+          if (in_row == 0xffffffffu) {          // all of it in pages
 #pragma unroll
-        for (int part = 0; part < 4; ++part) page[part] = row0 + __shfl_sync(0xffffffffu, slot[part >> 1], 16 * (part & 1));
+            for (int part = 0; part < 5; ++part) {
+              sa_tma_box(dst + part * 2048, box, &kv_full[s], 0, page[part]);
+              sa_tma_box(dst + part * 2048 + SKEYS * 128, box, &kv_full[s], 64, page[part]);
+            }
+          }
+        }
+        __syncwarp();
+        if (in_row == 0xffffffffu) continue;
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv, ++n) {
-          const int s = n % SSLOTS;
-          ok = sa_wait(&kv_empty[s], ((n / SSLOTS) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
-          if (!ok) break;
-          const CUtensorMap *box = kv ? &maps.v16 : &maps.k16, *one = kv ? &maps.v1 : &maps.k1;
-          if (elect_one()) mbar_expect_tx(&kv_full[s], 64 * 256);
+        for (int g = 0; g < SKEYS / 4; ++g) {
+          int y[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e] = row0 + __shfl_sync(0xffffffffu, slot[g / 8], 4 * (g & 7) + e);
+          if (elect_one()) {
+            sa_tma_rows(dst + g * 512, one, &kv_full[s], 0, y[0], y[1], y[2], y[3]);
+            sa_tma_rows(dst + g * 512 + SKEYS * 128, one, &kv_full[s], 64, y[0], y[1], y[2], y[3]);
+          }
           __syncwarp();
-          if ((in_row[0] & in_row[1]) == 0xffffffffu) {        // four pages
-            const uint32_t dst = smem_u32(sKV + s * kSTile) + 64 * lw * 128;
-            if (elect_one()) {
-#pragma unroll
-              for (int part = 0; part < 4; ++part) {
-                sa_tma_box(dst + part * 2048, box, &kv_full[s], 0, page[part]);
-                sa_tma_box(dst + part * 2048 + SKEYS * 128, box, &kv_full[s], 64, page[part]);
-              }
-            }
-            __syncwarp();
-            continue;
-          }
-#pragma unroll 1
-          for (int part = 0; part < 4; ++part) {
-            const uint32_t dst = smem_u32(sKV + s * kSTile) + (64 * lw + 16 * part) * 128;
-            const int mine = part < 2 ? slot[0] : slot[1];
-            if ((((part < 2 ? in_row[0] : in_row[1]) >> (16 * (part & 1))) & 0xffffu) == 0xffffu) {
-              const int y = row0 + __shfl_sync(0xffffffffu, mine, 16 * (part & 1));
-              if (elect_one()) {
-                sa_tma_box(dst, box, &kv_full[s], 0, y);
-                sa_tma_box(dst + SKEYS * 128, box, &kv_full[s], 64, y);
-              }
-            } else {
-#pragma unroll
-              for (int g = 0; g < 4; ++g) {
-                int y[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) y[e] = row0 + __shfl_sync(0xffffffffu, mine, 16 * (part & 1) + 4 * g + e);
-                if (elect_one()) {
-                  sa_tma_rows(dst + g * 512, one, &kv_full[s], 0, y[0], y[1], y[2], y[3]);
-                  sa_tma_rows(dst + g * 512 + SKEYS * 128, one, &kv_full[s], 64, y[0], y[1], y[2], y[3]);
-                }
-                __syncwarp();
-              }
-            }
-            __syncwarp();
-          }
         }
       }
       sa_done(w);
     }
   } else if (warp == 8) {
-    // ================================================================ MMA issuer: QK of job n + 2 goes behind PV of job n
-    constexpr uint32_t idesc_qk = umma_idesc_bf16(SROWS, SKEYS), idesc_pv = umma_idesc_bf16(SROWS, SD) | (1u << 16);
-    const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ)), k_desc = umma_desc_sw128(smem_u32(sKV)), v_desc = sa_desc_mn(smem_u32(sKV), SKEYS * 128);
-    // PV follows QK by two jobs, so by three segments at most: their lengths wait in a ring (this warp writes and reads it)
-    struct Cursor { int job, nt, tile0, q0; bool two, more; };       // job within the segment, its length; K/V tiles and Q buffers before it
-    int wrote = 0, read = 0;
-    auto open_qk = [&](Cursor& c) {
-      c.job = 0;
-      c.more = sa_next(p, w);
-      if (c.more) { c.nt = w.nt; c.two = w.two; }
-      if (lane == 0) segs[wrote & 3] = c.more ? 2 * c.nt + c.two : 0;
-      ++wrote;
-      __syncwarp();
-    };
-    auto open_pv = [&](Cursor& c) {
-      const int v = segs[read++ & 3];
-      c.job = 0;
-      c.more = v != 0;
-      c.nt = v >> 1;
-      c.two = v & 1;
-    };
-    auto step = [&](Cursor& c, auto open) {                           // behind the current job
-      if (++c.job < (c.two ? 2 * c.nt : c.nt)) return;
-      c.tile0 += c.nt;
-      c.q0 += c.two ? 2 : 1;
-      open(c);
-    };
-    auto tile_of = [&](const Cursor& c) { return c.tile0 + (c.two ? c.job >> 1 : c.job); };
-    Cursor qk{0, 0, 0, 0, false, false}, pv{0, 0, 0, 0, false, false};
-    open_qk(qk);
-    open_pv(pv);
-    int nq = 0, np = 0;                         // jobs issued
+    // ================================================================ issuer of the first product: S = Q K^T of a job once the group's scores before it are read
+    // (An issuer's waits and MMAs of a job take 700 cycles, about as long as the MMAs run: one warp for both products held them up.)
+    constexpr uint32_t idesc = umma_idesc_bf16(SROWS, SKEYS);
+    const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ)), k_desc = umma_desc_sw128(smem_u32(sKV));
+    int n = 0, tile = 0, use = 0;               // jobs; K tiles and Q buffers of the segments before
     bool ok = true;
-    auto issue_qk = [&] {
-      const int jobs = qk.two ? 2 * qk.nt : qk.nt, side = qk.two ? qk.job & 1 : 0, use = qk.q0 + side, buf = use & 1, g = nq & 1;
-      if (qk.job <= side && !sa_wait(&q_full[buf], (use >> 1) & 1, p.status, kTimeoutFull, gave_up)) return false;
-      const int n = 2 * tile_of(qk), s = n % SSLOTS;
-      if (!sa_wait(&kv_full[s], (n / SSLOTS) & 1, p.status, kTimeoutFull, gave_up)) return false;
-      tc_fence_after();
-      if (elect_one()) {
-        const uint64_t a = q_desc + static_cast<uint64_t>(buf * (kSTile >> 4)), b = k_desc + static_cast<uint64_t>(s * (kSTile >> 4));
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          umma_f16(tmem + g * SKEYS, a + (k >> 2) * (SROWS * 128 >> 4) + 2 * (k & 3), b + (k >> 2) * (SKEYS * 128 >> 4) + 2 * (k & 3), idesc_qk, k != 0);
-        if (!qk.two || side == 1) umma_commit(&kv_empty[s]);
-        if (qk.job + (qk.two ? 2 : 1) >= jobs) umma_commit(&q_empty[buf]);
-        umma_commit(&s_full[g]);
-      }
-      __syncwarp();
-      ++nq;
-      step(qk, [&](Cursor& c) { sa_done(w); open_qk(c); });
-      return true;
-    };
-    auto issue_pv = [&] {
-      const int jobs = pv.two ? 2 * pv.nt : pv.nt, g = np & 1, n = 2 * tile_of(pv) + 1, s = n % SSLOTS;
-      if (!sa_wait(&kv_full[s], (n / SSLOTS) & 1, p.status, kTimeoutFull, gave_up)) return false;
-      const uint64_t b = v_desc + static_cast<uint64_t>(s * (kSTile >> 4));
-#pragma unroll
-      for (int half = 1; half >= 0; --half) {        // the second half of the keys is weighed first
-        if (!sa_wait(&p_full[2 * g + half], (np >> 1) & 1, p.status, kTimeoutAccum, gave_up)) return false;
+    while (ok && sa_next(p, w)) {
+      const int sides = w.two ? 2 : 1, jobs = w.nt * sides;
+      for (int job = 0; job < jobs; ++job, ++n) {
+        const int g = n & 1, side = w.two ? job & 1 : 0, buf = (use + side) & 1, slot = 2 * (tile + (w.two ? job >> 1 : job)), s = slot % SSLOTS;
+        if (job < sides && !(ok = sa_wait(&q_full[buf], ((use + side) >> 1) & 1, p.status, kTimeoutFull, gave_up))) break;
+        if (side == 0 && !(ok = sa_wait(&kv_full[s], (slot / SSLOTS) & 1, p.status, kTimeoutFull, gave_up))) break;
+        if (n >= 2 && !(ok = sa_wait(&s_read[g], ((n >> 1) - 1) & 1, p.status, kTimeoutAccum, gave_up))) break;
         tc_fence_after();
         if (elect_one()) {
+          const uint64_t a = q_desc + static_cast<uint64_t>(buf * (kQTile >> 4)), b = k_desc + static_cast<uint64_t>(s * (kKTile >> 4));
 #pragma unroll
-          for (int k = 4 * half; k < 4 * half + 4; ++k)
-            sa_mma_tmem_a(tmem + 256 + g * SD, tmem + g * SKEYS + k * 8, b + k * (2048 >> 4), idesc_pv, k != 4 || pv.job >= 2);
+          for (int k = 0; k < 8; ++k)
+            umma_f16(tmem + g * 128, a + (k >> 2) * (SROWS * 128 >> 4) + 2 * (k & 3), b + (k >> 2) * (SKEYS * 128 >> 4) + 2 * (k & 3), idesc, k != 0);
+          umma_commit(&s_full[g]);
+          if (side == sides - 1) umma_commit(&kv_empty[s]);
+          if (job + sides >= jobs) umma_commit(&q_empty[buf]);
         }
         __syncwarp();
       }
-      if (elect_one()) {
-        if (!pv.two || (pv.job & 1)) umma_commit(&kv_empty[s]);
-        if (pv.job + 2 >= jobs) umma_commit(&o_full[g]);
+      tile += w.nt;
+      use += sides;
+      sa_done(w);
+    }
+  } else if (warp == 12) {
+    // ================================================================ issuer of the second product: O += P V
+    constexpr uint32_t idesc = umma_idesc_bf16(SROWS, SD) | (1u << 16);
+    const uint64_t v_desc = sa_desc_mn(smem_u32(sKV), SKEYS * 128);
+    int n = 0, tile = 0;
+    bool ok = true;
+    while (ok && sa_next(p, w)) {
+      const int sides = w.two ? 2 : 1, jobs = w.nt * sides;
+      for (int job = 0; job < jobs; ++job, ++n) {
+        const int g = n & 1, slot = 2 * (tile + (w.two ? job >> 1 : job)) + 1, s = slot % SSLOTS;
+        if (!(ok = sa_wait(&kv_full[s], (slot / SSLOTS) & 1, p.status, kTimeoutFull, gave_up))) break;
+        if (!(ok = sa_wait(&p_full[g], (n >> 1) & 1, p.status, kTimeoutAccum, gave_up))) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint64_t b = v_desc + static_cast<uint64_t>(s * (kKTile >> 4));
+#pragma unroll
+          for (int k = 0; k < SKEYS / 16; ++k)
+            sa_mma_tmem_a(tmem + kColO + g * 128, tmem + g * 128 + kColP + k * 8, b + k * (2048 >> 4), idesc, k != 0 || job >= 2);
+          umma_commit(&pv_done[g]);
+          if (!w.two || (job & 1)) umma_commit(&kv_empty[s]);
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      ++np;
-      step(pv, open_pv);
-      return true;
-    };
-    while (ok && qk.more && nq < 2) ok = issue_qk();
-    while (ok && pv.more) {
-      ok = issue_pv();
-      if (ok && qk.more) ok = issue_qk();
+      tile += w.nt;
+      sa_done(w);
     }
   } else {
     // ================================================================ softmax and epilogue: one row a thread
     const int g = warp >> 2, row = (warp & 3) * 32 + lane, tok = row / p.G, sub = row % p.G;
     const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + t_lane + g * SKEYS, to = tmem + t_lane + 256 + g * SD;
-    int jobs_done = 0, segs_done = 0;           // of this group: phases of its barriers
+    const uint32_t ts = tmem + t_lane + g * 128, to = tmem + t_lane + kColO + g * 128;
+    int jobs_done = 0;                          // of this group: the phase of its barriers
     bool ok = true;
     while (ok && sa_next(p, w)) {
       const bool prefix = w.b < 0;
@@ -559,101 +522,71 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         if (!ok) break;
         tc_fence_after();
         if (!busy) {
-          tc_fence_before();
-          mbar_arrive(&p_full[2 * g]);
-          mbar_arrive(&p_full[2 * g + 1]);
+          mbar_arrive(&s_read[g]);
+          if (jobs_done > 0) ok = sa_wait(&pv_done[g], (jobs_done - 1) & 1, p.status, kTimeoutAccum, gave_up);      // an arrival counts for the job that it is for
+          if (!ok) break;
+          mbar_arrive(&p_full[g]);
           continue;
         }
-        // The halves of the scores pass through registers in the order 0, 1 for the maximum and 1, 0 for the exponentials: half 1 stays,
-        // half 0 is read again behind its back.  All 128 columns at once, and what becomes of them, take more than 168 registers.
-        uint32_t s0[64], s1[64];
-        auto load = [&](int half, uint32_t* sr) {
-          tmem_ld_32x32(ts + 64 * half, sr);
-          tmem_ld_32x32(ts + 64 * half + 32, sr + 32);
-        };
-        auto hide = [&](int half, uint32_t* sr) {       // scores of keys the row does not see
+        uint32_t sr[SKEYS];
+        tmem_ld_32x32(ts, sr);
+        tmem_ld_32x32(ts + 32, sr + 32);
+        sa_tmem_ld16(ts + 64, sr + 64);
+        tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive(&s_read[g]);
+        if (!all) {                             // scores of keys the row does not see
 #pragma unroll
-          for (int c = 0; c < 64; c += 32) {
-            const uint32_t see = valid ? sa_visible(p, w.s, prefix, end, node, bits, k0 + 64 * half + c) : 0u;
+          for (int c = 0; c < SKEYS; c += 32) {
+            const uint32_t see = valid ? sa_visible(p, w.s, prefix, end, node, bits, k0 + c) : 0u;
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
+            for (int j = 0; j < 32 && c + j < SKEYS; ++j)
               if (!((see >> j) & 1u)) sr[c + j] = 0xff800000u;      // -inf
           }
-        };
-        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        auto top = [&](const uint32_t* sr) {
-#pragma unroll
-          for (int j = 0; j < 64; j += 8)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) mx4[e] = fmaxf(fmaxf(mx4[e], __uint_as_float(sr[j + 2 * e])), __uint_as_float(sr[j + 2 * e + 1]));
-        };
-        auto landed = [&](uint32_t* sr) {       // and nothing of it is used before this point
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 64; ++j) asm volatile("" : "+r"(sr[j]));
-        };
-        load(0, s0);
-        landed(s0);
-        load(1, s1);
-        if (!all) hide(0, s0);
-        top(s0);
-        landed(s1);
-        if (!all) {
-          sa_tmem_st32(ts, s0);                 // for the second look
-          sa_tmem_st32(ts + 32, s0 + 32);
-          hide(1, s1);
-          sa_tmem_st_wait();
         }
-        top(s1);
-        load(0, s0);
-        const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int j = 0; j < SKEYS; j += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx4[e] = sa_max3(mx4[e], __uint_as_float(sr[j + 2 * e]), __uint_as_float(sr[j + 2 * e + 1]));
+        const float mx = sa_max3(sa_max3(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY) * p.scale_log2;
         // integer running maximum in the log2 domain: probabilities are exact powers of two apart whatever the pieces
-        const float m_new = fmaxf(m_run, ceilf(mx)), m_safe = m_new == -INFINITY ? 0.f : m_new;
-        const float alpha = exp2f(m_run - m_safe);
+        const float m_new = sa_max3(m_run, ceilf(mx), -INFINITY), m_safe = m_new == -INFINITY ? 0.f : m_new;
+        const float alpha = sa_exp2(m_run - m_safe);
         m_run = m_new;
         const uint64_t scale2 = sa_pack(p.scale_log2, p.scale_log2), shift2 = sa_pack(-m_safe, -m_safe);
         uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
-        auto weigh = [&](const uint32_t* sr, uint32_t* pr) {      // 32 scores
+        uint32_t pr[SKEYS / 2];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            float p0, p1;
-            sa_unpack(sa_fma2(sa_pack(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), scale2, shift2), p0, p1);
-            p0 = sa_exp2(p0);
-            p1 = sa_exp2(p1);
-            sum2[j & 3] = sa_add2(sum2[j & 3], sa_pack(p0, p1));
-            const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);      // the MMA's operand: bf16, the sum keeps fp32
-            pr[j] = *reinterpret_cast<const uint32_t*>(&v);
-          }
-        };
-        auto publish = [&](int half) {
-          sa_tmem_st_wait();
-          tc_fence_before();
-          mbar_arrive(&p_full[2 * g + half]);
-        };
-        uint32_t pr[16];
-        weigh(s1, pr);
-        landed(s0);                             // half 0 is in registers: probabilities may take its place
-        // every earlier PV of this group ended before these scores did
+        for (int j = 0; j < SKEYS / 2; ++j) {
+          float p0, p1;
+          sa_unpack(sa_fma2(sa_pack(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), scale2, shift2), p0, p1);
+          p0 = sa_exp2(p0);
+          p1 = sa_exp2(p1);
+          sum2[j & 3] = sa_add2(sum2[j & 3], sa_pack(p0, p1));
+          const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);      // the MMA's operand: bf16, the sum keeps fp32
+          pr[j] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        // this group's PV before: its probabilities are read, its output is complete
+        if (jobs_done > 0) ok = sa_wait(&pv_done[g], (jobs_done - 1) & 1, p.status, kTimeoutAccum, gave_up);
+        if (!ok) break;
+        tc_fence_after();
+        sa_tmem_st32(ts + kColP, pr);
+        sa_tmem_st8(ts + kColP + 32, pr + 32);
         if (__any_sync(0xffffffffu, valid && jobs > 0 && alpha != 1.f)) {
 #pragma unroll 1
-          for (int c = 0; c < SD; c += 16) {
-            uint32_t o[16];
-            sa_tmem_ld16(to + c, o);
+          for (int c = 0; c < SD; c += 32) {
+            uint32_t o[32];
+            tmem_ld_32x32(to + c, o);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
-            sa_tmem_st16(to + c, o);
+            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * alpha);
+            sa_tmem_st32(to + c, o);
           }
         }
-        sa_tmem_st16(ts + 32, pr);
-        weigh(s1 + 32, pr);
-        sa_tmem_st16(ts + 48, pr);
-        publish(1);
-        weigh(s0, pr);
-        sa_tmem_st16(ts, pr);
-        weigh(s0 + 32, pr);
-        sa_tmem_st16(ts + 16, pr);
-        publish(0);
+        sa_tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[g]);
         float sum_lo, sum_hi;
         sa_unpack(sa_add2(sa_add2(sum2[0], sum2[1]), sa_add2(sum2[2], sum2[3])), sum_lo, sum_hi);
         l_run = l_run * alpha + (sum_lo + sum_hi);
@@ -666,9 +599,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const size_t seg = static_cast<size_t>(blockIdx.x) + (prefix ? item : item - p.prefix_items);
       const size_t at = (seg * 2 + rel) * rows + row;
       if (jobs > 0) {
-        ok = sa_wait(&o_full[g], segs_done & 1, p.status, kTimeoutAccum, gave_up);
+        ok = sa_wait(&pv_done[g], (jobs_done - 1) & 1, p.status, kTimeoutAccum, gave_up);
         if (!ok) break;
-        ++segs_done;
         tc_fence_after();
         const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
 #pragma unroll 1
