@@ -6,19 +6,24 @@
 // inverse CDF with v from p_n when a == n, else from max(p_a - q_a, 0): the committed tokens are then samples of the target.
 // A temperature below 1e-5 is a point mass at the lowest most likely index.
 //
-// Two launches.  chain_stats_kernel reads the rows once (maximum, sum of exponentials, index of the maximum), the rows of the first
-// drafts before those of later ones; a row behind a draft already known to be rejected is left out.  chain_token_kernel decides, and draws the
-// token with a cluster per sequence.  Sums that only decide `u q < p` are fp32 (a decision is off by 1e-7 of a probability); the
-// running sum that a token is found in is fp64, as its index would change with every rounding among 150,000 terms.
+// chain_stats_kernel reads the rows of some drafts (maximum, sum of exponentials) and decides about them; chain_token_kernel draws the token, a
+// cluster per sequence.  Where reading every row would take long, the first kernel runs for draft 0 of all sequences, then 1, 2, 3-4, 5-8 and the
+// rest, so that rows behind a rejection are not read.  (Measured at 64 sequences of 4 to 16 drafts over 151936 fp32 values, a third of the rows
+// needed: one persistent launch that picks drafts as they become known to be needed reads half of what it reads in vain and
+// waits for its own agreements, 136 us; launches in turn: see below.)  Sums that only decide `u q < p` are fp32 (a decision is off by 1e-7 of a
+// probability); the running sum that a token is found in is fp64, as its index would change with every rounding among 150,000 terms.
 #include "common.cuh"
 
 #include <math.h>
+#include <type_traits>
 
 namespace js {
 
+constexpr int kStatThreads = 256, kStatBlocks = 4;      // a block of the first kernel reads 4 x 16 bytes a thread of either row at once: 16 KB each
+constexpr int kChunkBytes = kStatThreads * kStatBlocks * 16;
 constexpr int kChainThreads = 512;
-constexpr int kChainCluster = 8;      // CTAs that share a sequence's last row
 constexpr float kGreedyBelow = 1e-5f;
+constexpr int kNoneRejected = 0x7fffffff;
 
 struct ChainParams {
   const void *target, *draft;          // (D + B, V), (D, V)
@@ -27,8 +32,10 @@ struct ChainParams {
   const float *accept_u, *sample_u;    // (D), (B)
   const float *temp, *draft_temp;      // (B), or null: the scalars
   double temp_all, draft_temp_all;
-  float4* stats;                       // (rows, chunks) of both matrices, the draft's behind the target's: maximum, sum, index of the maximum
-  int* rejected;                       // (B) a bound on the first rejected draft (all ones bytes 0x7f: none known)
+  float4* stats;                       // (rows, chunks) of both matrices, the draft's behind the target's: maximum, sum, index of the maximum;
+                                       // chunk 0 has the row's own figures in the end
+  int* rejected;                       // (B) kNoneRejected - i for the first draft i known to be rejected, 0: none; zero at the start
+  int* arrived;                        // (D + B) chunks of a target row (and its draft row) that are there; zero at the start
   int* accepted;
   long long* token;
   int* status;
@@ -50,215 +57,292 @@ JS_DEVICE int chain_span(const ChainParams& p, int b, int& first) {
   return max(0, min(p.cu[b + 1], p.D) - first);
 }
 
-// Base-2 exponent of a difference of logits: log2(e) / T as the sum of two fp32, so that the factor's rounding does not weigh on every term
-struct ChainScale { float hi, lo; };
-JS_DEVICE ChainScale chain_scale(double temp) {
-  const double f = temp < kGreedyBelow ? 1.0 : 1.4426950408889634 / temp;
-  const float hi = static_cast<float>(f);
-  return ChainScale{hi, static_cast<float>(f - hi)};
-}
-JS_DEVICE float chain_exp(float d, const ChainScale& f) {
-  d = fmaxf(d, -1e30f);      // -inf would meet the other part's sign
-  return exp2f(fmaf(d, f.hi, d * f.lo));
+// log2(e) / T.  Its rounding to fp32 is a change of the temperature by about 2^-23 of itself, for the sum and the drafted token alike.
+JS_DEVICE float chain_scale(double temp) { return temp < kGreedyBelow ? 1.f : 1.44269504f / static_cast<float>(temp); }
+// What a row's exponents are relative to: its maximum in the log2 domain, rounded the same way wherever it is needed.
+JS_DEVICE float chain_base(float m, float scale) { return __fmul_rn(m, scale); }
+JS_DEVICE float chain_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
 struct RowStat { float m, s; int at; };      // maximum, sum of the exponentials relative to it, lowest index of the maximum
-JS_DEVICE RowStat join(const RowStat& a, const RowStat& b, const ChainScale& f) {
+JS_DEVICE RowStat join(const RowStat& a, const RowStat& b, float scale) {
   RowStat r;
   r.m = fmaxf(a.m, b.m);
   r.at = a.m > b.m ? a.at : b.m > a.m ? b.at : min(a.at, b.at);
-  r.s = (a.m == r.m ? a.s : a.s != 0.f ? a.s * chain_exp(a.m - r.m, f) : 0.f) +
-        (b.m == r.m ? b.s : b.s != 0.f ? b.s * chain_exp(b.m - r.m, f) : 0.f);
+  const float base = chain_base(r.m, scale);
+  r.s = (a.m == r.m ? a.s : a.s != 0.f ? a.s * chain_exp2(chain_base(a.m, scale) - base) : 0.f) +
+        (b.m == r.m ? b.s : b.s != 0.f ? b.s * chain_exp2(chain_base(b.m, scale) - base) : 0.f);
   return r;
 }
-
-// The figures of elements [lo, hi) of a row, by the whole block
-template <typename T>
-JS_DEVICE RowStat row_stat(const T* x, int lo, int hi, const ChainScale& f, RowStat* red) {
-  constexpr int N = 16 / sizeof(T);
-  RowStat r{-INFINITY, 0.f, 0x7fffffff};
-  auto one = [&](float v, int i) {
-    if (v > r.m) {
-      r.s = r.s * chain_exp(r.m - v, f) + 1.f;
-      r.m = v;
-      r.at = i;
-    } else {
-      r.s += chain_exp(v - r.m, f);
-    }
-  };
-  // elements ahead of the first 16-byte boundary, then vectors, then the rest
-  const int lead = min(hi - lo, static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(x + lo) & 15)) & 15) / sizeof(T)));
-  const int n_vec = (hi - lo - lead) / N, tail = lo + lead + n_vec * N;
-  if (threadIdx.x < lead) one(chain_f(x[lo + threadIdx.x]), lo + threadIdx.x);
-  const uint4* v = reinterpret_cast<const uint4*>(x + lo + lead);
-#pragma unroll 4
-  for (int i = threadIdx.x; i < n_vec; i += kChainThreads) {
-    const uint4 w = __ldg(v + i);
-    const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-    for (int j = 0; j < N; ++j) one(chain_f(e[j]), lo + lead + i * N + j);
-  }
-  if (tail + static_cast<int>(threadIdx.x) < hi) one(chain_f(x[tail + threadIdx.x]), tail + threadIdx.x);
+JS_DEVICE RowStat warp_join(RowStat r, float scale) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const RowStat other{__shfl_xor_sync(0xffffffffu, r.m, o), __shfl_xor_sync(0xffffffffu, r.s, o), __shfl_xor_sync(0xffffffffu, r.at, o)};
-    r = join(r, other, f);
+    r = join(r, other, scale);
   }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = r;
-  __syncthreads();
-  r = red[0];
-  for (int w = 1; w < kChainThreads / 32; ++w) r = join(r, red[w], f);
   return r;
 }
 
 // probability of the element at `index`, whose logit is `x`
 JS_DEVICE double chain_prob(float x, int index, double temp, const RowStat& st) {
   if (temp < kGreedyBelow) return index == st.at ? 1.0 : 0.0;
-  return st.s > 0.f ? exp2((static_cast<double>(x) - st.m) * (1.4426950408889634 / temp)) / st.s : 0.0;
+  const float scale = chain_scale(temp);
+  return st.s > 0.f ? exp2(static_cast<double>(x) * scale - chain_base(st.m, scale)) / st.s : 0.0;
 }
 
+// A row as the 16-byte blocks that hold it: a copy starts and ends with a block, and never leaves the blocks that the row has a part in.
+struct ChainRow {
+  const uint8_t* start;
+  int bytes, ahead;            // of all blocks; values of the first block ahead of the row
+  template <typename T>
+  JS_DEVICE void set(const T* row, int V) {
+    const uintptr_t from = reinterpret_cast<uintptr_t>(row) & ~uintptr_t(15);
+    start = reinterpret_cast<const uint8_t*>(from);
+    ahead = static_cast<int>(reinterpret_cast<uintptr_t>(row) - from) / static_cast<int>(sizeof(T));
+    bytes = (static_cast<int>((ahead + V) * sizeof(T)) + 15) & ~15;
+  }
+};
+
+JS_DEVICE float chain_max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+JS_DEVICE float warp_max_f32(float v) {
+  float r;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+// One chunk of the rows of drafts lo + z, lo + z + Z, ... below hi of a sequence: block (chunk, sequence, z).
 template <typename T>
-__global__ void __launch_bounds__(kChainThreads) chain_stats_kernel(ChainParams p) {
-  __shared__ RowStat red[kChainThreads / 32];
-  __shared__ int longest, known;
-  const int tid = threadIdx.x;
-  if (tid == 0) longest = 0;
-  __syncthreads();
-  int most = 0;
-  for (int b = tid; b < p.B; b += kChainThreads) { int f; most = max(most, chain_span(p, b, f)); }
-  if (most > 0) atomicMax(&longest, most);
-  __syncthreads();
-  const long long tasks = static_cast<long long>(longest + 1) * p.B * p.chunks;
-  for (long long k = blockIdx.x; k < tasks; k += gridDim.x) {
-    const int chunk = k % p.chunks, b = (k / p.chunks) % p.B, i = k / p.chunks / p.B;
-    int first;
-    const int n = chain_span(p, b, first);
-    if (i > n) continue;
+__global__ void __launch_bounds__(kStatThreads, 4) chain_stats_kernel(ChainParams p, int lo, int hi) {
+  constexpr int N = 16 / sizeof(T), kWarps = kStatThreads / 32;
+  __shared__ float tops[2][kWarps], sums[2][kWarps];
+  __shared__ int where[2], go;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, chunk = blockIdx.x, b = blockIdx.y;
+  pdl_launch_dependents();
+  int first;
+  const int n = chain_span(p, b, first);
+  if (lo + static_cast<int>(blockIdx.z) > n) return;
+  const double temps[2] = {chain_temp(p.temp, p.temp_all, b), chain_temp(p.draft_temp, p.draft_temp_all, b)};
+  const float scales[2] = {chain_scale(temps[0]), chain_scale(temps[1])};
+  pdl_wait();                                  // what the launch before decided
+  for (int i = lo + blockIdx.z; i < hi && i <= n; i += gridDim.z) {
+    // Behind a known rejection nobody needs the rows; whether they are read all the same goes by time, results do not.
     __syncthreads();
-    if (tid == 0) known = *reinterpret_cast<volatile int*>(p.rejected + b);
+    if (tid == 0) go = kNoneRejected - *reinterpret_cast<volatile int*>(p.rejected + b) >= i;
+    if (tid < 2) where[tid] = 0x7fffffff;
     __syncthreads();
-    if (known < i) continue;              // nobody needs these rows; whether they are read all the same goes by time, results do not
-    const int lo = static_cast<long long>(p.V) * chunk / p.chunks, hi = static_cast<long long>(p.V) * (chunk + 1) / p.chunks;
-    const long long trow = first + b + i;
-    const T* x = reinterpret_cast<const T*>(p.target) + trow * p.ldt;
-    const double tt = chain_temp(p.temp, p.temp_all, b), td = chain_temp(p.draft_temp, p.draft_temp_all, b);
-    const RowStat st = row_stat(x, lo, hi, chain_scale(tt), red);
-    if (tid == 0) p.stats[trow * p.chunks + chunk] = make_float4(st.m, st.s, __int_as_float(st.at), 0.f);
-    if (i == n) continue;
-    const long long drow = first + i;
-    const T* y = reinterpret_cast<const T*>(p.draft) + drow * p.ldd;
-    const RowStat sd = row_stat(y, lo, hi, chain_scale(td), red);
-    if (tid == 0) {
-      p.stats[(p.D + p.B + drow) * p.chunks + chunk] = make_float4(sd.m, sd.s, __int_as_float(sd.at), 0.f);
-      const int tok = p.drafts[drow];
-      if (p.chunks == 1 && (tok < 0 || tok >= p.V ||
-          !(p.accept_u[drow] * chain_prob(chain_f(y[tok]), tok, td, sd) < chain_prob(chain_f(x[tok]), tok, tt, st))))
-        atomicMin(p.rejected + b, i);
+    if (!go) return;
+    const long long trow = static_cast<long long>(first) + b + i, drow = static_cast<long long>(first) + i;
+    const T* rows[2] = {reinterpret_cast<const T*>(p.target) + trow * p.ldt, reinterpret_cast<const T*>(p.draft) + drow * p.ldd};
+    uint4 raw[2][kStatBlocks];
+    int ahead[2];
+#pragma unroll
+    for (int row = 0; row < 2; ++row) {
+      ChainRow r{nullptr, 0, 0};
+      if (row == 0 || i < n) r.set(rows[row], p.V);
+      ahead[row] = r.ahead;
+      const int left = r.bytes - chunk * kChunkBytes;
+#pragma unroll
+      for (int q = 0; q < kStatBlocks; ++q) {
+        const int at = (q * kStatThreads + tid) * 16;
+        constexpr uint32_t kNone = sizeof(T) == 4 ? 0xff800000u : 0xff80ff80u;      // -inf
+        raw[row][q] = make_uint4(kNone, kNone, kNone, kNone);
+        if (at < left) raw[row][q] = __ldg(reinterpret_cast<const uint4*>(r.start + static_cast<size_t>(chunk) * kChunkBytes + at));
+      }
     }
+    constexpr int kChunk = kChunkBytes / static_cast<int>(sizeof(T));
+    auto value = [&](int row, int q, int c) {  // value c of this thread's block q
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(&raw[row][q]);
+      if constexpr (sizeof(T) == 4) return __uint_as_float(w[c]);
+      else return __uint_as_float(c & 1 ? w[c >> 1] & 0xffff0000u : w[c >> 1] << 16);
+    };
+    auto index = [&](int row, int q, int c) { return chunk * kChunk + (q * kStatThreads + tid) * N + c - ahead[row]; };
+#pragma unroll
+    for (int row = 0; row < 2; ++row) {
+      if (ahead[row] == 0 && (chunk + 1) * kChunk <= p.V) continue;
+      // a chunk at an end of the row: what is not the row's is -inf
+#pragma unroll
+      for (int q = 0; q < kStatBlocks; ++q) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&raw[row][q]);
+#pragma unroll
+        for (int c = 0; c < N; ++c) {
+          const int at = index(row, q, c);
+          if (at >= 0 && at < p.V) continue;
+          if constexpr (sizeof(T) == 4) w[c] = 0xff800000u;
+          else w[c >> 1] = c & 1 ? (w[c >> 1] & 0xffffu) | 0xff800000u : (w[c >> 1] & 0xffff0000u) | 0xff80u;
+        }
+      }
+    }
+    float tops2[2];
+#pragma unroll
+    for (int row = 0; row < 2; ++row) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < kStatBlocks; ++q)
+#pragma unroll
+        for (int c = 0; c < N; c += 2) top = chain_max3(top, value(row, q, c), value(row, q, c + 1));
+      top = warp_max_f32(top);
+      if (lane == 0) tops[row][warp] = top;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int row = 0; row < 2; ++row) {
+      float top = warp_max_f32(tops[row][lane % kWarps]);
+      if (row == 1 && i == n) top = -INFINITY;
+      tops2[row] = top;
+      float sum = 0.f;
+      if (top != -INFINITY) {
+        const float base = -chain_base(top, scales[row]);
+        float e[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int q = 0; q < kStatBlocks; ++q)
+#pragma unroll
+          for (int c = 0; c < N; ++c) e[c & 3] += chain_exp2(fmaf(value(row, q, c), scales[row], base));
+        sum = (e[0] + e[1]) + (e[2] + e[3]);
+        if (temps[row] < kGreedyBelow) {       // only a point mass wants to know where the maximum is
+#pragma unroll
+          for (int q = 0; q < kStatBlocks; ++q)
+#pragma unroll
+            for (int c = 0; c < N; ++c) if (value(row, q, c) == top) atomicMin(&where[row], index(row, q, c));
+        }
+      }
+      sum = warp_sum(sum);
+      if (lane == 0) sums[row][warp] = sum;
+    }
+    __syncthreads();
+    if (warp != 0) continue;
+    RowStat st{tops2[0], 0.f, where[0]}, sd{tops2[1], 0.f, where[1]};
+    for (int w = 0; w < kWarps; ++w) {
+      st.s += sums[0][w];
+      sd.s += sums[1][w];
+    }
+    float4 *tstat = p.stats + trow * p.chunks, *dstat = p.stats + (p.D + p.B + drow) * p.chunks;
+    if (p.chunks > 1) {                        // the last chunk to arrive joins them all, in order
+      int there = 0;
+      if (lane == 0) {
+        __stcg(tstat + chunk, make_float4(st.m, st.s, __int_as_float(st.at), 0.f));
+        if (i < n) __stcg(dstat + chunk, make_float4(sd.m, sd.s, __int_as_float(sd.at), 0.f));
+        asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(there) : "l"(p.arrived + trow) : "memory");
+      }
+      if (__shfl_sync(0xffffffffu, there, 0) != p.chunks - 1) continue;
+      __threadfence();
+      auto all = [&](const float4* at, float scale) {
+        RowStat r{-INFINITY, 0.f, 0x7fffffff};
+        for (int c = lane; c < p.chunks; c += 32) {
+          const float4 v = __ldcg(at + c);
+          r = join(r, RowStat{v.x, v.y, __float_as_int(v.z)}, scale);
+        }
+        return warp_join(r, scale);
+      };
+      st = all(tstat, scales[0]);
+      if (i < n) sd = all(dstat, scales[1]);
+      __syncwarp();
+    }
+    if (lane != 0) continue;
+    tstat[0] = make_float4(st.m, st.s, __int_as_float(st.at), 0.f);
+    if (i == n) continue;
+    dstat[0] = make_float4(sd.m, sd.s, __int_as_float(sd.at), 0.f);
+    const int tok = p.drafts[drow];
+    const bool known = tok >= 0 && tok < p.V;
+    if (!known) report(p.status, kBadToken);
+    if (!known || !(p.accept_u[drow] * chain_prob(chain_f(rows[1][tok]), tok, temps[1], sd) < chain_prob(chain_f(rows[0][tok]), tok, temps[0], st)))
+      atomicMax(p.rejected + b, kNoneRejected - i);
   }
 }
 
-// 2^t for t <= 0 (0 below 2^-1000): t = n / 32 + r, a table of 2^(j/32) and the series of e^(r ln 2) to the fourth power, |r| <= 1/64
-// (P. Tang's table-driven scheme): relative error below 2e-12.
+// 2^(t / 512) for t from -512,000 to 0: t = n + r, a table of 2^(j/512) and the series of 2^(r/512) to the second power, |r| <= 1/2
+// (P. Tang's table-driven scheme): relative error below 6e-11, of either sign.
+constexpr int kExpTable = 512;
 JS_DEVICE double exp2_table(double t, const double* table) {
-  if (!(t > -1000.0)) return 0.0;
-  const double shifted = t * 32.0 + 6755399441055744.0;      // 1.5 * 2^52: the integer part of the sum's low word
+  constexpr double kRound = 6755399441055744.0;              // 1.5 * 2^52: the integer part of the sum's low word
+  constexpr double c1 = 0.69314718055994531 / kExpTable;
+  const double shifted = t + kRound;
   const int n = __double2loint(shifted);
-  const double r = (t * 32.0 - (shifted - 6755399441055744.0)) * (0.69314718055994531 / 32.0);
-  const double e = fma(r, fma(r, fma(r, fma(r, 1.0 / 24.0, 1.0 / 6.0), 0.5), 1.0), 1.0);
-  const double scale = __hiloint2double(((n >> 5) + 1023) << 20, 0);
-  return e * table[n & 31] * scale;
+  const double r = t - (shifted - kRound);
+  const double e = fma(r, fma(r, c1 * c1 / 2.0, c1), 1.0) * table[n & (kExpTable - 1)];
+  return __hiloint2double(__double2hiint(e) + ((n >> 9) << 20), __double2loint(e));
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kChainThreads) chain_token_kernel(ChainParams p) {
+// CLUSTER CTAs share a sequence's last row.
+template <typename T, int CLUSTER>
+__global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainParams p) {
   constexpr int kWarps = kChainThreads / 32;
-  __shared__ double table[32], part[kWarps], sums[kChainCluster][2];
-  __shared__ RowStat tstat, dstat;
-  __shared__ int first_bad, passing, holding;
+  __shared__ double table[kExpTable], part[kWarps], part2[kWarps], sums[CLUSTER][2];
+  __shared__ int passing, holding;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = static_cast<int>(cluster_ctarank());
-  const int b = blockIdx.x / kChainCluster;
-  if (tid < 32) table[tid] = exp2(tid / 32.0);
-  int first;
-  const int n = chain_span(p, b, first);
-  const double tt = chain_temp(p.temp, p.temp_all, b), td = chain_temp(p.draft_temp, p.draft_temp_all, b);
-  const T* target = reinterpret_cast<const T*>(p.target);
-  const T* draft = reinterpret_cast<const T*>(p.draft);
-  auto stat_of = [&](long long row, const ChainScale& f) {
-    RowStat r{-INFINITY, 0.f, 0x7fffffff};
-    for (int c = 0; c < p.chunks; ++c) {
-      const float4 v = p.stats[row * p.chunks + c];
-      r = join(r, RowStat{v.x, v.y, __float_as_int(v.z)}, f);
-    }
-    return r;
-  };
-  const ChainScale tf = chain_scale(tt), df = chain_scale(td);
+  const int b = blockIdx.x / CLUSTER;
+  static_assert(kExpTable == kChainThreads, "an entry a thread");
+  table[tid] = exp2(static_cast<double>(tid) / kExpTable);
   if (tid == 0) {
-    first_bad = min(n, p.rejected[b]);
     passing = 0x7fffffff;
     holding = -1;
   }
-  __syncthreads();
-  // Every CTA of the cluster decides for itself.  Rows behind the first rejection may hold no figures: what is decided there does not count.
-  for (int i = tid; i < n; i += kChainThreads) {
-    const int tok = p.drafts[first + i];
-    const long long trow = first + b + i, drow = first + i;
-    bool good = tok >= 0 && tok < p.V;
-    if (good)
-      good = p.accept_u[drow] * chain_prob(chain_f(draft[drow * p.ldd + tok]), tok, td, stat_of(p.D + p.B + drow, df)) <
-             chain_prob(chain_f(target[trow * p.ldt + tok]), tok, tt, stat_of(trow, tf));
-    else if (rank == 0)
-      report(p.status, kBadToken);
-    if (!good) atomicMin(&first_bad, i);
-  }
-  __syncthreads();
-  const int a = first_bad;
+  pdl_wait();
+  int first;
+  const int n = chain_span(p, b, first);
+  const double tt = chain_temp(p.temp, p.temp_all, b), td = chain_temp(p.draft_temp, p.draft_temp_all, b);
+  const int a = min(n, kNoneRejected - p.rejected[b]);
   const bool left = a < n;                // draw from the difference
   const long long trow = first + b + a, drow = first + a;
-  if (tid == 0) {
-    tstat = stat_of(trow, tf);
-    if (left) dstat = stat_of(p.D + p.B + drow, df);
-    if (rank == 0) p.accepted[b] = a;
-  }
+  const float4 tstat = p.stats[trow * p.chunks], dstat = left ? p.stats[(p.D + p.B + drow) * p.chunks] : make_float4(0.f, 0.f, 0.f, 0.f);
+  const int t_at = __float_as_int(tstat.z), d_at = __float_as_int(dstat.z);      // where a point mass lies
+  if (rank == 0 && tid == 0) p.accepted[b] = a;
   __syncthreads();
-  const T* x = target + trow * p.ldt;
-  const T* y = draft + drow * p.ldd;
-  const int most_likely = tstat.at < p.V ? tstat.at : -1;       // -1: no index has a probability
-  if (tt < kGreedyBelow || most_likely < 0) {                   // the same for the whole cluster
-    if (rank == 0 && tid == 0) p.token[b] = most_likely;
+  const T* x = reinterpret_cast<const T*>(p.target) + trow * p.ldt;
+  const T* y = reinterpret_cast<const T*>(p.draft) + drow * p.ldd;
+  if (tt < kGreedyBelow || tstat.x == -INFINITY) {              // the same for the whole cluster; without a logit above -inf: no token
+    if (rank == 0 && tid == 0) p.token[b] = t_at < p.V ? t_at : -1;
     return;
   }
-  const double ts = 1.4426950408889634 / tt, ds = 1.4426950408889634 / td;
-  const float tm = tstat.m, dm = left ? dstat.m : 0.f;
+  const double ts = kExpTable * 1.4426950408889634 / tt, ds = kExpTable * 1.4426950408889634 / td;
+  const double tc = -tstat.x * ts, dc = -dstat.x * ds;
+  // logits below these have a probability under 2^-1000: none
+  const float t_least = static_cast<float>((-1000.0 * kExpTable - tc) / ts), d_least = static_cast<float>((-1000.0 * kExpTable - dc) / ds);
   const bool draft_point = td < kGreedyBelow;
-  auto ep = [&](int i) { return exp2_table((static_cast<double>(chain_f(x[i])) - tm) * ts, table); };
-  auto eq = [&](int i) {
-    return draft_point ? (i == dstat.at ? 1.0 : 0.0) : exp2_table((static_cast<double>(chain_f(y[i])) - dm) * ds, table);
+  auto ep = [&](float v) { return v > t_least ? exp2_table(fma(static_cast<double>(v), ts, tc), table) : 0.0; };
+  auto eq = [&](float v, int i) {
+    if (draft_point) return i == d_at ? 1.0 : 0.0;
+    return v > d_least ? exp2_table(fma(static_cast<double>(v), ds, dc), table) : 0.0;
   };
   // A CTA takes a slice of the vocabulary and a warp a slice of that, so sums follow the order of the indices.
-  const int lo = static_cast<long long>(p.V) * rank / kChainCluster, size = static_cast<int>(static_cast<long long>(p.V) * (rank + 1) / kChainCluster) - lo;
+  const int lo = static_cast<long long>(p.V) * rank / CLUSTER, size = static_cast<int>(static_cast<long long>(p.V) * (rank + 1) / CLUSTER) - lo;
   auto warp_lo = [&](int w) { return lo + static_cast<int>(static_cast<long long>(size) * w / kWarps); };
-  auto warp_sum64 = [&](double v) {
+  // f(index, target logit, draft logit) for this warp's elements; four at a time, as fp64 chains are long
+  auto each = [&](auto f) {
+    const int end = warp_lo(warp + 1);
+    int i = warp_lo(warp) + lane;
+    for (; i + 96 < end; i += 128) {
+      float v[4], w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = chain_f(x[i + 32 * j]);
+        w[j] = left ? chain_f(y[i + 32 * j]) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(i + 32 * j, v[j], w[j]);
+    }
+    for (; i < end; i += 32) f(i, chain_f(x[i]), left ? chain_f(y[i]) : 0.f);
+  };
+  // the warps' sums into `to`; their sum in order
+  auto block_sum = [&](double v, double* to) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-  };
-  // the warps' sums into `part`; their sum in order
-  auto block_sum = [&](double v) {
-    v = warp_sum64(v);
-    __syncthreads();
-    if (lane == 0) part[warp] = v;
+    if (lane == 0) to[warp] = v;
     __syncthreads();
     v = 0.0;
-    for (int w = 0; w < kWarps; ++w) v += part[w];
+    for (int w = 0; w < kWarps; ++w) v += to[w];
     return v;
   };
   // this CTA's pair of sums to every CTA of the cluster
   auto exchange = [&](double s0, double s1) {
     cluster_sync();                       // every CTA of the cluster runs, and is done with the sums of before
-    if (tid < kChainCluster) {
+    if (tid < CLUSTER) {
       const uint32_t at = map_to_cta(smem_u32(&sums[rank][0]), tid);
       asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at), "d"(s0) : "memory");
       asm volatile("st.shared::cluster.f64 [%0], %1;" ::"r"(at + 8), "d"(s1) : "memory");
@@ -269,33 +353,36 @@ __global__ void __launch_bounds__(kChainThreads) chain_token_kernel(ChainParams 
   double ip = 1.0, iq = 0.0;
   if (left) {
     double sp = 0.0, sq = 0.0;
-    for (int i = lo + tid; i < lo + size; i += kChainThreads) {
-      sp += ep(i);
-      sq += eq(i);
-    }
-    sp = block_sum(sp);
-    sq = block_sum(sq);
+    each([&](int i, float v, float w) {
+      sp += ep(v);
+      sq += eq(w, i);
+    });
+    sp = block_sum(sp, part);
+    sq = block_sum(sq, part2);
     exchange(sp, sq);
     sp = sq = 0.0;
-    for (int c = 0; c < kChainCluster; ++c) {
+    for (int c = 0; c < CLUSTER; ++c) {
       sp += sums[c][0];
       sq += sums[c][1];
     }
     ip = 1.0 / sp;
     iq = sq > 0.0 ? 1.0 / sq : 0.0;
   }
-  auto weight = [&](int i) {
-    const double w = left ? ep(i) * ip - eq(i) * iq : ep(i);
-    return w > 0.0 ? w : 0.0;
+  auto weight = [&](int i, float v, float w) {
+    const double r = left ? ep(v) * ip - eq(w, i) * iq : ep(v);
+    return r > 0.0 ? r : 0.0;
   };
   double sum = 0.0;
-  for (int i = warp_lo(warp) + lane; i < warp_lo(warp + 1); i += 32) sum += weight(i);
-  sum = block_sum(sum);
+  each([&](int i, float v, float w) { sum += weight(i, v, w); });
+  sum = block_sum(sum, part);
   exchange(sum, 0.0);
   double total = 0.0;
-  for (int c = 0; c < kChainCluster; ++c) total += sums[c][0];
-  if (!(total > 0.0)) {                   // rounding left nothing of the difference
-    if (rank == 0 && tid == 0) p.token[b] = most_likely;
+  for (int c = 0; c < CLUSTER; ++c) total += sums[c][0];
+  if (!(total > 0.0)) {                   // rounding left nothing of the difference: the target's most likely token
+    if (rank != 0) return;
+    for (int i = p.V - 1 - tid; i >= 0; i -= kChainThreads) if (chain_f(x[i]) == tstat.x) atomicMin(&passing, i);
+    __syncthreads();
+    if (tid == 0) p.token[b] = passing < p.V ? passing : -1;
     return;
   }
   // The first of `count` parts whose running sum passes the goal, or (where rounding lets none pass it) the last one with a weight;
@@ -317,13 +404,14 @@ __global__ void __launch_bounds__(kChainThreads) chain_token_kernel(ChainParams 
     return last;
   };
   double run = 0.0;
-  if (find(kChainCluster, [&](int c) { return sums[c][0]; }, run) != rank) return;
+  if (find(CLUSTER, [&](int c) { return sums[c][0]; }, run) != rank) return;
   const int w = find(kWarps, [&](int c) { return part[c]; }, run);
   // the warp's slice once more, a few neighbouring elements a thread
   const int from = warp_lo(w), to = warp_lo(w + 1), per = (to - from + kChainThreads - 1) / kChainThreads;
   const int mine = min(to, from + tid * per), stop = min(to, mine + per);
+  auto at = [&](int i) { return weight(i, chain_f(x[i]), left ? chain_f(y[i]) : 0.f); };
   sum = 0.0;
-  for (int i = mine; i < stop; ++i) sum += weight(i);
+  for (int i = mine; i < stop; ++i) sum += at(i);
   double inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -342,42 +430,90 @@ __global__ void __launch_bounds__(kChainThreads) chain_token_kernel(ChainParams 
   __syncthreads();
   if (tid == (passing != 0x7fffffff ? passing : holding)) {
     ahead += inc - sum;
-    const int i = find(stop - mine, [&](int c) { return weight(mine + c); }, ahead);
-    p.token[b] = mine + i;
+    p.token[b] = mine + find(stop - mine, [&](int c) { return at(mine + c); }, ahead);
   }
 }
 
-template <typename T>
-static int launch_chain(const ChainParams& p, int grid, cudaStream_t stream) {
-  chain_stats_kernel<T><<<grid, kChainThreads, 0, stream>>>(p);
-  if (cudaGetLastError() != cudaSuccess) return -4;
+template <typename T, int CLUSTER>
+static int launch_token(const ChainParams& p, cudaStream_t stream) {
+  auto kern = chain_token_kernel<T, CLUSTER>;
+  if (CLUSTER > 8) {
+    static int allowed[kMaxDevicesCached] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return -3;
+    if (dev >= kMaxDevicesCached || !__atomic_load_n(&allowed[dev], __ATOMIC_ACQUIRE)) {
+      if (cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return -3;
+      if (dev < kMaxDevicesCached) __atomic_store_n(&allowed[dev], 1, __ATOMIC_RELEASE);
+    }
+  }
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(p.B * kChainCluster);
+  cfg.gridDim = dim3(p.B * CLUSTER);
   cfg.blockDim = dim3(kChainThreads);
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = kChainCluster;
+  attr[0].val.clusterDim.x = CLUSTER;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, chain_token_kernel<T>, p) == cudaSuccess ? 0 : -5;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kern, p) == cudaSuccess ? 0 : -5;
+}
+
+template <typename T>
+static int launch_chain(const ChainParams& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(kStatThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 0;                            // the first launch waits for everything before it
+  auto launch = [&](int lo, int hi, int z) {
+    cfg.gridDim = dim3(p.chunks, p.B, z);
+    const bool good = cudaLaunchKernelEx(&cfg, chain_stats_kernel<T>, p, lo, hi) == cudaSuccess;
+    cfg.numAttrs = 1;
+    return good;
+  };
+  const int all = 0x7fffffff;
+  const int mean = p.D / p.B + 1;
+  // Launches in turn cost about 3 us each, so they pay where reading all rows takes several times that.
+  if (static_cast<double>(p.V) * sizeof(T) * (2.0 * p.D + p.B) < 160e6) {
+    if (!launch(0, all, mean < 64 ? mean : 64)) return -4;
+  } else {
+    for (int lo = 0, hi = 1; lo < 9; lo = hi, hi = lo < 3 ? lo + 1 : lo < 5 ? 5 : lo < 9 ? 9 : all)
+      if (!launch(lo, hi, hi - lo)) return -4;
+    if (!launch(9, all, 4)) return -4;
+  }
+  // few sequences: more SMs each (16 is more than a portable cluster has)
+  return p.B * 16 <= 144 ? launch_token<T, 16>(p, stream) : launch_token<T, 8>(p, stream);
 }
 
 }  // namespace js
 
+// Float4s of scratch for `rows` rows of V values: a chunk each.
+static int chain_chunks(int V, int size) { return (V * size + 15 + js::kChunkBytes) / js::kChunkBytes; }
+extern "C" long long js_chain_verify_ws(int B, int D, int V, int is_bf16) {
+  return (2ll * D + B) * chain_chunks(V, is_bf16 ? 2 : 4) * 16 + (static_cast<long long>(D) + 2 * B) * 4;
+}
+
 // target (D + B, V), draft (D, V) fp32 or bf16 (is_bf16), rows ldt / ldd elements apart; drafts (D), cu (B + 1) int32; accept_u (D),
-// sample_u (B) fp32 in [0, 1); temp, draft_temp (B) fp32 or null (the scalars hold).  stats: (2 D + B) * chunks float4,
-// rejected: B ints, both scratch.  accepted (B) int32, token (B) int64.
+// sample_u (B) fp32 in [0, 1); temp, draft_temp (B) fp32 or null (the scalars hold).  ws: js_chain_verify_ws bytes.  accepted (B) int32, token
+// (B) int64.
 extern "C" int js_chain_verify(const void* target, long long ldt, const void* draft, long long ldd, int is_bf16, const int* drafts,
                                const int* cu, const float* accept_u, const float* sample_u, const float* temp, double temp_all,
-                               const float* draft_temp, double draft_temp_all, void* stats, int* rejected, int* accepted, long long* token,
-                               int* status, int B, int D, int V, int chunks, int grid, cudaStream_t stream) {
+                               const float* draft_temp, double draft_temp_all, void* ws, int* accepted, long long* token,
+                               int* status, int B, int D, int V, cudaStream_t stream) {
   using namespace js;
-  if (B < 0 || D < 0 || V < 1 || chunks < 1 || grid < 1) return -10;
+  if (B < 0 || B > 0xffff || D < 0 || V < 1 || V > (1 << 28)) return -10;
   if (B == 0) return 0;
+  const int chunks = chain_chunks(V, is_bf16 ? 2 : 4);
+  float4* stats = reinterpret_cast<float4*>(ws);
+  int* rejected = reinterpret_cast<int*>(stats + (2ll * D + B) * chunks);
   ChainParams p{target, draft, ldt, ldd, drafts, cu, accept_u, sample_u, temp, draft_temp, temp_all, draft_temp_all,
-                reinterpret_cast<float4*>(stats), rejected, accepted, token, status, B, D, V, chunks};
-  if (cudaMemsetAsync(rejected, 0x7f, sizeof(int) * B, stream) != cudaSuccess) return -3;
-  return is_bf16 ? launch_chain<__nv_bfloat16>(p, grid, stream) : launch_chain<float>(p, grid, stream);
+                stats, rejected, rejected + B, accepted, token, status, B, D, V, chunks};
+  if (cudaMemsetAsync(rejected, 0, sizeof(int) * (static_cast<size_t>(D) + 2 * B), stream) != cudaSuccess) return -3;
+  return is_bf16 ? launch_chain<__nv_bfloat16>(p, stream) : launch_chain<float>(p, stream);
 }

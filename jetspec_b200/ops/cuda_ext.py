@@ -1566,7 +1566,7 @@ def verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, samp
     B, D = cu_drafts.numel() - 1, drafts.numel()
     _need(target_logits.dim() == 2 and draft_logits.dim() == 2 and draft_logits.device == dev, "logits: expected matrices on one device")
     V = target_logits.shape[1]
-    _need(B >= 0 and V >= 1 and draft_logits.shape == (D, V) and target_logits.shape[0] == D + B,
+    _need(0 <= B <= 65535 and 1 <= V <= 2 ** 28 and draft_logits.shape == (D, V) and target_logits.shape[0] == D + B,
           f"{D} drafts of {B} sequences: target_logits {tuple(target_logits.shape)}, draft_logits {tuple(draft_logits.shape)}")
     if target_logits.dtype != draft_logits.dtype or target_logits.dtype not in (torch.float32, torch.bfloat16):
         target_logits, draft_logits = target_logits.float(), draft_logits.float()
@@ -1581,12 +1581,11 @@ def verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, samp
     draft_temp = temp if draft_temperature is None else _temperatures(draft_temperature, B, dev, "draft_temperature")
     accepted = torch.empty(B, dtype=torch.int32, device=dev)
     token = torch.empty(B, dtype=torch.int64, device=dev)
-    # few rows are cut into chunks so that two CTAs are on every SM
-    chunks = max(1, min(2 * SM_COUNT // max(1, D + B), V // 2048))
-    ws = torch.empty((2 * D + B) * chunks * 4 + B, dtype=torch.int32, device=dev)
     lib = load()
+    size = target_logits.element_size()
+    chunks = (V * size + 15 + 16384) // 16384
+    ws = torch.empty((2 * D + B) * chunks * 4 + D + 2 * B, dtype=torch.int32, device=dev)
     _check(lib.js_chain_verify(_p(target_logits), ctypes.c_longlong(target_logits.stride(0)), _p(draft_logits), ctypes.c_longlong(draft_logits.stride(0)),
                                int(target_logits.dtype == torch.bfloat16), _p(drafts), _p(cu_drafts), _p(accept_u), _p(sample_u), *temp,
-                               *draft_temp, _p(ws), _p(ws[ws.numel() - B:]), _p(accepted), _p(token), _p(status_word(dev)), B, D, V, chunks,
-                               2 * SM_COUNT, _stream()), "js_chain_verify")
+                               *draft_temp, _p(ws), _p(accepted), _p(token), _p(status_word(dev)), B, D, V, _stream()), "js_chain_verify")
     return accepted, token
