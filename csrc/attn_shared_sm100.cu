@@ -7,7 +7,7 @@
 // sequence's rows take both ranges in one go.
 //
 // Work is a line of units, a unit being 80 keys for a pair of row tiles: items (pair of tiles, KV head) one after the other, an
-// item's units in key order.  Every CTA takes an equal piece of the line, so lengths, which only the device knows, balance by
+// item's units in key order behind a few that stand for what it costs beside them.  Every CTA takes an equal piece of the line, so lengths, which only the device knows, balance by
 // themselves; where a piece begins or ends inside an item its parts go through a workspace and attn_shared_merge_kernel.
 //
 // A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warps 8 and 12 issue the MMAs of either product, warps 9 and 10 load K and V by
@@ -26,6 +26,7 @@ constexpr int SD = 128;              // head dim
 constexpr int SROWS = 128;           // rows of a tile
 constexpr int SKEYS = 80;            // keys of a unit: scores (80 columns) and probabilities (40) of a group fit 128 columns side by side
 constexpr int SSLOTS = 8;            // ring of K and V tiles, in turn
+constexpr int kItemCost = 4;         // what an item costs beside its units, in units: setting out, and results out of tensor memory
 constexpr int kQTile = SROWS * 256, kKTile = SKEYS * 256;      // bytes of a Q, K or V tile: 2 halves x rows x 128 B
 constexpr int SWARPS = 13, STHREADS = 32 * SWARPS;      // 152 registers a thread
 constexpr int kSharedSmem = 2 * kQTile + SSLOTS * kKTile + 512;
@@ -35,7 +36,7 @@ struct SharedAttn {
   const __nv_bfloat16* q;      // (T, Hq, 128), ldq elements between tokens
   const int *slot_map, *seq_rows, *cu_q, *past_lens, *mask_bits;
   __nv_bfloat16* out;          // (T, Hq * 128)
-  int* plan;                   // units in all; of every item its first unit
+  int* plan;                   // length of the line; where every item begins on it
   float *po, *so;              // partial outputs of prefix and sequence segments: (segment, side, row, 128)
   float2 *pml, *sml;           // their (maximum, sum): (segment, side, row)
   int* status;
@@ -85,12 +86,17 @@ JS_DEVICE int sa_units(const SharedAttn& p, const SaSeq& s, int b, int pair) {
   return max(0, sa_end(p, s, b, pair) - s.first + SKEYS - 1) / SKEYS;
 }
 JS_DEVICE int sa_pairs(const SharedAttn& p, const SaSeq& s) { return (s.n + 2 * p.npt - 1) / (2 * p.npt); }
-JS_DEVICE int sa_total(const SharedAttn& p, int b) {       // units of one head
+// An item's length on the line: its units behind what it costs beside them (nothing without units)
+JS_DEVICE int sa_length(const SharedAttn& p, const SaSeq& s, int b, int pair) {
+  const int n = sa_units(p, s, b, pair);
+  return n > 0 ? n + kItemCost : 0;
+}
+JS_DEVICE int sa_total(const SharedAttn& p, int b) {       // length of one head's items
   const SaSeq s = sa_seq(p, b);
   const int pairs = sa_pairs(p, s);
-  if (b < 0 || !p.causal) return pairs * sa_units(p, s, b, 0);
+  if (b < 0 || !p.causal) return pairs * sa_length(p, s, b, 0);
   int n = 0;
-  for (int i = 0; i < pairs; ++i) n += sa_units(p, s, b, i);
+  for (int i = 0; i < pairs; ++i) n += sa_length(p, s, b, i);
   return n;
 }
 // Item numbers grow along the line (with gaps): a sequence starts behind the pairs of all rows before it.
@@ -108,40 +114,48 @@ JS_DEVICE int sa_start(const SharedAttn& p, int cta, int total) {
 
 // A CTA's piece of the line, item by item; every role walks it for itself.
 struct SaWalk {
-  int b, pair, h, t, left;     // next unit, units left
+  int b, pair, h, t, left;     // place in an item, what is left of the piece
+  int at;                      // place on the line
   int parity;                  // group of the next job
   SaSeq s;
-  int units, nt;               // of the item; of them in this segment, from t
+  int units, first, nt, span;  // of the item; this segment's units from the first one; its part of the line
   int group0;                  // the group of the segment's first job
   bool two;                    // both tiles of the pair have rows
 };
 JS_DEVICE void sa_begin(const SharedAttn& p, SaWalk& w) { if (w.left > 0) w.s = sa_seq(p, w.b); }
-// the next segment; t has been moved behind it when the call after this one is made
-JS_DEVICE bool sa_next(const SharedAttn& p, SaWalk& w) {
-  if (w.left <= 0) return false;
-  for (;;) {
-    w.units = sa_units(p, w.s, w.b, w.pair);
-    if (w.pair < sa_pairs(p, w.s) && w.t < w.units) break;
-    w.t = 0;
-    if (w.units == 0 || ++w.h == p.Hkv) {
-      w.h = 0;
-      ++w.pair;
-    }
-    while (w.pair >= sa_pairs(p, w.s)) {
-      w.pair = 0;
-      if (++w.b >= p.B) return false;
-      w.s = sa_seq(p, w.b);
-    }
-  }
-  w.nt = min(w.left, w.units - w.t);
-  w.two = w.s.n - w.pair * 2 * p.npt > p.npt;
-  w.group0 = w.parity;
-  return true;
-}
 JS_DEVICE void sa_done(SaWalk& w) {
-  w.left -= w.nt;
-  w.t += w.nt;
+  w.left -= w.span;
+  w.t += w.span;
+  w.at += w.span;
   if (!w.two) w.parity ^= w.nt & 1;
+}
+// the next segment; sa_done has been called for the one before
+JS_DEVICE bool sa_next(const SharedAttn& p, SaWalk& w) {
+  while (w.left > 0) {
+    for (;;) {
+      const int length = w.pair < sa_pairs(p, w.s) ? sa_length(p, w.s, w.b, w.pair) : 0;
+      if (w.t < length) break;
+      w.t = 0;
+      if (length == 0 || ++w.h == p.Hkv) {
+        w.h = 0;
+        ++w.pair;
+      }
+      while (w.pair >= sa_pairs(p, w.s)) {
+        w.pair = 0;
+        if (++w.b >= p.B) return false;
+        w.s = sa_seq(p, w.b);
+      }
+    }
+    w.units = sa_units(p, w.s, w.b, w.pair);
+    w.span = min(w.left, w.units + kItemCost - w.t);
+    w.first = max(0, w.t - kItemCost);
+    w.nt = max(0, w.t + w.span - kItemCost) - w.first;
+    w.two = w.s.n - w.pair * 2 * p.npt > p.npt;
+    w.group0 = w.parity;
+    if (w.nt > 0) return true;
+    sa_done(w);
+  }
+  return false;
 }
 
 JS_DEVICE void sa_mma_tmem_a(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
@@ -308,11 +322,11 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   if (u0 < prefix_units) {
     if (tid == 0) {
       const SaSeq s = sa_seq(p, -1);
-      const int units = sa_units(p, s, -1, 0);
+      const int length = sa_length(p, s, -1, 0);
       start[0] = -1;
-      start[1] = u0 / units / p.Hkv;
-      start[2] = u0 / units % p.Hkv;
-      start[3] = u0 % units;
+      start[1] = u0 / length / p.Hkv;
+      start[2] = u0 / length % p.Hkv;
+      start[3] = u0 % length;
     }
   } else if (u0 < u1) {
     int run = prefix_units;
@@ -328,12 +342,12 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       if (u0 >= before && u0 < before + v) {
         const SaSeq s = sa_seq(p, b);
         int pair = 0, at = u0 - before;
-        while (at >= sa_units(p, s, b, pair) * p.Hkv) at -= sa_units(p, s, b, pair++) * p.Hkv;
-        const int units = sa_units(p, s, b, pair);
+        while (at >= sa_length(p, s, b, pair) * p.Hkv) at -= sa_length(p, s, b, pair++) * p.Hkv;
+        const int length = sa_length(p, s, b, pair);
         start[0] = b;
         start[1] = pair;
-        start[2] = at / units;
-        start[3] = at % units;
+        start[2] = at / length;
+        start[3] = at % length;
       }
     }
   }
@@ -348,6 +362,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   const uint32_t tmem = *tmem_slot;
   SaWalk w;
   w.left = u1 - u0;
+  w.at = u0;
   if (w.left > 0) {
     w.b = start[0];
     w.pair = start[1];
@@ -360,11 +375,9 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   if (warp == 11) {
     // ================================================================ Q loader; it notes where items begin
     int uses = 0;                               // Q buffers filled so far: buffer uses % 2
-    int unit = u0;
     bool ok = true;
     while (ok && sa_next(p, w)) {
-      if (lane == 0 && w.t == 0) p.plan[1 + sa_item(p, w.s, w.b, w.pair, w.h)] = unit;
-      unit += w.nt;
+      if (lane == 0 && w.first == 0) p.plan[1 + sa_item(p, w.s, w.b, w.pair, w.h)] = w.at - w.t;
       for (int side = 0; side < (w.two ? 2 : 1) && ok; ++side, ++uses) {
         const int buf = uses & 1;
         ok = sa_wait(&q_empty[buf], ((uses >> 1) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
@@ -394,23 +407,33 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const int* slots = p.slot_map + static_cast<size_t>(known ? w.s.row : 0) * p.max_len;
       const int end = sa_end(p, w.s, w.b, w.pair), row0 = w.h * p.S;
       auto slot_at = [&](int i, int part) {     // keys past the end repeat the last one (no row sees them)
-        return __ldg(slots + min(w.s.first + (w.t + i) * SKEYS + 32 * part + lane, end - 1));
+        return __ldg(slots + min(w.s.first + (w.first + i) * SKEYS + 32 * part + lane, end - 1));
       };
       int next[3] = {slot_at(0, 0), slot_at(0, 1), slot_at(0, 2)};
       for (int i = 0; i < w.nt; ++i, n += 2) {
         int slot[3], page[6];
-        uint32_t in_row = 0xffffffffu;
+        unsigned paged = 0;                     // groups of 16 keys that lie in one page
 #pragma unroll
         for (int part = 0; part < 3; ++part) {
           slot[part] = next[part];
           if (i + 1 < w.nt) next[part] = slot_at(i + 1, part);
           if (slot[part] < 0 || slot[part] >= p.S) { report(p.status, kBadSlot); slot[part] = 0; }
           const int first = __shfl_sync(0xffffffffu, slot[part], lane & 16);
-          uint32_t seen = __ballot_sync(0xffffffffu, slot[part] == first + (lane & 15));
-          if (part == 2) seen |= 0xffff0000u;   // the tile ends after 16 of these
-          in_row &= seen;
+          const uint32_t in_row = __ballot_sync(0xffffffffu, slot[part] == first + (lane & 15));
+          if ((in_row & 0xffffu) == 0xffffu) paged |= 1u << (2 * part);
+          if ((in_row >> 16) == 0xffffu) paged |= 2u << (2 * part);
           page[2 * part] = row0 + __shfl_sync(0xffffffffu, slot[part], 0);
           page[2 * part + 1] = row0 + __shfl_sync(0xffffffffu, slot[part], 16);
+        }
+        // groups behind the last key repeat a page of the tile, where it has one: nobody sees them, but they have to be numbers
+        const int keys = end - (w.s.first + (w.first + i) * SKEYS);
+#pragma unroll
+        for (int part = 0; part < 5; ++part) {
+          if (16 * part < keys || (paged & 0x1fu) == 0) continue;
+          const int any = __ffs(paged & 0x1fu) - 1;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) if (e == any) page[part] = page[e];
+          paged |= 1u << part;
         }
         const int s = n % SSLOTS;
         ok = sa_wait(&kv_empty[s], ((n / SSLOTS) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
@@ -418,26 +441,29 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         const uint32_t dst = smem_u32(sKV + s * kKTile);
         if (elect_one()) {
           mbar_expect_tx(&kv_full[s], kKTile);
-          if (in_row == 0xffffffffu) {          // all of it in pages
 #pragma unroll
-            for (int part = 0; part < 5; ++part) {
-              sa_tma_box(dst + part * 2048, box, &kv_full[s], 0, page[part]);
-              sa_tma_box(dst + part * 2048 + SKEYS * 128, box, &kv_full[s], 64, page[part]);
-            }
+          for (int part = 0; part < 5; ++part) {
+            if (!((paged >> part) & 1u)) continue;
+            sa_tma_box(dst + part * 2048, box, &kv_full[s], 0, page[part]);
+            sa_tma_box(dst + part * 2048 + SKEYS * 128, box, &kv_full[s], 64, page[part]);
           }
         }
         __syncwarp();
-        if (in_row == 0xffffffffu) continue;
+        if ((paged & 0x1fu) == 0x1fu) continue;
 #pragma unroll
-        for (int g = 0; g < SKEYS / 4; ++g) {
-          int y[4];
+        for (int part = 0; part < 5; ++part) {
+          if ((paged >> part) & 1u) continue;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = row0 + __shfl_sync(0xffffffffu, slot[g / 8], 4 * (g & 7) + e);
-          if (elect_one()) {
-            sa_tma_rows(dst + g * 512, one, &kv_full[s], 0, y[0], y[1], y[2], y[3]);
-            sa_tma_rows(dst + g * 512 + SKEYS * 128, one, &kv_full[s], 64, y[0], y[1], y[2], y[3]);
+          for (int g = 4 * part; g < 4 * part + 4; ++g) {
+            int y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = row0 + __shfl_sync(0xffffffffu, slot[g / 8], 4 * (g & 7) + e);
+            if (elect_one()) {
+              sa_tma_rows(dst + g * 512, one, &kv_full[s], 0, y[0], y[1], y[2], y[3]);
+              sa_tma_rows(dst + g * 512 + SKEYS * 128, one, &kv_full[s], 64, y[0], y[1], y[2], y[3]);
+            }
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
       sa_done(w);
@@ -516,7 +542,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       int jobs = 0;
       const bool busy = __any_sync(0xffffffffu, valid);      // a warp without rows only keeps the barriers going
       for (int i = w.two ? 0 : rel; i < w.nt && ok; i += w.two ? 1 : 2, ++jobs, ++jobs_done) {
-        const int k0 = w.s.first + (w.t + i) * SKEYS;
+        const int k0 = w.s.first + (w.first + i) * SKEYS;
         const bool all = k0 + SKEYS <= min(w.s.past, end);      // every row of the item sees the whole block
         ok = sa_wait(&s_full[g], jobs_done & 1, p.status, kTimeoutAccum, gave_up);
         if (!ok) break;
@@ -644,8 +670,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
 // Joins the parts of the rows of a tile: a block takes up to kMergeRows rows of one head, a warp a row at a time, four columns a lane.
 constexpr int kMergeRows = 32, kMergeWarps = 8;
 __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(const SharedAttn p) {
-  pdl_launch_dependents();
-  pdl_wait();
+  // Until the wait below only the call's inputs are read: the kernel before, which is launched without overlap, began when they were there.
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, h = blockIdx.y, row0 = blockIdx.z * kMergeRows;
   {                                            // rows behind the last sequence are zero
     const int first = max(0, min(p.cu_q[p.B], p.T));
@@ -666,14 +691,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
   const int tile = blockIdx.x - (s.q_begin / p.npt + b), node0 = tile * p.npt;
   const int rows = min(p.npt, s.n - node0) * p.G;
   if (rows <= row0) return;
+  pdl_wait();
   const int total = p.plan[0], pair = tile >> 1, units = sa_units(p, s, b, pair);
   const bool two = s.n - pair * 2 * p.npt > p.npt;
   int c0 = 0, own = 0, item = 0;               // first CTA and number of CTAs with a part of the sequence's own keys
   if (units > 0) {
     item = sa_item(p, s, b, pair, h);
     const int u = p.plan[1 + item];
-    c0 = sa_cta(p, u, total);
-    own = sa_cta(p, u + units - 1, total) - c0 + 1;
+    c0 = sa_cta(p, u + kItemCost, total);
+    own = sa_cta(p, u + kItemCost + units - 1, total) - c0 + 1;
     item -= p.prefix_items;
   }
   if (own == 1 && two && p.prefix == 0) return;       // written by its CTA
@@ -687,7 +713,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
     if (all_units > 0) {
       const int p_tile = t / p.npt, p_pair = p_tile >> 1;
       p_item = sa_item(p, all, -1, p_pair, h);
-      const int u = (p_pair * p.Hkv + h) * all_units;
+      const int u = (p_pair * p.Hkv + h) * (all_units + kItemCost) + kItemCost;
       pc0 = sa_cta(p, u, total);
       p_two = all.n - p_pair * 2 * p.npt > p.npt;
       shared_parts = (sa_cta(p, u + all_units - 1, total) - pc0 + 1) * (p_two ? 1 : 2);

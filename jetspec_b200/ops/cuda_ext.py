@@ -1457,135 +1457,187 @@ def moe_forward(x, gate_w, w_gate_up, w_down, top_k: int, renorm: bool, router_l
 
 
 # ------------------------------------------------------------------ a batched serving step
+# Calls of a few microseconds on the device: arguments are checked with plain comparisons, messages are made only when one fails, and
+# the entry points are bound with their argument types once (pointers are passed as integers).
+_bound: dict = {}
+_ARG = {"p": ctypes.c_void_p, "i": ctypes.c_int, "l": ctypes.c_longlong, "f": ctypes.c_float, "d": ctypes.c_double}
+
+
+def _entry(name: str, args: str, restype=ctypes.c_int):
+    """Entry point ``name`` of the library, a letter of :data:`_ARG` for every argument."""
+    fn = _bound.get(name)
+    if fn is None:
+        fn = ctypes.CDLL(load()._name)[name]          # a function object of its own: the argument types hold for these calls alone
+        fn.argtypes, fn.restype = [_ARG[c] for c in args], restype
+        _bound[name] = fn
+    return fn
+
+
+_status_ptr: dict = {}
+
+
+def _status_at(index: int) -> int:
+    """Address of a CUDA device's status word (the word is kept by :func:`status_word`)."""
+    at = _status_ptr.get(index)
+    if at is None:
+        at = _status_ptr[index] = status_word(torch.device("cuda", index)).data_ptr()
+    return at
+
+
+def _current_device() -> int:
+    return _cur_device() if _cur_device is not None else torch.cuda.current_device()
+
+
+def _stream_at(index: int) -> int:
+    return _raw_stream(index) if _raw_stream is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def _refuse(what: str):
+    raise ValueError(what)
+
+
+def _ints(index: int, **tensors) -> None:
+    """Index tensors of a serving op: contiguous int32 on CUDA device ``index`` (-1: the host, where only the checks run)."""
+    for name, t in tensors.items():
+        if t.dtype is not torch.int32 or t.get_device() != index or not t.is_contiguous():
+            _refuse(f"{name}: expected a contiguous int32 tensor on device {index}, got {t.dtype} on {t.device}")
+
+
 def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale: float, prefix_len: int,
                             causal: bool, max_q: int, out: Optional[torch.Tensor] = None, ws: Optional[torch.Tensor] = None):
     """See :func:`jetspec_b200.ops.reference.shared_prefix_attention` for the contract.  bf16, heads of 128; ``max_q`` bounds a sequence's
     rows; ``q`` may be a view whose tokens lie further apart.  ``ws`` (uint8, :func:`shared_prefix_workspace` bytes) and ``out`` keep a
     captured launch's buffers outside; a workspace serves one launch at a time."""
-    dev = q.device
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
+    index = q.get_device()
+    if index >= 0 and index != _current_device():
+        with torch.cuda.device(index):
             return shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale, prefix_len, causal, max_q,
                                            out, ws)
-    _need(q.dim() == 3 and q.dtype == torch.bfloat16 and q.shape[2] == 128, f"q {tuple(q.shape)} {q.dtype}: expected (T, Hq, 128) in bf16")
+    bf16 = torch.bfloat16
+    if q.dim() != 3 or q.dtype is not bf16 or q.shape[2] != 128:
+        _refuse(f"q {tuple(q.shape)} {q.dtype}: expected (T, Hq, 128) in bf16")
     T, Hq, _ = q.shape
-    _need(k_pool.dim() == 3 and k_pool.shape == v_pool.shape and k_pool.shape[2] == 128 and k_pool.dtype == v_pool.dtype == torch.bfloat16
-          and k_pool.is_contiguous() and v_pool.is_contiguous() and k_pool.device == v_pool.device == dev,
-          "pools: expected contiguous bf16 (Hkv, S, 128) tensors on the queries' device")
+    if (k_pool.dim() != 3 or k_pool.shape != v_pool.shape or k_pool.shape[2] != 128 or k_pool.dtype is not bf16 or v_pool.dtype is not bf16
+            or not k_pool.is_contiguous() or not v_pool.is_contiguous() or k_pool.get_device() != index or v_pool.get_device() != index):
+        _refuse("pools: expected contiguous bf16 (Hkv, S, 128) tensors on the queries' device")
     Hkv, S, _ = k_pool.shape
-    _need(Hkv >= 1 and S >= 1 and Hq >= 1 and Hq % Hkv == 0 and Hq // Hkv <= 128 and Hkv * S < 2 ** 31, f"{Hq} query and {Hkv} KV heads over {S} slots")
-    causal = bool(causal)
-    _ints(dev, slot_map=slot_map, seq_rows=seq_rows, cu_q=cu_q, past_lens=past_lens, **({} if causal or mask_bits is None else {"mask_bits": mask_bits}))
+    if Hkv < 1 or S < 1 or Hq < 1 or Hq % Hkv or Hq // Hkv > 128 or Hkv * S >= 2 ** 31:
+        _refuse(f"{Hq} query and {Hkv} KV heads over {S} slots")
+    _ints(index, slot_map=slot_map, seq_rows=seq_rows, cu_q=cu_q, past_lens=past_lens)
     B, (max_seqs, max_len) = seq_rows.numel(), slot_map.shape
-    _need(cu_q.numel() == B + 1 and past_lens.numel() == B and max_seqs >= 1, f"{B} sequences: cu_q {cu_q.numel()}, past_lens {past_lens.numel()}")
-    _need(causal or (mask_bits is not None and mask_bits.dim() == 2 and mask_bits.shape[0] == T and mask_bits.shape[1] >= 1),
-          "mask_bits: a row of words for every query is needed without the causal rule")
-    _need(0 <= prefix_len <= max_len and max_q >= 1 and scale > 0.0, f"prefix_len={prefix_len}, max_q={max_q}, scale={scale}")
-    if q.stride(2) != 1 or q.stride(1) != 128 or q.stride(0) % 8 or q.data_ptr() % 16:
+    if cu_q.numel() != B + 1 or past_lens.numel() != B or max_seqs < 1:
+        _refuse(f"{B} sequences: cu_q {cu_q.numel()}, past_lens {past_lens.numel()}")
+    words, bits = 0, 0
+    if not causal:
+        if mask_bits is None or mask_bits.dim() != 2 or mask_bits.shape[0] != T or mask_bits.shape[1] < 1:
+            _refuse("mask_bits: without the causal rule every query needs a row of words")
+        _ints(index, mask_bits=mask_bits)
+        words, bits = mask_bits.shape[1], mask_bits.data_ptr()
+    if not (0 <= prefix_len <= max_len and max_q >= 1 and 0.0 < scale < math.inf):
+        _refuse(f"prefix_len={prefix_len} of {max_len}, max_q={max_q}, scale={scale}")
+    if q.stride(2) != 1 or q.stride(1) != 128 or q.stride(0) % 8 or q.stride(0) < Hq * 128 or q.data_ptr() % 16:
         q = q.contiguous()
     if out is None:
-        out = torch.empty(T, Hq * 128, dtype=q.dtype, device=dev)
-    _need(out.shape == (T, Hq * 128) and out.dtype == q.dtype and out.is_contiguous() and out.device == dev and out.data_ptr() % 16 == 0,
-          "out: expected a contiguous (T, Hq * 128) bf16 tensor")
+        out = torch.empty(T, Hq * 128, dtype=bf16, device=q.device)
+    elif out.shape != (T, Hq * 128) or out.dtype is not bf16 or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 16:
+        _refuse("out: expected a contiguous (T, Hq * 128) bf16 tensor on the queries' device")
     if T == 0 or B == 0:
         return out.zero_()
     need = shared_prefix_workspace(B, T, Hq, Hkv, max_len, prefix_len, max_q)
     if ws is None:
-        ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    _need(ws.dtype == torch.uint8 and ws.is_contiguous() and ws.device == dev and ws.numel() >= need and ws.data_ptr() % 16 == 0,
-          f"ws: expected {need} bytes on {dev}")
-    _check(load().js_shared_attention(
-        _p(q), ctypes.c_longlong(q.stride(0)), _p(k_pool), _p(v_pool), _p(slot_map), _p(seq_rows), _p(cu_q), _p(past_lens), _p(mask_bits), _p(out),
-        _p(ws), ctypes.c_longlong(ws.numel()), _p(status_word(dev)), B, T, Hq, Hkv, S, max_seqs, max_len,
-        0 if causal else mask_bits.shape[1], int(causal), ctypes.c_float(scale), prefix_len, max_q, SM_COUNT, _stream()), "js_shared_attention")
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif ws.dtype is not torch.uint8 or not ws.is_contiguous() or ws.get_device() != index or ws.numel() < need or ws.data_ptr() % 16:
+        _refuse(f"ws: expected {need} contiguous bytes on the queries' device")
+    rc = _entry("js_shared_attention", "plppppppppplpiiiiiiiiifiiip")(
+        q.data_ptr(), q.stride(0), k_pool.data_ptr(), v_pool.data_ptr(), slot_map.data_ptr(), seq_rows.data_ptr(), cu_q.data_ptr(),
+        past_lens.data_ptr(), bits, out.data_ptr(), ws.data_ptr(), ws.numel(), _status_at(index), B, T, Hq, Hkv, S, max_seqs, max_len, words,
+        1 if causal else 0, scale, prefix_len, max_q, SM_COUNT, _stream_at(index))
+    if rc:
+        _check(rc, "js_shared_attention")
     return out
 
 
 def shared_prefix_workspace(B: int, T: int, Hq: int, Hkv: int, max_len: int, prefix_len: int, max_q: int) -> int:
     """Bytes of workspace that :func:`shared_prefix_attention` wants for these sizes."""
-    fn = load().js_shared_attention_ws
-    fn.restype = ctypes.c_longlong
-    n = fn(B, T, Hq, Hkv, max_len, prefix_len, max_q, SM_COUNT)
-    _check(min(n, 0), "js_shared_attention_ws")
+    n = _entry("js_shared_attention_ws", "iiiiiiii", ctypes.c_longlong)(B, T, Hq, Hkv, max_len, prefix_len, max_q, SM_COUNT)
+    if n < 0:
+        _check(n, "js_shared_attention_ws")
     return n
-
-
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise ValueError(what)
-
-
-def _ints(device, **tensors) -> None:
-    """Index tensors of a serving op: contiguous int32 on its device."""
-    for name, t in tensors.items():
-        _need(t.dtype == torch.int32 and t.device == device and t.is_contiguous(), f"{name}: expected a contiguous int32 tensor on {device}")
-
-
-def _elsewhere(device) -> bool:
-    """Whether ``device`` is not the current one (kernels launch on the current device's stream)."""
-    return device.index is not None and device.index != (_cur_device() if _cur_device is not None else torch.cuda.current_device())
 
 
 def plan_slots(past_lens, counts, seq_rows, free_pages, page_size: int, slot_map, rows: int, mapped_lens=None):
     """See :func:`jetspec_b200.ops.reference.plan_slots` for the contract."""
-    dev = slot_map.device
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
+    index = slot_map.get_device()
+    if index >= 0 and index != _current_device():
+        with torch.cuda.device(index):
             return plan_slots(past_lens, counts, seq_rows, free_pages, page_size, slot_map, rows, mapped_lens)
     mapped = past_lens if mapped_lens is None else mapped_lens
-    _ints(dev, past_lens=past_lens, counts=counts, seq_rows=seq_rows, free_pages=free_pages, slot_map=slot_map, mapped_lens=mapped)
+    _ints(index, past_lens=past_lens, counts=counts, seq_rows=seq_rows, free_pages=free_pages, slot_map=slot_map, mapped_lens=mapped)
     B, (max_seqs, max_len) = past_lens.numel(), slot_map.shape
-    _need(counts.numel() == seq_rows.numel() == mapped.numel() == B, "past_lens, counts, seq_rows and mapped_lens differ in length")
-    _need(B <= 65535 and page_size >= 1 and rows >= 0, f"plan_slots(B={B}, page_size={page_size}, rows={rows})")
+    if counts.numel() != B or seq_rows.numel() != B or mapped.numel() != B:
+        _refuse("past_lens, counts, seq_rows and mapped_lens differ in length")
+    if B > 65535 or page_size < 1 or rows < 0:
+        _refuse(f"plan_slots(B={B}, page_size={page_size}, rows={rows})")
+    buf = slot_map.new_empty(2 * (B + 1) + 2 * rows)
+    at = buf.data_ptr()
+    cu_q, cu_pages, positions, slots = buf.split_with_sizes((B + 1, B + 1, rows, rows))
     # blocks a request: enough to fill the SMs, a couple of thousand positions each
     chunks = max(1, min(4 * SM_COUNT // max(1, B), max_len // 2048))
-    cu_q, cu_pages, positions, slots = torch.empty(2 * (B + 1) + 2 * rows, dtype=torch.int32, device=dev).split((B + 1, B + 1, rows, rows))
-    lib = load()
-    _check(lib.js_slot_plan(_p(past_lens), _p(counts), _p(mapped), _p(seq_rows), _p(free_pages), _p(slot_map), _p(cu_q), _p(cu_pages),
-                            _p(positions), _p(slots), _p(status_word(dev)), B, free_pages.numel(), page_size, max_seqs, max_len, rows,
-                            chunks, _stream()), "js_slot_plan")
+    rc = _entry("js_slot_plan", "pppppppppppiiiiiiip")(
+        past_lens.data_ptr(), counts.data_ptr(), mapped.data_ptr(), seq_rows.data_ptr(), free_pages.data_ptr(), slot_map.data_ptr(),
+        at, at + 4 * (B + 1), at + 8 * (B + 1), at + 8 * (B + 1) + 4 * rows, _status_at(index), B, free_pages.numel(), page_size,
+        max_seqs, max_len, rows, chunks, _stream_at(index))
+    if rc:
+        _check(rc, "js_slot_plan")
     return cu_q, positions, slots, cu_pages
 
 
-def _temperatures(t, B: int, device, name: str) -> tuple:
-    """Pointer to a temperature per sequence, or null and the one that holds for all."""
+def _temperatures(t, B: int, index: int, name: str) -> tuple:
+    """Address of a temperature per sequence, or 0 and the one that holds for all."""
     if torch.is_tensor(t):
-        _need(t.dtype == torch.float32 and t.device == device and t.is_contiguous() and t.numel() == B, f"{name}: expected a number or {B} fp32 values on {device}")
-        return _p(t), ctypes.c_double(0.0)
-    _need(t >= 0.0, f"{name}={t}")
-    return None, ctypes.c_double(t)
+        if t.dtype is not torch.float32 or t.get_device() != index or not t.is_contiguous() or t.numel() != B:
+            _refuse(f"{name}: expected a number or {B} fp32 values on device {index}")
+        return t.data_ptr(), 0.0
+    if not 0.0 <= t < math.inf:
+        _refuse(f"{name}={t}")
+    return 0, t
 
 
 def verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, sample_u, temperature=1.0, draft_temperature=None):
     """See :func:`jetspec_b200.ops.reference.verify_chains` for the contract.  Logits in fp32 or bf16 (other types are converted), any row
     stride."""
-    dev = target_logits.device
-    if _elsewhere(dev):
-        with torch.cuda.device(dev):
+    index = target_logits.get_device()
+    if index >= 0 and index != _current_device():
+        with torch.cuda.device(index):
             return verify_chains(target_logits, draft_logits, drafts, cu_drafts, accept_u, sample_u, temperature, draft_temperature)
     B, D = cu_drafts.numel() - 1, drafts.numel()
-    _need(target_logits.dim() == 2 and draft_logits.dim() == 2 and draft_logits.device == dev, "logits: expected matrices on one device")
+    if target_logits.dim() != 2 or draft_logits.dim() != 2 or draft_logits.get_device() != index:
+        _refuse("logits: expected matrices on one device")
     V = target_logits.shape[1]
-    _need(0 <= B <= 65535 and 1 <= V <= 2 ** 28 and draft_logits.shape == (D, V) and target_logits.shape[0] == D + B,
-          f"{D} drafts of {B} sequences: target_logits {tuple(target_logits.shape)}, draft_logits {tuple(draft_logits.shape)}")
-    if target_logits.dtype != draft_logits.dtype or target_logits.dtype not in (torch.float32, torch.bfloat16):
-        target_logits, draft_logits = target_logits.float(), draft_logits.float()
+    if not 0 <= B <= 65535 or not 1 <= V <= 2 ** 28 or draft_logits.shape != (D, V) or target_logits.shape[0] != D + B:
+        _refuse(f"{D} drafts of {B} sequences: target_logits {tuple(target_logits.shape)}, draft_logits {tuple(draft_logits.shape)}")
+    f32, dtype = torch.float32, target_logits.dtype
+    if dtype is not draft_logits.dtype or (dtype is not f32 and dtype is not torch.bfloat16):
+        target_logits, draft_logits, dtype = target_logits.float(), draft_logits.float(), f32
     if target_logits.stride(1) != 1:
         target_logits = target_logits.contiguous()
     if draft_logits.stride(1) != 1:
         draft_logits = draft_logits.contiguous()
-    _ints(dev, drafts=drafts, cu_drafts=cu_drafts)
+    _ints(index, drafts=drafts, cu_drafts=cu_drafts)
     for name, u, n in (("accept_u", accept_u, D), ("sample_u", sample_u, B)):
-        _need(u.dtype == torch.float32 and u.device == dev and u.is_contiguous() and u.numel() == n, f"{name}: expected {n} fp32 values on {dev}")
-    temp = _temperatures(temperature, B, dev, "temperature")
-    draft_temp = temp if draft_temperature is None else _temperatures(draft_temperature, B, dev, "draft_temperature")
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    token = torch.empty(B, dtype=torch.int64, device=dev)
-    lib = load()
-    size = target_logits.element_size()
-    chunks = (V * size + 15 + 16384) // 16384
-    ws = torch.empty((2 * D + B) * chunks * 4 + D + 2 * B, dtype=torch.int32, device=dev)
-    _check(lib.js_chain_verify(_p(target_logits), ctypes.c_longlong(target_logits.stride(0)), _p(draft_logits), ctypes.c_longlong(draft_logits.stride(0)),
-                               int(target_logits.dtype == torch.bfloat16), _p(drafts), _p(cu_drafts), _p(accept_u), _p(sample_u), *temp,
-                               *draft_temp, _p(ws), _p(accepted), _p(token), _p(status_word(dev)), B, D, V, _stream()), "js_chain_verify")
+        if u.dtype is not f32 or u.get_device() != index or not u.is_contiguous() or u.numel() != n:
+            _refuse(f"{name}: expected {n} contiguous fp32 values on device {index}")
+    temp = _temperatures(temperature, B, index, "temperature")
+    draft_temp = temp if draft_temperature is None else _temperatures(draft_temperature, B, index, "draft_temperature")
+    device = target_logits.device
+    accepted = torch.empty(B, dtype=torch.int32, device=device)
+    token = torch.empty(B, dtype=torch.int64, device=device)
+    bf16 = 0 if dtype is f32 else 1
+    ws = torch.empty(_entry("js_chain_verify_ws", "iiii", ctypes.c_longlong)(B, D, V, bf16), dtype=torch.uint8, device=device)
+    rc = _entry("js_chain_verify", "plplipppppdpdppppiiip")(
+        target_logits.data_ptr(), target_logits.stride(0), draft_logits.data_ptr(), draft_logits.stride(0), bf16, drafts.data_ptr(),
+        cu_drafts.data_ptr(), accept_u.data_ptr(), sample_u.data_ptr(), temp[0], temp[1], draft_temp[0], draft_temp[1], ws.data_ptr(),
+        accepted.data_ptr(), token.data_ptr(), _status_at(index), B, D, V, _stream_at(index))
+    if rc:
+        _check(rc, "js_chain_verify")
     return accepted, token
