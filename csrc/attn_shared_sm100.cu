@@ -26,7 +26,7 @@ constexpr int SD = 128;              // head dim
 constexpr int SROWS = 128;           // rows of a tile
 constexpr int SKEYS = 80;            // keys of a unit: scores (80 columns) and probabilities (40) of a group fit 128 columns side by side
 constexpr int SSLOTS = 8;            // ring of K and V tiles, in turn
-constexpr int kItemCost = 4;         // what an item costs beside its units, in units: setting out, and results out of tensor memory
+constexpr int kItemCost = 8;         // what an item costs beside its jobs, in jobs: setting out, and results out of tensor memory
 constexpr int kQTile = SROWS * 256, kKTile = SKEYS * 256;      // bytes of a Q, K or V tile: 2 halves x rows x 128 B
 constexpr int SWARPS = 13, STHREADS = 32 * SWARPS;      // 152 registers a thread
 constexpr int kSharedSmem = 2 * kQTile + SSLOTS * kKTile + 512;
@@ -36,7 +36,8 @@ struct SharedAttn {
   const __nv_bfloat16* q;      // (T, Hq, 128), ldq elements between tokens
   const int *slot_map, *seq_rows, *cu_q, *past_lens, *mask_bits;
   __nv_bfloat16* out;          // (T, Hq * 128)
-  int* plan;                   // length of the line; where every item begins on it
+  int* plan;                   // length of a piece of the line; where every item begins on it
+  uint8_t* parted;             // (tile of the sequences' rows, head): its output is in parts (without a prefix)
   float *po, *so;              // partial outputs of prefix and sequence segments: (segment, side, row, 128)
   float2 *pml, *sml;           // their (maximum, sum): (segment, side, row)
   int* status;
@@ -86,15 +87,17 @@ JS_DEVICE int sa_units(const SharedAttn& p, const SaSeq& s, int b, int pair) {
   return max(0, sa_end(p, s, b, pair) - s.first + SKEYS - 1) / SKEYS;
 }
 JS_DEVICE int sa_pairs(const SharedAttn& p, const SaSeq& s) { return (s.n + 2 * p.npt - 1) / (2 * p.npt); }
-// An item's length on the line: its units behind what it costs beside them (nothing without units)
+// An item's length on the line: its jobs (two a unit where both tiles have rows) behind what it costs beside them (nothing without units)
+JS_DEVICE int sa_weight(const SharedAttn& p, const SaSeq& s, int pair) { return s.n - pair * 2 * p.npt > p.npt ? 2 : 1; }
 JS_DEVICE int sa_length(const SharedAttn& p, const SaSeq& s, int b, int pair) {
   const int n = sa_units(p, s, b, pair);
-  return n > 0 ? n + kItemCost : 0;
+  return n > 0 ? n * sa_weight(p, s, pair) + kItemCost : 0;
 }
 JS_DEVICE int sa_total(const SharedAttn& p, int b) {       // length of one head's items
   const SaSeq s = sa_seq(p, b);
   const int pairs = sa_pairs(p, s);
-  if (b < 0 || !p.causal) return pairs * sa_length(p, s, b, 0);
+  if (pairs == 0) return 0;
+  if (b < 0 || !p.causal) return (pairs - 1) * sa_length(p, s, b, 0) + sa_length(p, s, b, pairs - 1);
   int n = 0;
   for (int i = 0; i < pairs; ++i) n += sa_length(p, s, b, i);
   return n;
@@ -103,14 +106,11 @@ JS_DEVICE int sa_total(const SharedAttn& p, int b) {       // length of one head
 JS_DEVICE int sa_item(const SharedAttn& p, const SaSeq& s, int b, int pair, int h) {
   return (b < 0 ? pair : p.prefix_items / p.Hkv + s.q_begin / (2 * p.npt) + b + pair) * p.Hkv + h;
 }
-// The line is cut into as many pieces as there are CTAs, none of them empty: with fewer units than CTAs the last CTAs have none.
-JS_DEVICE int sa_cta(const SharedAttn& p, int unit, int total) {
-  return static_cast<int>((static_cast<long long>(unit + 1) * min(p.ctas, total) - 1) / total);
-}
-JS_DEVICE int sa_start(const SharedAttn& p, int cta, int total) {
-  const int pieces = min(p.ctas, total);
-  return cta >= pieces ? total : static_cast<int>(static_cast<long long>(total) * cta / pieces);
-}
+// The line is cut into pieces of one length, one for each CTA (none for the last ones where it is short).
+JS_DEVICE int sa_piece(const SharedAttn& p, int total) { return max(1, (total + p.ctas - 1) / p.ctas); }
+
+// Units of an item that begin ahead of place t in it
+JS_DEVICE int sa_unit(int t, bool two) { return (max(0, t - kItemCost) + two) >> two; }
 
 // A CTA's piece of the line, item by item; every role walks it for itself.
 struct SaWalk {
@@ -147,10 +147,11 @@ JS_DEVICE bool sa_next(const SharedAttn& p, SaWalk& w) {
       }
     }
     w.units = sa_units(p, w.s, w.b, w.pair);
-    w.span = min(w.left, w.units + kItemCost - w.t);
-    w.first = max(0, w.t - kItemCost);
-    w.nt = max(0, w.t + w.span - kItemCost) - w.first;
-    w.two = w.s.n - w.pair * 2 * p.npt > p.npt;
+    w.two = sa_weight(p, w.s, w.pair) == 2;
+    w.span = min(w.left, (w.units << w.two) + kItemCost - w.t);
+    // a unit that a cut goes through is the earlier CTA's
+    w.first = sa_unit(w.t, w.two);
+    w.nt = sa_unit(w.t + w.span, w.two) - w.first;
     w.group0 = w.parity;
     if (w.nt > 0) return true;
     sa_done(w);
@@ -318,15 +319,18 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     total += all;
   }
   total += prefix_units;
-  const int u0 = sa_start(p, blockIdx.x, total), u1 = sa_start(p, blockIdx.x + 1, total);
+  const int piece = sa_piece(p, total), u0 = min(static_cast<int>(blockIdx.x) * piece, total), u1 = min(u0 + piece, total);
   if (u0 < prefix_units) {
     if (tid == 0) {
       const SaSeq s = sa_seq(p, -1);
-      const int length = sa_length(p, s, -1, 0);
+      int pair = 0, at = u0, length = sa_length(p, s, -1, 0);      // all pairs but the last are alike
+      if (length > 0) pair = min(at / (length * p.Hkv), sa_pairs(p, s) - 1);
+      at -= pair * length * p.Hkv;
+      length = sa_length(p, s, -1, pair);
       start[0] = -1;
-      start[1] = u0 / length / p.Hkv;
-      start[2] = u0 / length % p.Hkv;
-      start[3] = u0 % length;
+      start[1] = pair;
+      start[2] = at / length;
+      start[3] = at % length;
     }
   } else if (u0 < u1) {
     int run = prefix_units;
@@ -355,7 +359,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (tid == 0 && blockIdx.x == 0) p.plan[0] = total;
+  if (tid == 0 && blockIdx.x == 0) p.plan[0] = piece;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -399,65 +403,74 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     // ================================================================ loaders: warp 9 takes the K tiles, warp 10 the V tiles
     const bool values = warp == 10;
     const CUtensorMap *box = values ? &maps.v16 : &maps.k16, *one = values ? &maps.v1 : &maps.k1;
-    int n = values;                             // ring slots used so far
-    bool ok = true;
-    while (ok && sa_next(p, w)) {
+    // One tile ahead: the slots of the next one, which may be another sequence's, are asked for before this one is issued.
+    struct Tile { int slot[3], row0, keys; };   // keys: to the end of what the item sees, from the tile's first
+    const int* slots = nullptr;
+    int at = 0;                                 // tile of the segment
+    auto open = [&] {
+      at = 0;
+      if (!sa_next(p, w)) return false;
       const bool known = w.s.row >= 0 && w.s.row < p.max_seqs;
       if (!known) report(p.status, kBadSlot);
-      const int* slots = p.slot_map + static_cast<size_t>(known ? w.s.row : 0) * p.max_len;
-      const int end = sa_end(p, w.s, w.b, w.pair), row0 = w.h * p.S;
-      auto slot_at = [&](int i, int part) {     // keys past the end repeat the last one (no row sees them)
-        return __ldg(slots + min(w.s.first + (w.first + i) * SKEYS + 32 * part + lane, end - 1));
-      };
-      int next[3] = {slot_at(0, 0), slot_at(0, 1), slot_at(0, 2)};
-      for (int i = 0; i < w.nt; ++i, n += 2) {
-        int slot[3], page[6];
-        unsigned paged = 0;                     // groups of 16 keys that lie in one page
+      slots = p.slot_map + static_cast<size_t>(known ? w.s.row : 0) * p.max_len;
+      return true;
+    };
+    auto ask = [&](Tile& t) {
+      const int first = w.s.first + (w.first + at) * SKEYS, end = sa_end(p, w.s, w.b, w.pair);
+      t.keys = end - first;
+      t.row0 = w.h * p.S;
 #pragma unroll
-        for (int part = 0; part < 3; ++part) {
-          slot[part] = next[part];
-          if (i + 1 < w.nt) next[part] = slot_at(i + 1, part);
-          if (slot[part] < 0 || slot[part] >= p.S) { report(p.status, kBadSlot); slot[part] = 0; }
-          const int first = __shfl_sync(0xffffffffu, slot[part], lane & 16);
-          const uint32_t in_row = __ballot_sync(0xffffffffu, slot[part] == first + (lane & 15));
-          if ((in_row & 0xffffu) == 0xffffu) paged |= 1u << (2 * part);
-          if ((in_row >> 16) == 0xffffu) paged |= 2u << (2 * part);
-          page[2 * part] = row0 + __shfl_sync(0xffffffffu, slot[part], 0);
-          page[2 * part + 1] = row0 + __shfl_sync(0xffffffffu, slot[part], 16);
-        }
-        // groups behind the last key repeat a page of the tile, where it has one: nobody sees them, but they have to be numbers
-        const int keys = end - (w.s.first + (w.first + i) * SKEYS);
+      for (int part = 0; part < 3; ++part) t.slot[part] = __ldg(slots + min(first + 32 * part + lane, end - 1));      // keys past the end repeat the last one
+      if (++at < w.nt) return true;
+      sa_done(w);
+      return open();
+    };
+    Tile tile, next{};
+    bool have = open(), more = have && ask(tile);
+    for (int n = values; have; n += 2) {
+      have = more;
+      if (more) more = ask(next);
+      // Groups of 16 keys: those in one page load as a box, others four rows at a time, and those behind the last key not at all (the
+      // second product leaves them out, and the scores of the first are masked).
+      unsigned paged = 0;
+      int page[6];
 #pragma unroll
-        for (int part = 0; part < 5; ++part) {
-          if (16 * part < keys || (paged & 0x1fu) == 0) continue;
-          const int any = __ffs(paged & 0x1fu) - 1;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) if (e == any) page[part] = page[e];
-          paged |= 1u << part;
-        }
-        const int s = n % SSLOTS;
-        ok = sa_wait(&kv_empty[s], ((n / SSLOTS) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
-        if (!ok) break;
-        const uint32_t dst = smem_u32(sKV + s * kKTile);
-        if (elect_one()) {
-          mbar_expect_tx(&kv_full[s], kKTile);
-#pragma unroll
-          for (int part = 0; part < 5; ++part) {
-            if (!((paged >> part) & 1u)) continue;
-            sa_tma_box(dst + part * 2048, box, &kv_full[s], 0, page[part]);
-            sa_tma_box(dst + part * 2048 + SKEYS * 128, box, &kv_full[s], 64, page[part]);
-          }
-        }
-        __syncwarp();
-        if ((paged & 0x1fu) == 0x1fu) continue;
+      for (int part = 0; part < 3; ++part) {
+        int& slot = tile.slot[part];
+        if (slot < 0 || slot >= p.S) { report(p.status, kBadSlot); slot = 0; }
+        const int first = __shfl_sync(0xffffffffu, slot, lane & 16);
+        // keys have to be there but need not be seen: the last group's box may go on behind the last key
+        const bool fits = slot == first + (lane & 15) || (!values && 32 * part + lane >= tile.keys && first + 15 < p.S);
+        const uint32_t in_row = __ballot_sync(0xffffffffu, fits);
+        if ((in_row & 0xffffu) == 0xffffu) paged |= 1u << (2 * part);
+        if ((in_row >> 16) == 0xffffu) paged |= 2u << (2 * part);
+        page[2 * part] = tile.row0 + __shfl_sync(0xffffffffu, slot, 0);
+        page[2 * part + 1] = tile.row0 + __shfl_sync(0xffffffffu, slot, 16);
+      }
+      const int groups = min(SKEYS / 16, (tile.keys + 15) / 16);
+      const int s = n % SSLOTS;
+      if (!sa_wait(&kv_empty[s], ((n / SSLOTS) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up)) break;
+      const uint32_t dst = smem_u32(sKV + s * kKTile);
+      if (elect_one()) {
+        mbar_expect_tx(&kv_full[s], groups * 4096);
 #pragma unroll
         for (int part = 0; part < 5; ++part) {
-          if ((paged >> part) & 1u) continue;
+          if (part >= groups || !((paged >> part) & 1u)) continue;
+          sa_tma_box(dst + part * 2048, box, &kv_full[s], 0, page[part]);
+          sa_tma_box(dst + part * 2048 + SKEYS * 128, box, &kv_full[s], 64, page[part]);
+        }
+      }
+      __syncwarp();
+      const unsigned rest = ((1u << groups) - 1u) & ~paged;
+      if (rest != 0) {
+#pragma unroll
+        for (int part = 0; part < 5; ++part) {
+          if (!((rest >> part) & 1u)) continue;
 #pragma unroll
           for (int g = 4 * part; g < 4 * part + 4; ++g) {
             int y[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = row0 + __shfl_sync(0xffffffffu, slot[g / 8], 4 * (g & 7) + e);
+            for (int e = 0; e < 4; ++e) y[e] = tile.row0 + __shfl_sync(0xffffffffu, tile.slot[g / 8], 4 * (g & 7) + e);
             if (elect_one()) {
               sa_tma_rows(dst + g * 512, one, &kv_full[s], 0, y[0], y[1], y[2], y[3]);
               sa_tma_rows(dst + g * 512 + SKEYS * 128, one, &kv_full[s], 64, y[0], y[1], y[2], y[3]);
@@ -466,7 +479,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
           }
         }
       }
-      sa_done(w);
+      tile = next;
     }
   } else if (warp == 8) {
     // ================================================================ issuer of the first product: S = Q K^T of a job once the group's scores before it are read
@@ -505,6 +518,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     int n = 0, tile = 0;
     bool ok = true;
     while (ok && sa_next(p, w)) {
+      const int end = sa_end(p, w.s, w.b, w.pair);
       const int sides = w.two ? 2 : 1, jobs = w.nt * sides;
       for (int job = 0; job < jobs; ++job, ++n) {
         const int g = n & 1, slot = 2 * (tile + (w.two ? job >> 1 : job)) + 1, s = slot % SSLOTS;
@@ -513,9 +527,10 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         tc_fence_after();
         if (elect_one()) {
           const uint64_t b = v_desc + static_cast<uint64_t>(s * (kKTile >> 4));
+          const int keys = end - (w.s.first + (w.first + (w.two ? job >> 1 : job)) * SKEYS);
 #pragma unroll
           for (int k = 0; k < SKEYS / 16; ++k)
-            sa_mma_tmem_a(tmem + kColO + g * 128, tmem + g * 128 + kColP + k * 8, b + k * (2048 >> 4), idesc, k != 0 || job >= 2);
+            if (16 * k < keys) sa_mma_tmem_a(tmem + kColO + g * 128, tmem + g * 128 + kColP + k * 8, b + k * (2048 >> 4), idesc, k != 0 || job >= 2);
           umma_commit(&pv_done[g]);
           if (!w.two || (job & 1)) umma_commit(&kv_empty[s]);
         }
@@ -651,6 +666,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
           }
         }
       }
+      if (p.prefix == 0 && (warp & 3) == 0 && lane == 0 && (w.two || rel == 0))
+        p.parted[(w.s.q_begin / p.npt + w.b + w.pair * 2 + side) * p.Hkv + w.h] = !direct;
       if (valid && !direct) {
         if (row < rows) (prefix ? p.pml : p.sml)[at] = make_float2(m_run, l_run);
         else report(p.status, kRowsOverflow);   // more rows in a sequence than the caller's bound
@@ -679,6 +696,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
     const size_t block = (static_cast<size_t>(blockIdx.z) * gridDim.y + h) * gridDim.x + blockIdx.x;
     for (size_t i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) out[i] = make_uint4(0u, 0u, 0u, 0u);
   }
+  if (p.prefix == 0) {                         // most tiles were written by their CTA
+    pdl_wait();
+    if (p.parted[blockIdx.x * p.Hkv + h] == 0) return;
+  }
   // tiles are numbered like pairs: those of a sequence start behind the tiles of all rows before it
   int b = -1;                                  // the last sequence that starts at or before this tile
   for (int base = 0; base < p.B; base += 32) {
@@ -692,14 +713,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
   const int rows = min(p.npt, s.n - node0) * p.G;
   if (rows <= row0) return;
   pdl_wait();
-  const int total = p.plan[0], pair = tile >> 1, units = sa_units(p, s, b, pair);
+  const int piece = p.plan[0], pair = tile >> 1, units = sa_units(p, s, b, pair);
   const bool two = s.n - pair * 2 * p.npt > p.npt;
-  int c0 = 0, own = 0, item = 0;               // first CTA and number of CTAs with a part of the sequence's own keys
+  int c0 = 0, own = 0, item = 0, own_begin = 0;      // first CTA and number of CTAs with a part of the sequence's own keys
   if (units > 0) {
     item = sa_item(p, s, b, pair, h);
-    const int u = p.plan[1 + item];
-    c0 = sa_cta(p, u + kItemCost, total);
-    own = sa_cta(p, u + kItemCost + units - 1, total) - c0 + 1;
+    const int u = own_begin = p.plan[1 + item];
+    c0 = (u + kItemCost) / piece;
+    own = (u + kItemCost + ((units - 1) << two)) / piece - c0 + 1;
     item -= p.prefix_items;
   }
   if (own == 1 && two && p.prefix == 0) return;       // written by its CTA
@@ -708,15 +729,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
   const int own_parts = two ? own : 2 * own;
   for (int row = row0 + warp; row < min(rows, row0 + kMergeRows); row += kMergeWarps) {
     const int tok = row / p.G, t = s.q_begin + node0 + tok, head = h * p.G + row - tok * p.G;
-    int pc0 = 0, shared_parts = 0, p_item = 0, p_row = 0;
+    int pc0 = 0, shared_parts = 0, p_item = 0, p_row = 0, p_begin = 0;
     bool p_two = false;
     if (all_units > 0) {
       const int p_tile = t / p.npt, p_pair = p_tile >> 1;
       p_item = sa_item(p, all, -1, p_pair, h);
-      const int u = (p_pair * p.Hkv + h) * (all_units + kItemCost) + kItemCost;
-      pc0 = sa_cta(p, u, total);
-      p_two = all.n - p_pair * 2 * p.npt > p.npt;
-      shared_parts = (sa_cta(p, u + all_units - 1, total) - pc0 + 1) * (p_two ? 1 : 2);
+      p_two = sa_weight(p, all, p_pair) == 2;
+      p_begin = p_pair * p.Hkv * sa_length(p, all, -1, 0) + h * sa_length(p, all, -1, p_pair);
+      pc0 = (p_begin + kItemCost) / piece;
+      shared_parts = ((p_begin + kItemCost + ((all_units - 1) << p_two)) / piece - pc0 + 1) * (p_two ? 1 : 2);
       p_row = (t - p_tile * p.npt) * p.G + row - tok * p.G + (p_two ? (p_tile & 1) * SROWS : 0);
     }
     const int parts = shared_parts + own_parts;
@@ -726,7 +747,12 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
       const int k = base + lane;
       const float* at = nullptr;
       float2 ml = make_float2(-INFINITY, 0.f);
-      if (k < shared_parts) {
+      // a cut piece may hold no unit's beginning, and then no part
+      const int c = k < shared_parts ? pc0 + (p_two ? k : k >> 1) : c0 + (two ? k - shared_parts : (k - shared_parts) >> 1);
+      const int begin = k < shared_parts ? p_begin : own_begin;
+      const bool pair_of = k < shared_parts ? p_two : two;
+      if (k >= parts || sa_unit(c * piece - begin, pair_of) == sa_unit((c + 1) * piece - begin, pair_of)) {
+      } else if (k < shared_parts) {
         const size_t r = (static_cast<size_t>(pc0 + (p_two ? k : k >> 1) + p_item) * 2 + (p_two ? 0 : k & 1)) * SROWS + p_row;
         ml = p.pml[r];
         at = p.po + r * SD;
@@ -786,6 +812,7 @@ static long long shared_layout(SharedAttn* p, uint8_t* ws, int max_q) {
   long long at = 0;
   auto take = [&](long long bytes) { uint8_t* r = ws + at; at += shared_round(bytes); return r; };
   p->plan = reinterpret_cast<int*>(take(4ll * (1 + p->prefix_items + p->seq_items)));
+  p->parted = take((p->T / p->npt + p->B + 1ll) * p->Hkv);
   p->pml = reinterpret_cast<float2*>(take(8 * prefix_rows));
   p->sml = reinterpret_cast<float2*>(take(8 * rows));
   p->po = reinterpret_cast<float*>(take(4 * SD * prefix_rows));
