@@ -10,8 +10,8 @@
 // item's units in key order behind a few that stand for what it costs beside them.  Every CTA takes an equal piece of the line, so lengths, which only the device knows, balance by
 // themselves; where a piece begins or ends inside an item its parts go through a workspace and attn_shared_merge_kernel.
 //
-// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warps 8 and 12 issue the MMAs of either product, warps 9 and 10 load K and V by
-// TMA (boxes of 16 rows where slots follow one another, gathers of four rows where not), warp 11 loads Q.  A job is one row tile against 80 keys; jobs alternate between the
+// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warps 8 and 11 issue the MMAs of either product, warps 9 and 10 load K and V (and Q) by
+// TMA (boxes of 16 rows where slots follow one another, gathers of four rows where not).  A job is one row tile against 80 keys; jobs alternate between the
 // groups: the two tiles of a pair on the same keys, or, for a single tile, every other block of keys.  Tensor memory holds
 // scores (80 columns), probabilities as bf16 (40; the second MMA's A operand) and output (128) of both groups, so that a group's next scores
 // are there while it weighs its last ones.  Every wait is bounded (status word).
@@ -26,9 +26,9 @@ constexpr int SD = 128;              // head dim
 constexpr int SROWS = 128;           // rows of a tile
 constexpr int SKEYS = 80;            // keys of a unit: scores (80 columns) and probabilities (40) of a group fit 128 columns side by side
 constexpr int SSLOTS = 8;            // ring of K and V tiles, in turn
-constexpr int kItemCost = 8;         // what an item costs beside its jobs, in jobs: setting out, and results out of tensor memory
+constexpr int kItemCost = 6;         // what an item costs beside its jobs, in jobs: setting out, and results out of tensor memory
 constexpr int kQTile = SROWS * 256, kKTile = SKEYS * 256;      // bytes of a Q, K or V tile: 2 halves x rows x 128 B
-constexpr int SWARPS = 13, STHREADS = 32 * SWARPS;      // 152 registers a thread
+constexpr int SWARPS = 12, STHREADS = 32 * SWARPS;      // three warps to a quarter of the SM: 168 registers a thread
 constexpr int kSharedSmem = 2 * kQTile + SSLOTS * kKTile + 512;
 constexpr int kColP = SKEYS, kColO = 256;      // tensor memory: scores of group g from column 128 g, its probabilities behind them, its output from 256 + 128 g
 
@@ -291,7 +291,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   }
   int* scan = start + 8;                        // a total per warp
   const int prefix_units = p.prefix > 0 ? sa_total(p, -1) * p.Hkv : 0;
-  // units of the sequences ahead of this thread's (of every 416), and of all of them
+  // units of the sequences ahead of this thread's (of every 384), and of all of them
   auto ahead = [&](int value, int& all) {
     int inc = value;
 #pragma unroll
@@ -376,35 +376,15 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   w.parity = 0;
   sa_begin(p, w);
 
-  if (warp == 11) {
-    // ================================================================ Q loader; it notes where items begin
-    int uses = 0;                               // Q buffers filled so far: buffer uses % 2
-    bool ok = true;
-    while (ok && sa_next(p, w)) {
-      if (lane == 0 && w.first == 0) p.plan[1 + sa_item(p, w.s, w.b, w.pair, w.h)] = w.at - w.t;
-      for (int side = 0; side < (w.two ? 2 : 1) && ok; ++side, ++uses) {
-        const int buf = uses & 1;
-        ok = sa_wait(&q_empty[buf], ((uses >> 1) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
-        if (!ok) break;
-        // A box holds the G heads of npt tokens.  Those behind the sequence's last one are another's or zero: a row's scores and output
-        // are its own, and nobody reads these.
-        if (elect_one()) {
-          mbar_expect_tx(&q_full[buf], p.npt * p.G * SD * 2);
-          const uint32_t dst = smem_u32(sQ + buf * kQTile);
-          const int token = w.s.q_begin + (w.pair * 2 + side) * p.npt;
-          sa_tma_heads(dst, &maps.q, &q_full[buf], 0, w.h * p.G, token);
-          sa_tma_heads(dst + SROWS * 128, &maps.q, &q_full[buf], 64, w.h * p.G, token);
-        }
-        __syncwarp();
-      }
-      sa_done(w);
-    }
-  } else if (warp == 9 || warp == 10) {
-    // ================================================================ loaders: warp 9 takes the K tiles, warp 10 the V tiles
+  if (warp == 9 || warp == 10) {
+    // ================================================================ loaders: warp 9 takes the K tiles, warp 10 the V tiles and, ahead of an item's first, its Q tiles
     const bool values = warp == 10;
     const CUtensorMap *box = values ? &maps.v16 : &maps.k16, *one = values ? &maps.v1 : &maps.k1;
     // One tile ahead: the slots of the next one, which may be another sequence's, are asked for before this one is issued.
-    struct Tile { int slot[3], row0, keys; };   // keys: to the end of what the item sees, from the tile's first
+    struct Tile {
+      int slot[3], row0, keys;                  // keys: to the end of what the item sees, from the tile's first
+      int token, h, sides;                      // a segment's first tile: its Q tiles (sides 0: another tile)
+    };
     const int* slots = nullptr;
     int at = 0;                                 // tile of the segment
     auto open = [&] {
@@ -413,12 +393,16 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const bool known = w.s.row >= 0 && w.s.row < p.max_seqs;
       if (!known) report(p.status, kBadSlot);
       slots = p.slot_map + static_cast<size_t>(known ? w.s.row : 0) * p.max_len;
+      if (values && lane == 0 && w.first == 0) p.plan[1 + sa_item(p, w.s, w.b, w.pair, w.h)] = w.at - w.t;      // where the item begins
       return true;
     };
     auto ask = [&](Tile& t) {
       const int first = w.s.first + (w.first + at) * SKEYS, end = sa_end(p, w.s, w.b, w.pair);
       t.keys = end - first;
       t.row0 = w.h * p.S;
+      t.token = w.s.q_begin + w.pair * 2 * p.npt;
+      t.h = w.h;
+      t.sides = at > 0 ? 0 : w.two ? 2 : 1;
 #pragma unroll
       for (int part = 0; part < 3; ++part) t.slot[part] = __ldg(slots + min(first + 32 * part + lane, end - 1));      // keys past the end repeat the last one
       if (++at < w.nt) return true;
@@ -426,10 +410,27 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       return open();
     };
     Tile tile, next{};
-    bool have = open(), more = have && ask(tile);
+    bool have = open(), more = have && ask(tile), ok = true;
+    int uses = 0;                               // Q buffers filled so far: buffer uses % 2
     for (int n = values; have; n += 2) {
       have = more;
       if (more) more = ask(next);
+      for (int side = 0; values && side < tile.sides && ok; ++side, ++uses) {
+        const int buf = uses & 1;
+        ok = sa_wait(&q_empty[buf], ((uses >> 1) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up);
+        if (!ok) break;
+        // A box holds the G heads of npt tokens.  Those behind the sequence's last one are another's or zero: a row's scores and output
+        // are its own, and nobody reads these.
+        if (elect_one()) {
+          mbar_expect_tx(&q_full[buf], p.npt * p.G * SD * 2);
+          const uint32_t dst = smem_u32(sQ + buf * kQTile);
+          const int token = tile.token + side * p.npt;
+          sa_tma_heads(dst, &maps.q, &q_full[buf], 0, tile.h * p.G, token);
+          sa_tma_heads(dst + SROWS * 128, &maps.q, &q_full[buf], 64, tile.h * p.G, token);
+        }
+        __syncwarp();
+      }
+      if (!ok) break;
       // Groups of 16 keys: those in one page load as a box, others four rows at a time, and those behind the last key not at all (the
       // second product leaves them out, and the scores of the first are masked).
       unsigned paged = 0;
@@ -511,7 +512,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       use += sides;
       sa_done(w);
     }
-  } else if (warp == 12) {
+  } else if (warp == 11) {
     // ================================================================ issuer of the second product: O += P V
     constexpr uint32_t idesc = umma_idesc_bf16(SROWS, SD) | (1u << 16);
     const uint64_t v_desc = sa_desc_mn(smem_u32(sKV), SKEYS * 128);
@@ -546,7 +547,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     const uint32_t ts = tmem + t_lane + g * 128, to = tmem + t_lane + kColO + g * 128;
     int jobs_done = 0;                          // of this group: the phase of its barriers
     bool ok = true;
-    while (ok && sa_next(p, w)) {
+    bool more = sa_next(p, w);
+    while (ok && more) {
       const bool prefix = w.b < 0;
       const int rel = g ^ w.group0, side = w.two ? rel : 0;
       const int node = (w.pair * 2 + side) * p.npt + tok, head = w.h * p.G + sub;
@@ -559,6 +561,11 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       for (int i = w.two ? 0 : rel; i < w.nt && ok; i += w.two ? 1 : 2, ++jobs, ++jobs_done) {
         const int k0 = w.s.first + (w.first + i) * SKEYS;
         const bool all = k0 + SKEYS <= min(w.s.past, end);      // every row of the item sees the whole block
+        uint32_t see[3] = {0u, 0u, 0u};
+        if (!all && valid) {
+#pragma unroll
+          for (int c = 0; c < 3; ++c) see[c] = sa_visible(p, w.s, prefix, end, node, bits, k0 + 32 * c);
+        }
         ok = sa_wait(&s_full[g], jobs_done & 1, p.status, kTimeoutAccum, gave_up);
         if (!ok) break;
         tc_fence_after();
@@ -578,12 +585,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         mbar_arrive(&s_read[g]);
         if (!all) {                             // scores of keys the row does not see
 #pragma unroll
-          for (int c = 0; c < SKEYS; c += 32) {
-            const uint32_t see = valid ? sa_visible(p, w.s, prefix, end, node, bits, k0 + c) : 0u;
-#pragma unroll
-            for (int j = 0; j < 32 && c + j < SKEYS; ++j)
-              if (!((see >> j) & 1u)) sr[c + j] = 0xff800000u;      // -inf
-          }
+          for (int j = 0; j < SKEYS; ++j)
+            if (!((see[j >> 5] >> (j & 31)) & 1u)) sr[j] = 0xff800000u;      // -inf
         }
         float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -639,40 +642,45 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const int rows = prefix ? SROWS : p.seq_rows_kept;
       const size_t seg = static_cast<size_t>(blockIdx.x) + (prefix ? item : item - p.prefix_items);
       const size_t at = (seg * 2 + rel) * rows + row;
+      const bool keep = valid && !direct && row < rows;
+      __nv_bfloat16* out = direct ? p.out + (static_cast<size_t>(w.s.q_begin + node) * p.Hq + head) * SD : nullptr;
+      float* part = (prefix ? p.po : p.so) + at * SD;
+      if (keep) (prefix ? p.pml : p.sml)[at] = make_float2(m_run, l_run);
+      else if (valid && !direct) report(p.status, kRowsOverflow);      // more rows in a sequence than the caller's bound
+      if (p.prefix == 0 && (warp & 3) == 0 && lane == 0 && (w.two || rel == 0))
+        p.parted[(w.s.q_begin / p.npt + w.b + w.pair * 2 + side) * p.Hkv + w.h] = !direct;
+      sa_done(w);
+      more = sa_next(p, w);                     // what it asks memory for comes while the last product ends
       if (jobs > 0) {
         ok = sa_wait(&pv_done[g], (jobs_done - 1) & 1, p.status, kTimeoutAccum, gave_up);
         if (!ok) break;
         tc_fence_after();
         const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
 #pragma unroll 1
-        for (int c = 0; busy && c < SD; c += 32) {
-          uint32_t o[32];
+        for (int c = 0; busy && c < SD; c += 64) {
+          uint32_t o[64];
           tmem_ld_32x32(to + c, o);
+          tmem_ld_32x32(to + c + 32, o + 32);
           tmem_ld_wait();
-          if (!valid) continue;
-          if (direct) {
-            uint4 pk[4];
-            __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(pk);
+          if (direct && valid) {
+            uint4* dst = reinterpret_cast<uint4*>(out + c);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) o2[j] = __floats2bfloat162_rn(__uint_as_float(o[2 * j]) * inv, __uint_as_float(o[2 * j + 1]) * inv);
-            uint4* dst = reinterpret_cast<uint4*>(p.out + (static_cast<size_t>(w.s.q_begin + node) * p.Hq + head) * SD + c);
+            for (int j = 0; j < 8; ++j) {
+              uint4 pk;
+              __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&pk);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) dst[j] = pk[j];
-          } else if (row < rows) {
-            float4* dst = reinterpret_cast<float4*>((prefix ? p.po : p.so) + at * SD + c);
+              for (int e = 0; e < 4; ++e)
+                o2[e] = __floats2bfloat162_rn(__uint_as_float(o[8 * j + 2 * e]) * inv, __uint_as_float(o[8 * j + 2 * e + 1]) * inv);
+              dst[j] = pk;
+            }
+          } else if (keep) {
+            float4* dst = reinterpret_cast<float4*>(part + c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 16; ++j)
               dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
           }
         }
       }
-      if (p.prefix == 0 && (warp & 3) == 0 && lane == 0 && (w.two || rel == 0))
-        p.parted[(w.s.q_begin / p.npt + w.b + w.pair * 2 + side) * p.Hkv + w.h] = !direct;
-      if (valid && !direct) {
-        if (row < rows) (prefix ? p.pml : p.sml)[at] = make_float2(m_run, l_run);
-        else report(p.status, kRowsOverflow);   // more rows in a sequence than the caller's bound
-      }
-      sa_done(w);
     }
   }
 
