@@ -30,6 +30,9 @@ constexpr int kItemCost = 6;         // what an item costs beside its jobs, in j
 constexpr int kQTile = SROWS * 256, kKTile = SKEYS * 256;      // bytes of a Q, K or V tile: 2 halves x rows x 128 B
 constexpr int SWARPS = 12, STHREADS = 32 * SWARPS;      // three warps to a quarter of the SM: 168 registers a thread
 constexpr int kSharedSmem = 2 * kQTile + SSLOTS * kKTile + 512;
+// Of eight pairs of exponentials, those computed on the FMA pipe: 16 trees of 128 nodes 332 us without, 321, 316, 325 and 329 us with 1 to 4
+// (the special function unit alone takes 640 cycles a job, the MMAs 730).
+constexpr int kOnFma = 2;
 constexpr int kColP = SKEYS, kColO = 256;      // tensor memory: scores of group g from column 128 g, its probabilities behind them, its output from 256 + 128 g
 
 struct SharedAttn {
@@ -213,6 +216,27 @@ JS_DEVICE uint64_t sa_add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+// 2^x for both of a pair on the FMA pipe, x <= 0: the nearest integer goes to the exponent, the rest f through the cubic that is 1 at 0 and
+// nearest to 2^f in relative error over [-1/2, 1/2] (1.0e-4, a fortieth of half a bf16 step).  x is cut at -127, which gives 0.
+JS_DEVICE void sa_exp2_pair(uint64_t x, float& lo, float& hi) {
+  constexpr float kRound = 12582912.f;           // 1.5 * 2^23: the sum's low bits are the integer
+  float a, b;
+  sa_unpack(x, a, b);
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));      // -127
+  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
+  x = sa_pack(a, b);
+  const uint64_t t = sa_add2(x, sa_pack(kRound, kRound));
+  const uint64_t n = sa_add2(t, sa_pack(-kRound, -kRound));
+  const uint64_t f = sa_fma2(n, sa_pack(-1.f, -1.f), x);
+  uint64_t y = sa_fma2(f, sa_pack(0.05500864f, 0.05500864f), sa_pack(0.2422105f, 0.2422105f));
+  y = sa_fma2(y, f, sa_pack(0.69328291f, 0.69328291f));
+  y = sa_fma2(y, f, sa_pack(1.f, 1.f));
+  float ta, tb, ya, yb;
+  sa_unpack(t, ta, tb);
+  sa_unpack(y, ya, yb);
+  lo = __int_as_float((__float_as_int(ta) << 23) + __float_as_int(ya));
+  hi = __int_as_float((__float_as_int(tb) << 23) + __float_as_int(yb));
 }
 JS_DEVICE void sa_tma_heads(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int head, int token) {
   asm volatile(
@@ -604,9 +628,14 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
 #pragma unroll
         for (int j = 0; j < SKEYS / 2; ++j) {
           float p0, p1;
-          sa_unpack(sa_fma2(sa_pack(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), scale2, shift2), p0, p1);
-          p0 = sa_exp2(p0);
-          p1 = sa_exp2(p1);
+          const uint64_t x = sa_fma2(sa_pack(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), scale2, shift2);
+          if (j % 8 < kOnFma) {
+            sa_exp2_pair(x, p0, p1);
+          } else {
+            sa_unpack(x, p0, p1);
+            p0 = sa_exp2(p0);
+            p1 = sa_exp2(p1);
+          }
           sum2[j & 3] = sa_add2(sum2[j & 3], sa_pack(p0, p1));
           const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);      // the MMA's operand: bf16, the sum keeps fp32
           pr[j] = *reinterpret_cast<const uint32_t*>(&v);
@@ -704,6 +733,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
     const size_t block = (static_cast<size_t>(blockIdx.z) * gridDim.y + h) * gridDim.x + blockIdx.x;
     for (size_t i = block * blockDim.x + threadIdx.x; i < n; i += blocks * blockDim.x) out[i] = make_uint4(0u, 0u, 0u, 0u);
   }
+  // Every block waits, also one without a row: this kernel ends behind the one before, and what follows it on the stream waits for this one alone.
   if (p.prefix == 0) {                         // most tiles were written by their CTA
     pdl_wait();
     if (p.parted[blockIdx.x * p.Hkv + h] == 0) return;
@@ -715,12 +745,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
     b += __popc(some);
     if (some != 0xffffffffu) break;
   }
-  if (b < 0) return;
+  if (b < 0) {
+    pdl_wait();
+    return;
+  }
   const SaSeq s = sa_seq(p, b);
   const int tile = blockIdx.x - (s.q_begin / p.npt + b), node0 = tile * p.npt;
   const int rows = min(p.npt, s.n - node0) * p.G;
-  if (rows <= row0) return;
   pdl_wait();
+  if (rows <= row0) return;
   const int piece = p.plan[0], pair = tile >> 1, units = sa_units(p, s, b, pair);
   const bool two = s.n - pair * 2 * p.npt > p.npt;
   int c0 = 0, own = 0, item = 0, own_begin = 0;      // first CTA and number of CTAs with a part of the sequence's own keys

@@ -8,9 +8,7 @@
 //
 // chain_stats_kernel reads the rows of some drafts (maximum, sum of exponentials) and decides about them; chain_token_kernel draws the token, a
 // cluster per sequence.  Where reading every row would take long, the first kernel runs for draft 0 of all sequences, then 1, 2, 3-4, 5-8 and the
-// rest, so that rows behind a rejection are not read.  (Measured at 64 sequences of 4 to 16 drafts over 151936 fp32 values, a third of the rows
-// needed: one persistent launch that picks drafts as they become known to be needed reads half of what it reads in vain and
-// waits for its own agreements, 136 us; launches in turn: see below.)  Sums that only decide `u q < p` are fp32 (a decision is off by 1e-7 of a
+// rest, so that rows behind a rejection are not read.  Sums that only decide `u q < p` are fp32 (a decision is off by 1e-7 of a
 // probability); the running sum that a token is found in is fp64, as its index would change with every rounding among 150,000 terms.
 #include "common.cuh"
 
@@ -126,10 +124,10 @@ __global__ void __launch_bounds__(kStatThreads, 4) chain_stats_kernel(ChainParam
   pdl_launch_dependents();
   int first;
   const int n = chain_span(p, b, first);
+  pdl_wait();                                  // what the launch before decided; ahead of any return, so that launches end in their order
   if (lo + static_cast<int>(blockIdx.z) > n) return;
   const double temps[2] = {chain_temp(p.temp, p.temp_all, b), chain_temp(p.draft_temp, p.draft_temp_all, b)};
   const float scales[2] = {chain_scale(temps[0]), chain_scale(temps[1])};
-  pdl_wait();                                  // what the launch before decided
   for (int i = lo + blockIdx.z; i < hi && i <= n; i += gridDim.z) {
     // Behind a known rejection nobody needs the rows; whether they are read all the same goes by time, results do not.
     __syncthreads();
