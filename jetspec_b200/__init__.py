@@ -20,6 +20,7 @@ _LAZY = {
     "RandomTreeDrafter": "jetspec_b200.drafters",
     "TargetEchoTreeDrafter": "jetspec_b200.drafters",
     "DraftHeadDrafter": "jetspec_b200.drafters",
+    "SamplingHeadDrafter": "jetspec_b200.drafters",
     "DraftHeadTreeDrafter": "jetspec_b200.drafters",
     "OracleTreeDrafter": "jetspec_b200.drafters",
     "GraphedDraftHead": "jetspec_b200.drafters",

@@ -16,6 +16,7 @@ from typing import Optional
 
 import torch
 
+from .. import ops
 from ..models import is_model, load_target
 from ..sampling import SamplingParams, sample
 from ..tree import build_ancestor_matrix, get_algorithm, gpu_tree_accept, tree_accept
@@ -103,7 +104,9 @@ class LLM:
                        sampling_params: SamplingParams = None) -> dict:
         """Linear speculative decode: ``k = max(1, block_size-1)`` drafts per round, verified in one
         forward over ``[anchor | drafts]``; the longest greedy-equal prefix plus one correction is
-        committed and the rejected drafts' KV cropped.  Returns ``{"token_ids","text","tpf"}``."""
+        committed and the rejected drafts' KV cropped.  With a temperature and a drafter that samples
+        (see :class:`~jetspec_b200.drafters.base.Drafter`) drafts are verified against the target's probabilities instead
+        (:func:`jetspec_b200.ops.verify_chains`): the tokens are then samples of the target.  Returns ``{"token_ids","text","tpf"}``."""
         sp = sampling_params or SamplingParams()
         committed = self._ids(prompt)
         check_positions(self.model.config, committed.shape[1] + sp.max_new_tokens - 1)
@@ -111,6 +114,7 @@ class LLM:
             drafter.reset_cache()
         k = max(1, block_size - 1)
         taps = list(target_layer_ids) if (target_layer_ids is not None and block_size > 1) else None
+        sampled = sp.temperature > 0.0 and hasattr(drafter, "propose_sampled")
         cache = self.runner.new_cache(committed.shape[1] + sp.max_new_tokens + k + 2)
         logits, cache, target_hidden = self.runner.forward(committed, cache, target_layer_ids=taps,
                                                            last_position_logits_only=True)
@@ -121,18 +125,30 @@ class LLM:
             return {"token_ids": new_ids[: sp.max_new_tokens], "text": decode_text(self.tokenizer, new_ids), "tpf": 0.0}
         done = False
         while len(new_ids) < sp.max_new_tokens and not done:
-            drafts = drafter.propose(committed, k, target_hidden=target_hidden).to(self.device).reshape(-1)[:k]
+            draft_logits = None
+            if sampled:
+                drafts, draft_logits = drafter.propose_sampled(committed, k, sp.temperature, target_hidden=target_hidden)
+                drafts, draft_logits = drafts.to(self.device).reshape(-1)[:k], draft_logits.to(self.device)[:k]
+            else:
+                drafts = drafter.propose(committed, k, target_hidden=target_hidden).to(self.device).reshape(-1)[:k]
             step = torch.cat((committed[:, -1:], drafts.reshape(1, -1)), 1)
             past = cache.length
             logits, cache, hid = self.runner.forward(step, cache, target_layer_ids=taps)
             rounds += 1
-            greedy = logits[0].argmax(-1)
-            agree = (drafts == greedy[:k]).to(torch.int64)
-            acc = int(torch.cumprod(agree, 0).sum())
+            if sampled:
+                n = drafts.numel()
+                kept, nxt = ops.verify_chains(logits[0], draft_logits, drafts.to(torch.int32), torch.tensor([0, n], dtype=torch.int32, device=self.device),
+                                              torch.rand(n, device=self.device), torch.rand(1, device=self.device), temperature=sp.temperature)
+                acc = int(kept)
+            else:
+                greedy = logits[0].argmax(-1)
+                agree = (drafts == greedy[:k]).to(torch.int64)
+                acc = int(torch.cumprod(agree, 0).sum())
+                nxt = greedy[acc]
             cache.crop(past + 1 + acc)
             if hid is not None:
                 target_hidden = torch.cat((target_hidden, hid[:, : 1 + acc]), 1)
-            block = torch.cat((drafts[:acc], greedy[acc].reshape(1)))
+            block = torch.cat((drafts[:acc], nxt.reshape(1).to(drafts.dtype)))
             committed = torch.cat((committed, block.reshape(1, -1)), 1)
             for t in block.tolist():
                 new_ids.append(int(t))

@@ -18,7 +18,10 @@ class Drafter(ABC):
     @abstractmethod
     def propose(self, context_ids: torch.Tensor, k: int, target_hidden: torch.Tensor = None, **kwargs) -> torch.Tensor:
         """``context_ids (1, T)`` → ``(k,)`` proposed token ids.  ``target_hidden``
-        ``(1, T-1, taps*H)`` is what a real draft head conditions on; stubs ignore it."""
+        ``(1, T-1, taps*H)`` is what a real draft head conditions on; stubs ignore it.
+
+        A drafter that draws its tokens may also offer ``propose_sampled(context_ids, k, temperature, target_hidden=None)`` → ``(k,)``
+        token ids, each drawn from ``softmax(logits / temperature)`` of its row, and the ``(k, V)`` logits."""
 
 
 class TreeDrafter(ABC):

@@ -99,6 +99,15 @@ class DraftHeadDrafter(_HeadDrafterMixin, Drafter):
         return idx
 
 
+class SamplingHeadDrafter(DraftHeadDrafter):
+    """Chain drafter whose tokens are draws: at a temperature the drafts can then be verified against the target's probabilities."""
+
+    @torch.inference_mode()
+    def propose_sampled(self, context_ids, k, temperature, target_hidden=None, **kwargs):
+        logits = self._fwd.logits(context_ids, target_hidden, k)[0]
+        return ops.sample(logits, temperature), logits
+
+
 class DraftHeadTreeDrafter(_HeadDrafterMixin, TreeDrafter):
     """Tree drafter: raw per-depth logits (or their top-k) from one head forward."""
 

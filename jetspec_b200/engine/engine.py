@@ -233,12 +233,12 @@ class JetSpecEngine:
             sid, toks, _ = entries[i]
             have = pool.state(sid).length if pool.has(sid) else 0
             check_positions(self.cfg, have + len(toks))
-            pool.reserve(sid, have + len(toks))
             seqs.append(sid)
             rows.append(torch.tensor(toks, dtype=torch.long, device=self.device))
             past.append(have)
             start[i] = first
             first += len(toks)
+        pool.reserve_batch(seqs, [have + int(t.numel()) for have, t in zip(past, rows)])
         want = [start[i] + int(k) for i, (_, _, w) in enumerate(entries) for k in w]
         logits, _, _ = self._forward(seqs, rows, past, logits_rows=torch.tensor(want, dtype=torch.long, device=self.device))
         for sid, have, toks in zip(seqs, past, rows):

@@ -1533,8 +1533,9 @@ def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_le
             _refuse("mask_bits: without the causal rule every query needs a row of words")
         _ints(index, mask_bits=mask_bits)
         words, bits = mask_bits.shape[1], mask_bits.data_ptr()
-    if not (0 <= prefix_len <= max_len and max_q >= 1 and 0.0 < scale < math.inf):
+    if not (0 <= prefix_len <= max_len and max_q >= 0 and 0.0 < scale < math.inf):
         _refuse(f"prefix_len={prefix_len} of {max_len}, max_q={max_q}, scale={scale}")
+    max_q = max(max_q, 1)
     if q.stride(2) != 1 or q.stride(1) != 128 or q.stride(0) % 8 or q.stride(0) < Hq * 128 or q.data_ptr() % 16:
         q = q.contiguous()
     if out is None:

@@ -244,12 +244,8 @@ class PagedKVPool:
             except EvictionFailed:
                 return False
         if need > 0:
-            new_pages = [self._free_pages.popleft() for _ in range(need)]
-            for p in new_pages:
-                assert self._refcount[p] == 0, f"page {p} handed out twice"
-                self._refcount[p] = 1
             base = len(st.pages) * self.page_size
-            st.pages.extend(new_pages)
+            new_pages = self._take_pages(st, need)
             ids = (torch.tensor(new_pages, dtype=torch.int32).repeat_interleave(self.page_size) * self.page_size
                    + torch.arange(self.page_size, dtype=torch.int32).repeat(len(new_pages)))
             end = min(base + ids.numel(), self.max_seq_len)
@@ -260,11 +256,58 @@ class PagedKVPool:
         st.last_used = next(self._clock)
         return True
 
+    def _take_pages(self, st: SeqState, need: int) -> list:
+        """The next ``need`` free pages, now ``st``'s."""
+        new_pages = [self._free_pages.popleft() for _ in range(need)]
+        for p in new_pages:
+            assert self._refcount[p] == 0, f"page {p} handed out twice"
+            self._refcount[p] = 1
+        st.pages.extend(new_pages)
+        return new_pages
+
     def reserve(self, seq_id: int, num_tokens: int) -> None:
         """Like :meth:`allocate_slots` but never evicts and raises when it does not fit."""
         if not self.allocate_slots(seq_id, num_tokens, allow_evict=False):
             raise EvictionRequired(f"sequence {seq_id} needs {self.pages_for(num_tokens)} pages; "
                                    f"{len(self._free_pages)} free")
+
+    def reserve_batch(self, seq_ids: list, num_tokens: list) -> None:
+        """:meth:`reserve` for several sequences, in order; their slot maps are written by one
+        :func:`~jetspec_b200.ops.plan_slots`."""
+        grown, pages = {}, []      # slot-map row -> (sequence, positions it held), in the order that pages were taken
+
+        def write():
+            if not pages:
+                return
+            from .. import ops
+            n, states = len(grown), list(grown.values())
+            covered = [min(len(st.pages) * self.page_size, self.max_seq_len) for st, _ in states]
+            packed = torch.tensor([*grown, *covered, *(base for _, base in states), *([0] * n), *pages], dtype=torch.int32)
+            rows, covered, held, none, free = packed.to(self.device, non_blocking=True).split((n, n, n, n, len(pages)))
+            ops.plan_slots(covered, none, rows, free, self.page_size, self.slot_map, 0, mapped_lens=held)
+            for st, base in states:
+                if self.block_maps:
+                    self._map_blocks(st, base)
+            grown.clear()
+            pages.clear()
+
+        for sid, tokens in zip(seq_ids, num_tokens):
+            st = self._seqs.get(sid)
+            need = self.pages_for(tokens) - (len(st.pages) if st is not None else 0)
+            if tokens > self.max_seq_len or (st is None and not self._free_rows) or need > len(self._free_pages):
+                write()
+                self.reserve(sid, tokens)          # raises, and says why it does not fit
+                continue
+            if st is None:
+                st = self._seqs[sid] = SeqState(sid, self._free_rows.popleft())
+            if need > 0:
+                if st.row in grown:                # a plan serves a slot-map row once
+                    write()
+                grown[st.row] = (st, len(st.pages) * self.page_size)
+                pages.extend(self._take_pages(st, need))
+            st.capacity = min(len(st.pages) * self.page_size, self.max_seq_len)
+            st.last_used = next(self._clock)
+        write()
 
     def free(self, seq_id: int) -> None:
         st = self._seqs.pop(seq_id, None)

@@ -242,6 +242,18 @@ def test_verify_chains_kernel(clean, lens, V, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("lens,shift", [([0, 1, 2, 3, 4, 5, 8, 9, 10, 12, 17, 30, 40], 0.05), ([1] * 100 + [0, 2], 0.75)])
+def test_verify_chains_kernel_of_many_rows(clean, lens, shift):
+    """Enough rows that they are read in several launches: chains that are kept for long, and launches without anything to read."""
+    c = chains(1, lens, 151936, shift=shift)
+    dev = {k: v.cuda() for k, v in c.items()}
+    want = ref.verify_chains(**c)
+    for _ in range(3):
+        got = ops.verify_chains(**dev)
+        assert got[0].tolist() == want[0].tolist() and got[1].tolist() == want[1].tolist()
+
+
+@gpu
 def test_verify_chains_kernel_masked_and_strided(clean):
     """Vocabularies cut down to a few tokens (-inf elsewhere), empty rows, views of wider matrices, rows off 16-byte boundaries, drafts
     with the same token again, numbers at the ends of [0, 1)."""
@@ -406,3 +418,264 @@ def test_shared_prefix_attention_kernel(clean, heads, kv, prefix, behind, counts
     got = attend(c, max_q=max(1, max(counts)))
     attention_close(got, want)
     attention_close(attend(c), want)      # without a bound on the rows
+
+
+def test_shared_prefix_attention_refusals():
+    from jetspec_b200.ops import cuda_ext
+    c = attention_case(0, 4, 2, 20, [0, 5], [4, 3], False)
+    call = lambda **kw: cuda_ext.shared_prefix_attention(**{**c, "max_q": 4, **kw})
+    kernel_refuses(lambda: call(q=c["q"].float()), "q ")
+    kernel_refuses(lambda: call(q=c["q"][..., :64]), "q ")
+    kernel_refuses(lambda: call(k_pool=c["k_pool"][:, ::2]), "pools")
+    kernel_refuses(lambda: call(v_pool=c["v_pool"].half()), "pools")
+    kernel_refuses(lambda: call(q=c["q"][:, :3]), "heads")
+    kernel_refuses(lambda: call(slot_map=c["slot_map"].long()), "slot_map")
+    kernel_refuses(lambda: call(cu_q=c["cu_q"][:2]), "cu_q")
+    kernel_refuses(lambda: call(mask_bits=None), "mask_bits")
+    kernel_refuses(lambda: call(mask_bits=c["mask_bits"][:-1]), "mask_bits")
+    kernel_refuses(lambda: call(prefix_len=-1), "prefix_len")
+    kernel_refuses(lambda: call(prefix_len=c["slot_map"].shape[1] + 1), "prefix_len")
+    kernel_refuses(lambda: call(max_q=-1), "max_q")
+    kernel_refuses(lambda: call(scale=math.nan), "scale")
+    kernel_refuses(lambda: call(out=torch.empty(7, 512)), "out")
+
+
+@gpu
+def test_shared_prefix_attention_of_odd_calls(clean):
+    """A view of joint projections as queries, nothing to do, sequences without rows, a bound that is too low, slots that do not exist."""
+    c = attention_case(1, 16, 4, 90, [0, 33, 7], [5, 0, 3], False, device="cuda")
+    want = attention_exact(c)
+    wide = torch.full((8, 24, 128), math.nan, dtype=torch.bfloat16, device="cuda")
+    wide[:, :16] = c["q"]
+    attention_close(attend({**c, "q": wide[:, :16]}), want)
+    attention_close(attend({**c, "q": c["q"].transpose(0, 1).contiguous().transpose(0, 1)}), want)
+    none = {k: c[k][:0] for k in ("q", "mask_bits", "seq_rows", "past_lens")}
+    assert attend({**c, **none, "cu_q": i32(0, device="cuda")}).shape == (0, 16 * 128)
+    assert not attend({**c, "cu_q": i32(0, 0, 0, 0, device="cuda")}, max_q=0).any()
+    assert not attend({**c, "seq_rows": c["seq_rows"][:0], "past_lens": c["past_lens"][:0], "cu_q": i32(0, device="cuda")}).any()
+    attend(c, max_q=4)
+    with pytest.raises(RuntimeError, match="more new rows"):
+        clean.check_status("cuda")
+    for slot in (-1, c["k_pool"].shape[1]):
+        m = c["slot_map"].clone()
+        m[3, 95] = slot          # row 2 is the sequence without rows: nobody reads it
+        attend({**c, "slot_map": m})
+        with pytest.raises(RuntimeError, match="slot"):
+            clean.check_status("cuda")
+
+
+# ------------------------------------------------------------------ the three in a row
+class Step:
+    """Pages, rows and slots of a batch behind a shared prompt; its attention; what of its drafts the target keeps."""
+
+    def __init__(self, device, prompt=37, lens=(5, 1, 8, 3), heads=8, kv=2, V=1009, dim=128):
+        g = torch.Generator().manual_seed(11)
+        B, T, page = len(lens), sum(lens), 16
+        pages, shared = 12 * B, prompt // page * page
+        put = lambda *s, dtype=torch.bfloat16: torch.randn(*s, generator=g).to(dtype).to(device)
+        self.page, self.T, self.prefix = page, T, shared
+        self.slot_map = torch.zeros(B + 1, 128, dtype=I32)
+        self.slot_map[:, :shared] = torch.arange(shared, dtype=I32).flip(0)
+        self.slot_map = self.slot_map.to(device)
+        self.past, self.counts = (torch.tensor(v, dtype=I32, device=device) for v in ([prompt + 16 * b for b in range(B)], lens))
+        self.mapped = torch.full((B,), shared, dtype=I32, device=device)
+        self.rows = torch.arange(B, 0, -1, device=device).to(I32)
+        self.free = (shared // page + torch.randperm(pages, generator=g)).to(I32).to(device)
+        S = shared + pages * page
+        self.k, self.v, self.q, self.knew, self.vnew = put(kv, S, dim), put(kv, S, dim), put(T, heads, dim), put(T, kv, dim), put(T, kv, dim)
+        self.head = put(V, heads * dim, dtype=torch.float32) * 0.05
+        self.draft = put(T - B, V, dtype=torch.float32)
+        self.drafts = self.draft.argmax(-1).to(I32)
+        self.cu_drafts = torch.tensor([0] + torch.tensor([n - 1 for n in lens]).cumsum(0).tolist(), dtype=I32, device=device)
+        self.accept_u, self.sample_u = (torch.rand(n, generator=g).to(device) * 0.3 for n in (T - B, B))
+
+    def __call__(self, o=ops):
+        cu, positions, slots, cu_pages = o.plan_slots(self.past, self.counts, self.rows, self.free, self.page, self.slot_map, self.T,
+                                                      mapped_lens=self.mapped)
+        self.k[:, slots.long()], self.v[:, slots.long()] = self.knew.transpose(0, 1), self.vnew.transpose(0, 1)
+        a = o.shared_prefix_attention(self.q, self.k, self.v, self.slot_map, self.rows, cu, self.past, None, 128 ** -0.5, self.prefix, causal=True)
+        logits = a.float() @ self.head.t()
+        accepted, token = o.verify_chains(logits, self.draft, self.drafts, self.cu_drafts, self.accept_u, self.sample_u, temperature=0.8)
+        return cu, positions, slots, cu_pages, a, logits, accepted, token
+
+
+def test_a_serving_step_by_hand():
+    s = Step("cpu")
+    cu, positions, slots, cu_pages, a, logits, accepted, token = s()
+    assert cu.tolist() == [0, 5, 6, 14, 17] and cu_pages.tolist() == [0, 1, 3, 6, 10]
+    assert positions.tolist() == [37 + i for i in range(5)] + [53] + [69 + i for i in range(8)] + [85 + i for i in range(3)]
+    assert slots.unique().numel() == 17 and torch.equal(slots[:5], s.slot_map[4, 37:42])
+    c = dict(q=s.q, k_pool=s.k, v_pool=s.v, slot_map=s.slot_map, seq_rows=s.rows, cu_q=cu, past_lens=s.past, mask_bits=None, scale=128 ** -0.5,
+             causal=True)
+    attention_close(a, attention_exact(c))
+    assert bool((accepted >= 0).all()) and bool((accepted < s.counts).all()) and bool((token >= 0).all())
+
+
+def same_step(got, want, exact):
+    """Integers are equal; ``exact`` is the attention in 64 bits; verification is compared on the same logits."""
+    for g, w in zip(got[:4], want[:4]):
+        assert g.tolist() == w.tolist()
+    attention_close(got[4].cpu(), exact)
+
+
+@gpu
+def test_a_serving_step_with_kernels(clean):
+    """Eager, on another stream, and captured: a replay sees what its inputs hold then, and two graphs of one step do not disturb each
+    other."""
+    cpu, dev = Step("cpu"), Step("cuda")
+    want = cpu(ref)
+
+    def exact(s, cu):
+        return attention_exact(dict(q=s.q, k_pool=s.k, v_pool=s.v, slot_map=s.slot_map, seq_rows=s.rows, cu_q=cu, past_lens=s.past, mask_bits=None,
+                                    scale=128 ** -0.5, causal=True))
+
+    def check(got, s, want, full):
+        same_step(got, want, full)
+        again = ref.verify_chains(got[5].cpu(), s.draft.cpu(), s.drafts.cpu(), s.cu_drafts.cpu(), s.accept_u.cpu(), s.sample_u.cpu(), temperature=0.8)
+        assert got[6].tolist() == again[0].tolist() and got[7].tolist() == again[1].tolist()
+
+    full = exact(cpu, want[0])
+    check(dev(), dev, want, full)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = dev()
+        got2 = dev()
+    side.synchronize()
+    check(got, dev, want, full)
+    check(got2, dev, want, full)
+
+    others = [Step("cuda"), Step("cuda")]
+    graphs, outs = [], []
+    for s in others:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=side):
+            outs.append(s())
+    for turn in range(3):
+        cpu.counts[:] = torch.tensor([(5, 1, 8, 3), (1, 8, 3, 5), (3, 3, 8, 3)][turn])
+        cpu.cu_drafts[1:] = (cpu.counts - 1).cumsum(0)
+        cpu.q += 0.25
+        for s in others:
+            s.counts.copy_(cpu.counts)
+            s.cu_drafts.copy_(cpu.cu_drafts)
+            s.q.copy_(cpu.q)
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        want = cpu(ref)
+        full = exact(cpu, want[0])
+        for s, got in zip(others, outs):
+            check(got, s, want, full)
+
+
+# ------------------------------------------------------------------ in the framework's own paths
+def pool_of(device, **kw):
+    from jetspec_b200.runtime.kv_pool import PagedKVPool
+    return PagedKVPool(1, 1, 8, 10, page_size=4, max_seqs=4, max_seq_len=18, device=device, **kw)
+
+
+def grow_pools(device):
+    from jetspec_b200.runtime.kv_pool import EvictionRequired
+    one, many = pool_of(device), pool_of(device)
+    asks = [([7, 3, 9], [5, 0, 4]), ([3, 7], [18, 6]), ([7, 7, 9], [9, 13, 4]), ([9], [8]), ([3, 7, 9], [18, 18, 9])]
+    for seqs, tokens in asks:
+        failed = []
+        try:
+            for s, n in zip(seqs, tokens):
+                one.reserve(s, n)
+        except EvictionRequired as e:
+            failed.append(str(e))
+        try:
+            many.reserve_batch(seqs, tokens)
+        except EvictionRequired as e:
+            failed.append(str(e))
+        assert len(failed) in (0, 2) and len(set(failed)) <= 1
+        assert torch.equal(one.slot_map, many.slot_map)
+        for s in seqs:
+            a, b = one.state(s), many.state(s)
+            assert (a.row, a.pages, a.capacity) == (b.row, b.pages, b.capacity)
+    assert failed and one._refcount == many._refcount and list(one._free_pages) == list(many._free_pages)
+    with pytest.raises(EvictionRequired):
+        many.reserve_batch([3], [19])
+    return many
+
+
+def causal_rows(pool):
+    from jetspec_b200.runtime.attn_metadata import build_attn_metadata
+    past, counts = [17, 2, 5], [1, 4, 3]
+    m = build_attn_metadata(pool, [3, 9, 7], past, num_query_nodes=counts)
+    assert m.cu_q.tolist() == [0, 1, 5, 8] and m.past_lens.tolist() == past and m.seq_rows.tolist() == [pool.state(s).row for s in (3, 9, 7)]
+    assert m.positions.tolist() == [17, 2, 3, 4, 5, 5, 6, 7] and (m.max_q, m.num_tokens, m.counts) == (4, 8, counts)
+    rows = [pool.slot_map[pool.state(s).row, p:p + n] for s, p, n in zip((3, 9, 7), past, counts)]
+    assert torch.equal(m.slots, torch.cat(rows)) and m.causal and m.mask_bits is None
+    assert {t.dtype for t in (m.cu_q, m.past_lens, m.seq_rows, m.positions, m.slots)} == {I32}
+
+
+def test_pools_and_batches_plan_their_slots():
+    causal_rows(grow_pools("cpu"))
+
+
+@gpu
+def test_pools_and_batches_plan_their_slots_on_the_gpu(clean):
+    causal_rows(grow_pools("cuda"))
+
+
+class Sampler:
+    """Draws from the target's logits plus ``noise``."""
+
+    def __init__(self, runner, noise):
+        self.runner, self.noise = runner, noise
+
+    def propose_sampled(self, context_ids, k, temperature, target_hidden=None):
+        ids, rows = context_ids, []
+        for _ in range(k):
+            rows.append(self.runner.forward(ids, self.runner.new_cache(64), last_position_logits_only=True)[0][0, -1] + self.noise)
+            ids = torch.cat((ids, ops.sample(rows[-1], temperature).view(1, 1)), 1)
+        return ids[0, -k:], torch.stack(rows)
+
+
+def chains_of_a_model(device, monkeypatch):
+    from jetspec_b200 import LLM, SamplingParams
+    from jetspec_b200.models import Qwen3ForCausalLM, tiny_config
+    llm = LLM(Qwen3ForCausalLM.random_init(tiny_config(), seed=0, dtype=torch.float32), device=device, dtype=torch.float32)
+    prompt = torch.randint(0, 1024, (1, 9), generator=torch.Generator().manual_seed(0))
+    noise = torch.randn(1024, generator=torch.Generator().manual_seed(1)).to(device)
+    torch.manual_seed(0)
+    calls = []
+    monkeypatch.setattr(ops, "verify_chains", lambda *a, _f=ops.verify_chains, **kw: calls.append(kw) or _f(*a, **kw))
+    run = lambda shift, t, n: llm.generate_chain(prompt, Sampler(llm.runner, noise * shift), block_size=4, sampling_params=SamplingParams(t, n))
+    same = run(0.0, 0.9, 13)                 # drafts from the target's own probabilities are kept, but for rounding
+    assert len(same["token_ids"]) == 13 and calls == [dict(temperature=0.9)] * 3
+    assert len(run(1.0, 0.9, 10)["token_ids"]) == 10
+    # a temperature that counts as none: the target's most likely tokens, whatever was drafted
+    want = llm.generate(prompt, SamplingParams(0.0, 12))["token_ids"]
+    assert run(3.0, 1e-6, 12)["token_ids"] == want
+
+
+def test_generate_chain_with_a_sampling_head():
+    from jetspec_b200 import LLM, SamplingHeadDrafter, SamplingParams
+    from jetspec_b200.models import DraftHeadModel, Qwen3ForCausalLM, draft_head_config, tiny_config
+    model = Qwen3ForCausalLM.random_init(tiny_config(), seed=0, dtype=torch.float32)
+    head = DraftHeadModel.random_init(draft_head_config(model.config, num_layers=1, block_size=4, num_taps=2), seed=5, dtype=torch.float32)
+    drafter = SamplingHeadDrafter(head, model, block_size=4, target_layer_ids=[0, 1])
+    llm, prompt = LLM(model, device="cpu", dtype=torch.float32), torch.arange(1, 10).view(1, -1)
+    run = lambda t, n: llm.generate_chain(prompt, drafter, block_size=4, target_layer_ids=drafter.target_layer_ids,
+                                          sampling_params=SamplingParams(t, n))["token_ids"]
+    torch.manual_seed(0)
+    assert len(run(1.0, 11)) == 11
+    greedy = llm.generate(prompt, SamplingParams(0.0, 11))["token_ids"]
+    assert run(1e-6, 11) == greedy and run(0.0, 11) == greedy
+
+
+def test_generate_chain_verifies_draws(monkeypatch):
+    chains_of_a_model("cpu", monkeypatch)
+
+
+@gpu
+def test_generate_chain_verifies_draws_on_the_gpu(clean, monkeypatch):
+    chains_of_a_model("cuda", monkeypatch)
+
+
