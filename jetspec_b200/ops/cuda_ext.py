@@ -1579,14 +1579,16 @@ def plan_slots(past_lens, counts, seq_rows, free_pages, page_size: int, slot_map
         _refuse("past_lens, counts, seq_rows and mapped_lens differ in length")
     if B > 65535 or page_size < 1 or rows < 0:
         _refuse(f"plan_slots(B={B}, page_size={page_size}, rows={rows})")
-    buf = slot_map.new_empty(2 * (B + 1) + 2 * rows)
+    whole = rows + 3 & ~3              # results start on 16-byte boundaries
+    buf = slot_map.new_empty(2 * whole + 2 * (B + 1))
     at = buf.data_ptr()
-    cu_q, cu_pages, positions, slots = buf.split_with_sizes((B + 1, B + 1, rows, rows))
-    # blocks a request: enough to fill the SMs, a couple of thousand positions each
-    chunks = max(1, min(4 * SM_COUNT // max(1, B), max_len // 2048))
+    positions, _, slots, _, cu_q, cu_pages = buf.split_with_sizes((rows, whole - rows, rows, whole - rows, B + 1, B + 1))
+    # Blocks a request: 4096 positions each, as every block sums the requests before it anew (128 requests: 4.1 us, with 1024 positions 6.1),
+    # and no more blocks than the SMs hold at once (8 of 256 threads; 256 prompts: 14 us, with 4 14.9, with 32 22).
+    chunks = max(1, min(8 * SM_COUNT // max(1, B), max_len // 4096))
     rc = _entry("js_slot_plan", "pppppppppppiiiiiiip")(
         past_lens.data_ptr(), counts.data_ptr(), mapped.data_ptr(), seq_rows.data_ptr(), free_pages.data_ptr(), slot_map.data_ptr(),
-        at, at + 4 * (B + 1), at + 8 * (B + 1), at + 8 * (B + 1) + 4 * rows, _status_at(index), B, free_pages.numel(), page_size,
+        at + 8 * whole, at + 8 * whole + 4 * (B + 1), at, at + 4 * whole, _status_at(index), B, free_pages.numel(), page_size,
         max_seqs, max_len, rows, chunks, _stream_at(index))
     if rc:
         _check(rc, "js_slot_plan")
