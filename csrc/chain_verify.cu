@@ -298,21 +298,23 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
     if (rank == 0 && tid == 0) p.token[b] = t_at < p.V ? t_at : -1;
     return;
   }
+  // The draft's share of a weight: none behind the last draft and beside a row without a logit above -inf; a point mass takes all of its index
+  // (p <= 1) and nothing elsewhere.
+  const bool point = left && td < kGreedyBelow, both = left && !point && dstat.x != -INFINITY;
+  const int skip = point ? d_at : -1;
   const double ts = kExpTable * 1.4426950408889634 / tt, ds = kExpTable * 1.4426950408889634 / td;
-  const double tc = -tstat.x * ts, dc = -dstat.x * ds;
-  // logits below these have a probability under 2^-1000: none
-  const float t_least = static_cast<float>((-1000.0 * kExpTable - tc) / ts), d_least = static_cast<float>((-1000.0 * kExpTable - dc) / ds);
-  const bool draft_point = td < kGreedyBelow;
-  auto ep = [&](float v) { return v > t_least ? exp2_table(fma(static_cast<double>(v), ts, tc), table) : 0.0; };
-  auto eq = [&](float v, int i) {
-    if (draft_point) return i == d_at ? 1.0 : 0.0;
-    return v > d_least ? exp2_table(fma(static_cast<double>(v), ds, dc), table) : 0.0;
-  };
+  double tc = -tstat.x * ts, dc = both ? -dstat.x * ds : 0.0;
+  // logits below these have a probability under 2^-1000; they are cut there, and sums too small for any other count as zero
+  const float t_least = fmaxf(static_cast<float>((-1000.0 * kExpTable - tc) / ts), -3.4e38f);
+  const float d_least = fmaxf(static_cast<float>((-1000.0 * kExpTable - dc) / ds), -3.4e38f);
+  auto ep = [&](float v) { return exp2_table(fma(static_cast<double>(fmaxf(v, t_least)), ts, tc), table); };
+  auto eq = [&](float v) { return exp2_table(fma(static_cast<double>(fmaxf(v, d_least)), ds, dc), table); };
   // A CTA takes a slice of the vocabulary and a warp a slice of that, so sums follow the order of the indices.
   const int lo = static_cast<long long>(p.V) * rank / CLUSTER, size = static_cast<int>(static_cast<long long>(p.V) * (rank + 1) / CLUSTER) - lo;
   auto warp_lo = [&](int w) { return lo + static_cast<int>(static_cast<long long>(size) * w / kWarps); };
   // f(index, target logit, draft logit) for this warp's elements; four at a time, as fp64 chains are long
-  auto each = [&](auto f) {
+  auto each = [&](auto two, auto f) {
+    constexpr bool kTwo = decltype(two)::value;
     const int end = warp_lo(warp + 1);
     int i = warp_lo(warp) + lane;
     for (; i + 96 < end; i += 128) {
@@ -320,18 +322,18 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         v[j] = chain_f(x[i + 32 * j]);
-        w[j] = left ? chain_f(y[i + 32 * j]) : 0.f;
+        w[j] = kTwo ? chain_f(y[i + 32 * j]) : 0.f;
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) f(i + 32 * j, v[j], w[j]);
     }
-    for (; i < end; i += 32) f(i, chain_f(x[i]), left ? chain_f(y[i]) : 0.f);
+    for (; i < end; i += 32) f(i, chain_f(x[i]), kTwo ? chain_f(y[i]) : 0.f);
   };
   // the warps' sums into `to`; their sum in order
   auto block_sum = [&](double v, double* to) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (lane == 0) to[warp] = v;
+    if (lane == 0) to[warp] = v > 1e-290 ? v : 0.0;      // (2^-963)
     __syncthreads();
     v = 0.0;
     for (int w = 0; w < kWarps; ++w) v += to[w];
@@ -348,12 +350,12 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
     __syncwarp();
     cluster_sync();
   };
-  double ip = 1.0, iq = 0.0;
-  if (left) {
+  double sum = 0.0;
+  if (both) {
     double sp = 0.0, sq = 0.0;
-    each([&](int i, float v, float w) {
+    each(std::true_type{}, [&](int, float v, float w) {
       sp += ep(v);
-      sq += eq(w, i);
+      sq += eq(w);
     });
     sp = block_sum(sp, part);
     sq = block_sum(sq, part2);
@@ -363,15 +365,17 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
       sp += sums[c][0];
       sq += sums[c][1];
     }
-    ip = 1.0 / sp;
-    iq = sq > 0.0 ? 1.0 / sq : 0.0;
+    tc -= kExpTable * log2(sp);           // probabilities from here on
+    dc -= kExpTable * log2(sq);
+    each(std::true_type{}, [&](int, float v, float w) { sum += fmax(ep(v) - eq(w), 0.0); });
+  } else {
+    each(std::false_type{}, [&](int i, float v, float) { sum += i != skip ? ep(v) : 0.0; });
   }
-  auto weight = [&](int i, float v, float w) {
-    const double r = left ? ep(v) * ip - eq(w, i) * iq : ep(v);
-    return r > 0.0 ? r : 0.0;
+  auto weight = [&](int i) {
+    const float v = chain_f(x[i]);
+    if (!(v > t_least) || i == skip) return 0.0;
+    return both ? fmax(ep(v) - eq(chain_f(y[i])), 0.0) : ep(v);
   };
-  double sum = 0.0;
-  each([&](int i, float v, float w) { sum += weight(i, v, w); });
   sum = block_sum(sum, part);
   exchange(sum, 0.0);
   double total = 0.0;
@@ -407,9 +411,8 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
   // the warp's slice once more, a few neighbouring elements a thread
   const int from = warp_lo(w), to = warp_lo(w + 1), per = (to - from + kChainThreads - 1) / kChainThreads;
   const int mine = min(to, from + tid * per), stop = min(to, mine + per);
-  auto at = [&](int i) { return weight(i, chain_f(x[i]), left ? chain_f(y[i]) : 0.f); };
   sum = 0.0;
-  for (int i = mine; i < stop; ++i) sum += at(i);
+  for (int i = mine; i < stop; ++i) sum += weight(i);
   double inc = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -428,7 +431,7 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
   __syncthreads();
   if (tid == (passing != 0x7fffffff ? passing : holding)) {
     ahead += inc - sum;
-    p.token[b] = mine + find(stop - mine, [&](int c) { return at(mine + c); }, ahead);
+    p.token[b] = mine + find(stop - mine, [&](int c) { return weight(mine + c); }, ahead);
   }
 }
 
