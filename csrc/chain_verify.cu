@@ -17,8 +17,13 @@
 
 namespace js {
 
-constexpr int kStatThreads = 256, kStatBlocks = 4;      // a block of the first kernel reads 4 x 16 bytes a thread of either row at once: 16 KB each
-constexpr int kChunkBytes = kStatThreads * kStatBlocks * 16;
+// A block of the first kernel reads 16 KB of either row at once.  fp32: 128 threads, six blocks an SM (64 sequences 192 us, 208 with four of 256
+// threads); bf16 has twice the values, that want the registers of 256 threads (16 sequences 61 us, 81 with 128).
+constexpr int kChunkBytes = 16384;
+template <typename T>
+struct StatShape { static constexpr int kThreads = 256, kResident = 4; };
+template <>
+struct StatShape<float> { static constexpr int kThreads = 128, kResident = 6; };
 constexpr int kChainThreads = 512;
 constexpr float kGreedyBelow = 1e-5f;
 constexpr int kNoneRejected = 0x7fffffff;
@@ -116,8 +121,8 @@ JS_DEVICE float warp_max_f32(float v) {
 }
 // One chunk of the rows of drafts lo + z, lo + z + Z, ... below hi of a sequence: block (chunk, sequence, z).
 template <typename T>
-__global__ void __launch_bounds__(kStatThreads, 4) chain_stats_kernel(ChainParams p, int lo, int hi) {
-  constexpr int N = 16 / sizeof(T), kWarps = kStatThreads / 32;
+__global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResident) chain_stats_kernel(ChainParams p, int lo, int hi) {
+  constexpr int N = 16 / sizeof(T), kStatThreads = StatShape<T>::kThreads, kStatBlocks = kChunkBytes / 16 / kStatThreads, kWarps = kStatThreads / 32;
   __shared__ float tops[2][kWarps], sums[2][kWarps];
   __shared__ int where[2], go;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, chunk = blockIdx.x, b = blockIdx.y;
@@ -465,7 +470,7 @@ static int launch_token(const ChainParams& p, cudaStream_t stream) {
 template <typename T>
 static int launch_chain(const ChainParams& p, cudaStream_t stream) {
   cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(kStatThreads);
+  cfg.blockDim = dim3(StatShape<T>::kThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
