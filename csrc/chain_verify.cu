@@ -493,8 +493,11 @@ static int launch_chain(const ChainParams& p, cudaStream_t stream) {
       if (!launch(lo, hi, hi - lo)) return -4;
     if (!launch(9, all, 4)) return -4;
   }
-  // few sequences: more SMs each (16 is more than a portable cluster has)
-  return p.B * 16 <= 144 ? launch_token<T, 16>(p, stream) : launch_token<T, 8>(p, stream);
+  // As many CTAs a sequence as are there at once, two an SM (16 is more than a portable cluster has): 16 sequences 56 us with 16, 61 with 8, 68 with
+  // 4; 64 sequences 184 us with 4, 193 with 8, 214 with 2.
+  constexpr int kAtOnce = 2 * 148;
+  if (p.B * 16 <= kAtOnce) return launch_token<T, 16>(p, stream);
+  return p.B * 8 <= kAtOnce ? launch_token<T, 8>(p, stream) : launch_token<T, 4>(p, stream);
 }
 
 }  // namespace js
