@@ -41,7 +41,7 @@ struct SharedAttn {
   __nv_bfloat16* out;          // (T, Hq * 128)
   int* plan;                   // length of a piece of the line; where every item begins on it
   uint8_t* parted;             // (tile of the sequences' rows, head): its output is in parts (without a prefix)
-  float *po, *so;              // partial outputs of prefix and sequence segments: (segment, side, row, 128)
+  float *po, *so;              // partial outputs of prefix and sequence segments: (segment, side, 16, row, 8), as a row a thread writes them
   float2 *pml, *sml;           // their (maximum, sum): (segment, side, row)
   int* status;
   long long ldq;
@@ -173,6 +173,12 @@ JS_DEVICE void sa_tmem_st16(uint32_t taddr, const uint32_t* r) {
       "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
       ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]) : "memory");
+}
+// 32 bytes, a whole sector of the L2 cache, in one store
+JS_DEVICE void sa_store32(void* to, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]),
+               "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 JS_DEVICE void sa_tmem_ld16(uint32_t taddr, uint32_t* r) {
   asm volatile(
@@ -673,7 +679,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const size_t at = (seg * 2 + rel) * rows + row;
       const bool keep = valid && !direct && row < rows;
       __nv_bfloat16* out = direct ? p.out + (static_cast<size_t>(w.s.q_begin + node) * p.Hq + head) * SD : nullptr;
-      float* part = (prefix ? p.po : p.so) + at * SD;
+      float* part = (prefix ? p.po : p.so) + ((seg * 2 + rel) * rows * SD + row * 8);
       if (keep) (prefix ? p.pml : p.sml)[at] = make_float2(m_run, l_run);
       else if (valid && !direct) report(p.status, kRowsOverflow);      // more rows in a sequence than the caller's bound
       if (p.prefix == 0 && (warp & 3) == 0 && lane == 0 && (w.two || rel == 0))
@@ -692,21 +698,19 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
           tmem_ld_32x32(to + c + 32, o + 32);
           tmem_ld_wait();
           if (direct && valid) {
-            uint4* dst = reinterpret_cast<uint4*>(out + c);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              uint4 pk;
-              __nv_bfloat162* o2 = reinterpret_cast<__nv_bfloat162*>(&pk);
+            for (int j = 0; j < 64; j += 16) {
+              uint32_t pk[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                o2[e] = __floats2bfloat162_rn(__uint_as_float(o[8 * j + 2 * e]) * inv, __uint_as_float(o[8 * j + 2 * e + 1]) * inv);
-              dst[j] = pk;
+              for (int e = 0; e < 8; ++e) {
+                const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(o[j + 2 * e]) * inv, __uint_as_float(o[j + 2 * e + 1]) * inv);
+                pk[e] = *reinterpret_cast<const uint32_t*>(&v);
+              }
+              sa_store32(out + c + j, pk);
             }
           } else if (keep) {
-            float4* dst = reinterpret_cast<float4*>(part + c);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              dst[j] = make_float4(__uint_as_float(o[4 * j]), __uint_as_float(o[4 * j + 1]), __uint_as_float(o[4 * j + 2]), __uint_as_float(o[4 * j + 3]));
+            for (int j = 0; j < 64; j += 8) sa_store32(part + static_cast<size_t>(c + j) * rows, o + j);
           }
         }
       }
@@ -796,12 +800,12 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
       } else if (k < shared_parts) {
         const size_t r = (static_cast<size_t>(pc0 + (p_two ? k : k >> 1) + p_item) * 2 + (p_two ? 0 : k & 1)) * SROWS + p_row;
         ml = p.pml[r];
-        at = p.po + r * SD;
+        at = p.po + ((r - p_row % SROWS) * SD + p_row % SROWS * 8);
       } else if (k < parts && row < p.seq_rows_kept) {
         const int j = k - shared_parts;
         const size_t r = (static_cast<size_t>(c0 + (two ? j : j >> 1) + item) * 2 + (two ? tile & 1 : j & 1)) * p.seq_rows_kept + row;
         ml = p.sml[r];
-        at = p.so + r * SD;
+        at = p.so + ((r - row) * SD + row * 8);
       }
       if (ml.y == 0.f) ml.x = -INFINITY;       // no visible key: the part's output may be unwritten
       const float m_new = fmaxf(m, warp_max(ml.x)), safe = m_new == -INFINITY ? 0.f : m_new;      // NaN scores leave a sum without a maximum
@@ -816,7 +820,8 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
         const float f = __shfl_sync(0xffffffffu, add, j);
         const unsigned long long from = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), j);
         const bool use = __shfl_sync(0xffffffffu, ml.y, j) != 0.f;
-        const float4 x = use ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const int stride = 8 * (base + j < shared_parts ? SROWS : p.seq_rows_kept);      // two lanes a stretch of eight columns
+        const float4 x = use ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + (lane >> 1) * stride + (lane & 1) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
         acc[0] = fmaf(x.x, f, acc[0]);
         acc[1] = fmaf(x.y, f, acc[1]);
         acc[2] = fmaf(x.z, f, acc[2]);

@@ -1540,14 +1540,14 @@ def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_le
         q = q.contiguous()
     if out is None:
         out = torch.empty(T, Hq * 128, dtype=bf16, device=q.device)
-    elif out.shape != (T, Hq * 128) or out.dtype is not bf16 or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 16:
+    elif out.shape != (T, Hq * 128) or out.dtype is not bf16 or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 32:
         _refuse("out: expected a contiguous (T, Hq * 128) bf16 tensor on the queries' device")
     if T == 0 or B == 0:
         return out.zero_()
     need = shared_prefix_workspace(B, T, Hq, Hkv, max_len, prefix_len, max_q)
     if ws is None:
         ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif ws.dtype is not torch.uint8 or not ws.is_contiguous() or ws.get_device() != index or ws.numel() < need or ws.data_ptr() % 16:
+    elif ws.dtype is not torch.uint8 or not ws.is_contiguous() or ws.get_device() != index or ws.numel() < need or ws.data_ptr() % 32:
         _refuse(f"ws: expected {need} contiguous bytes on the queries' device")
     rc = _entry("js_shared_attention", "plppppppppplpiiiiiiiiifiiip")(
         q.data_ptr(), q.stride(0), k_pool.data_ptr(), v_pool.data_ptr(), slot_map.data_ptr(), seq_rows.data_ptr(), cu_q.data_ptr(),
