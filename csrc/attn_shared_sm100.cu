@@ -725,7 +725,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   }
 }
 
-// Joins the parts of the rows of a tile: a block takes up to kMergeRows rows of one head, a warp a row at a time, four columns a lane.
+// Joins the parts of the rows of a tile: a block takes up to kMergeRows rows of one head.
 constexpr int kMergeRows = 32, kMergeWarps = 8;
 __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(const SharedAttn p) {
   // Until the wait below only the call's inputs are read: the kernel before, which is launched without overlap, began when they were there.
@@ -772,67 +772,69 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
   const SaSeq all = p.prefix > 0 ? sa_seq(p, -1) : s;
   const int all_units = p.prefix > 0 ? sa_units(p, all, -1, 0) : 0;
   const int own_parts = two ? own : 2 * own;
-  for (int row = row0 + warp; row < min(rows, row0 + kMergeRows); row += kMergeWarps) {
-    const int tok = row / p.G, t = s.q_begin + node0 + tok, head = h * p.G + row - tok * p.G;
-    int pc0 = 0, shared_parts = 0, p_item = 0, p_row = 0, p_begin = 0;
-    bool p_two = false;
-    if (all_units > 0) {
-      const int p_tile = t / p.npt, p_pair = p_tile >> 1;
-      p_item = sa_item(p, all, -1, p_pair, h);
-      p_two = sa_weight(p, all, p_pair) == 2;
-      p_begin = p_pair * p.Hkv * sa_length(p, all, -1, 0) + h * sa_length(p, all, -1, p_pair);
-      pc0 = (p_begin + kItemCost) / piece;
-      shared_parts = ((p_begin + kItemCost + ((all_units - 1) << p_two)) / piece - pc0 + 1) * (p_two ? 1 : 2);
-      p_row = (t - p_tile * p.npt) * p.G + row - tok * p.G + (p_two ? (p_tile & 1) * SROWS : 0);
-    }
-    const int parts = shared_parts + own_parts;
-    float m = -INFINITY, l = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int base = 0; base < parts; base += 32) {
-      // a part a lane: where it lies, its maximum and sum
-      const int k = base + lane;
-      const float* at = nullptr;
-      float2 ml = make_float2(-INFINITY, 0.f);
-      // a cut piece may hold no unit's beginning, and then no part
-      const int c = k < shared_parts ? pc0 + (p_two ? k : k >> 1) : c0 + (two ? k - shared_parts : (k - shared_parts) >> 1);
-      const int begin = k < shared_parts ? p_begin : own_begin;
-      const bool pair_of = k < shared_parts ? p_two : two;
-      if (k >= parts || sa_unit(c * piece - begin, pair_of) == sa_unit((c + 1) * piece - begin, pair_of)) {
-      } else if (k < shared_parts) {
-        const size_t r = (static_cast<size_t>(pc0 + (p_two ? k : k >> 1) + p_item) * 2 + (p_two ? 0 : k & 1)) * SROWS + p_row;
-        ml = p.pml[r];
-        at = p.po + ((r - p_row % SROWS) * SD + p_row % SROWS * 8);
-      } else if (k < parts && row < p.seq_rows_kept) {
-        const int j = k - shared_parts;
-        const size_t r = (static_cast<size_t>(c0 + (two ? j : j >> 1) + item) * 2 + (two ? tile & 1 : j & 1)) * p.seq_rows_kept + row;
-        ml = p.sml[r];
-        at = p.so + ((r - row) * SD + row * 8);
-      }
-      if (ml.y == 0.f) ml.x = -INFINITY;       // no visible key: the part's output may be unwritten
-      const float m_new = fmaxf(m, warp_max(ml.x)), safe = m_new == -INFINITY ? 0.f : m_new;      // NaN scores leave a sum without a maximum
-      const float old = exp2f(m - safe), add = ml.y == 0.f ? 0.f : exp2f(ml.x - safe);
-      m = m_new;
-      l = l * old + warp_sum(ml.y * add);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] *= old;
-      const int here = min(32, parts - base);
-#pragma unroll 4
-      for (int j = 0; j < here; ++j) {
-        const float f = __shfl_sync(0xffffffffu, add, j);
-        const unsigned long long from = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(at), j);
-        const bool use = __shfl_sync(0xffffffffu, ml.y, j) != 0.f;
-        const int stride = 8 * (base + j < shared_parts ? SROWS : p.seq_rows_kept);      // two lanes a stretch of eight columns
-        const float4 x = use ? *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(from) + (lane >> 1) * stride + (lane & 1) * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-        acc[0] = fmaf(x.x, f, acc[0]);
-        acc[1] = fmaf(x.y, f, acc[1]);
-        acc[2] = fmaf(x.z, f, acc[2]);
-        acc[3] = fmaf(x.w, f, acc[3]);
-      }
-    }
-    const float inv = l > 0.f ? 1.f / l : 0.f;
-    __nv_bfloat16* out = p.out + (static_cast<size_t>(t) * p.Hq + head) * SD + lane * 4;
-    *reinterpret_cast<__nv_bfloat162*>(out) = __floats2bfloat162_rn(acc[0] * inv, acc[1] * inv);
-    *reinterpret_cast<__nv_bfloat162*>(out + 2) = __floats2bfloat162_rn(acc[2] * inv, acc[3] * inv);
+  // a row and 16 columns a thread, a warp's lanes on neighbouring rows; with fewer rows than lanes, lanes share a row's parts among them
+  const int there = min(rows - row0, kMergeRows);
+  int wide = 1;
+  while (wide < there) wide <<= 1;
+  const int row = row0 + (lane & (wide - 1)), share = 32 / wide;
+  const bool live = row < row0 + there;
+  const int tok = (live ? row : row0) / p.G, t = s.q_begin + node0 + tok, sub = (live ? row : row0) - tok * p.G;
+  int pc0 = 0, shared_parts = 0, p_item = 0, p_row = 0, p_begin = 0;
+  bool p_two = false;
+  if (all_units > 0) {
+    const int p_tile = t / p.npt, p_pair = p_tile >> 1;
+    p_item = sa_item(p, all, -1, p_pair, h);
+    p_two = sa_weight(p, all, p_pair) == 2;
+    p_begin = p_pair * p.Hkv * sa_length(p, all, -1, 0) + h * sa_length(p, all, -1, p_pair);
+    pc0 = (p_begin + kItemCost) / piece;
+    shared_parts = ((p_begin + kItemCost + ((all_units - 1) << p_two)) / piece - pc0 + 1) * (p_two ? 1 : 2);
+    p_row = (t - p_tile * p.npt) * p.G + sub + (p_two ? (p_tile & 1) * SROWS : 0);
   }
+  const int parts = live ? shared_parts + own_parts : 0;
+  float m = -INFINITY, l = 0.f, acc[16];
+#pragma unroll
+  for (int j = 0; j < 16; ++j) acc[j] = 0.f;
+  auto exp_of = [](float v, float top) { return top == -INFINITY ? (v == v ? 0.f : v) : exp2f(v - top); };      // NaN scores leave a sum without a maximum
+#pragma unroll 2
+  for (int k = lane / wide; k < parts; k += share) {
+    const bool common = k < shared_parts, pair_of = common ? p_two : two;
+    const int j = common ? k : k - shared_parts, c = (common ? pc0 : c0) + (pair_of ? j : j >> 1), begin = common ? p_begin : own_begin;
+    // a cut piece may hold no unit's beginning, and then no part
+    if (sa_unit(c * piece - begin, pair_of) == sa_unit((c + 1) * piece - begin, pair_of) || (!common && row >= p.seq_rows_kept)) continue;
+    const int kept = common ? SROWS : p.seq_rows_kept, at_row = common ? p_row % SROWS : row;
+    const size_t seg = static_cast<size_t>(c + (common ? p_item : item)) * 2 + (common ? (p_two ? p_row / SROWS : j & 1) : two ? tile & 1 : j & 1);
+    const float2 ml = (common ? p.pml : p.sml)[seg * kept + at_row];
+    const float4* from = reinterpret_cast<const float4*>((common ? p.po : p.so) + (seg * SD + 16 * warp) * kept + 8 * at_row);
+    const float4 x[4] = {from[0], from[1], from[2 * kept], from[2 * kept + 1]};
+    if (ml.y == 0.f) continue;                 // no visible key: the part's output may be unwritten
+    const float top = fmaxf(m, ml.x), old = exp_of(m, top), add = exp_of(ml.x, top);
+    m = top;
+    l = l * old + ml.y * add;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      acc[4 * q] = fmaf(x[q].x, add, acc[4 * q] * old);
+      acc[4 * q + 1] = fmaf(x[q].y, add, acc[4 * q + 1] * old);
+      acc[4 * q + 2] = fmaf(x[q].z, add, acc[4 * q + 2] * old);
+      acc[4 * q + 3] = fmaf(x[q].w, add, acc[4 * q + 3] * old);
+    }
+  }
+  for (int o = wide; o < 32; o <<= 1) {
+    const float m2 = __shfl_xor_sync(0xffffffffu, m, o), l2 = __shfl_xor_sync(0xffffffffu, l, o);
+    const float top = fmaxf(m, m2), f = exp_of(m, top), f2 = exp_of(m2, top);
+    m = top;
+    l = l * f + l2 * f2;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) acc[j] = acc[j] * f + __shfl_xor_sync(0xffffffffu, acc[j], o) * f2;
+  }
+  if (!live || lane >= wide) return;
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  uint32_t pk[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+    pk[j] = *reinterpret_cast<const uint32_t*>(&v);
+  }
+  sa_store32(p.out + (static_cast<size_t>(t) * p.Hq + h * p.G + sub) * SD + 16 * warp, pk);
 }
 
 // Queries as (tokens, heads, 128), tokens ldq elements apart
