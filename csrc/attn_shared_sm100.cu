@@ -340,6 +340,10 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     }
     return before;
   };
+  for (int b = tid; blockIdx.x == 0 && b < p.B; b += STHREADS) {
+    const SaSeq s = sa_seq(p, b);
+    if (s.n > 0 && s.past < p.prefix) report(p.status, kShortPrefix);
+  }
   const int mine = tid < p.B ? sa_total(p, tid) * p.Hkv : 0;
   int total;
   const int mine_ahead = ahead(mine, total);
@@ -883,7 +887,9 @@ static int shared_setup(SharedAttn* p, int max_q, int prefix_len, int ctas) {
   p->ctas = ctas;
   // The sequences' own items begin at a multiple of 16 positions, where pages do, so that their keys load in boxes.
   p->prefix = p->first_key = shared_pays(p->B, p->T, p->npt) ? prefix_len / 16 * 16 : 0;
-  return 0;
+  // places on the line are 32-bit: at most this many items, of at most that length
+  const double items = (2.0 * (p->T / (2 * p->npt)) + p->B + 2) * p->Hkv;
+  return items * (2.0 * (p->max_len / SKEYS + 1) + kItemCost) < 2e9 ? 0 : -16;
 }
 
 }  // namespace js

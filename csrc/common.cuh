@@ -33,6 +33,7 @@ enum : int {
   kNoPage = 13,           // slot plan: the free pages ran out
   kRowsOverflow = 14,     // slot plan: more new rows than the row buffers hold
   kBadToken = 15,         // a drafted token outside the vocabulary
+  kShortPrefix = 16,      // a sequence that is shorter than the prefix it shares
 };
 
 constexpr uint32_t kSpinLimit = 1u << 20;  // polls; each try_wait already suspends for a while

@@ -183,7 +183,7 @@ STATUS_NAMES = {0: "ok", 1: "timeout waiting for a TMA stage", 2: "timeout waiti
                 11: "vocabulary-parallel top-k: a rank's record never arrived",
                 12: "expert-parallel dispatch: more rows for one expert than the grouped launch covers",
                 13: "slot plan: the free pages ran out", 14: "more new rows than the caller's bound",
-                15: "drafted token outside the vocabulary"}
+                15: "drafted token outside the vocabulary", 16: "sequence shorter than the prefix it shares"}
 
 
 def check_status(device) -> None:

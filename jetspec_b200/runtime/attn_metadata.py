@@ -47,10 +47,10 @@ def build_attn_metadata(pool, seq_ids: Sequence[int], past_lens: Sequence[int],
     causal = trees is None
     counts = [int(t.num_nodes) for t in trees] if not causal else [int(n) for n in num_query_nodes]
     rows = np.array([pool.state(s).row for s in seq_ids], dtype=np.int32)
-    if causal and B:
+    if causal and B and np.unique(rows).size == B:      # a plan serves a slot-map row once
         # lengths are all that is uploaded: offsets, positions and slots follow from them on the device
         from .. import ops
-        past = np.asarray(past_lens, dtype=np.int32)
+        past = np.asarray([int(n) for n in past_lens], dtype=np.int32)
         new = np.asarray(counts, dtype=np.int32)
         packed = torch.from_numpy(np.concatenate((rows, past, new, past + new))).to(device)
         seq_rows, past_t, counts_t, mapped = packed.split((B, B, B, B))
@@ -69,13 +69,16 @@ def build_attn_metadata(pool, seq_ids: Sequence[int], past_lens: Sequence[int],
     slot_rows = []
     for b in range(B):
         s, e, past = int(cu[b]), int(cu[b + 1]), int(past_lens[b])
-        t = trees[b]
-        host = getattr(t, "host", None)          # builder's own lists: no device read per sequence
-        depth_h = np.asarray(host[2], dtype=np.int32) if host is not None else t.depth.cpu().numpy().astype(np.int32)
-        parents_h = host[1] if host is not None else t.parent_indices.tolist()
-        pos[s:e] = past + depth_h
-        bits[s:e, : max(1, (counts[b] + 31) // 32)] = ancestor_bits_np(
-            parents_h, counts[b], max(1, (counts[b] + 31) // 32))
+        if causal:
+            pos[s:e] = past + np.arange(e - s, dtype=np.int32)
+        else:
+            t = trees[b]
+            host = getattr(t, "host", None)          # builder's own lists: no device read per sequence
+            depth_h = np.asarray(host[2], dtype=np.int32) if host is not None else t.depth.cpu().numpy().astype(np.int32)
+            parents_h = host[1] if host is not None else t.parent_indices.tolist()
+            pos[s:e] = past + depth_h
+            bits[s:e, : max(1, (counts[b] + 31) // 32)] = ancestor_bits_np(
+                parents_h, counts[b], max(1, (counts[b] + 31) // 32))
         slot_rows.append(pool.slot_map[int(rows[b]), past:past + (e - s)])
     slots = torch.cat(slot_rows) if slot_rows else torch.zeros(0, dtype=torch.int32, device=device)
     to = lambda a: torch.from_numpy(a).to(device)

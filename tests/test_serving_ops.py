@@ -456,6 +456,9 @@ def test_shared_prefix_attention_of_odd_calls(clean):
     attend(c, max_q=4)
     with pytest.raises(RuntimeError, match="more new rows"):
         clean.check_status("cuda")
+    attend({**attention_case(2, 8, 2, 64, [0, 0, 0, 0], [1, 1, 1, 1], True, device="cuda"), "past_lens": i32(64, 64, 47, 64, device="cuda")})
+    with pytest.raises(RuntimeError, match="shorter than the prefix"):
+        clean.check_status("cuda")
     for slot in (-1, c["k_pool"].shape[1]):
         m = c["slot_map"].clone()
         m[3, 95] = slot          # row 2 is the sequence without rows: nobody reads it
@@ -612,6 +615,8 @@ def causal_rows(pool):
     rows = [pool.slot_map[pool.state(s).row, p:p + n] for s, p, n in zip((3, 9, 7), past, counts)]
     assert torch.equal(m.slots, torch.cat(rows)) and m.causal and m.mask_bits is None
     assert {t.dtype for t in (m.cu_q, m.past_lens, m.seq_rows, m.positions, m.slots)} == {I32}
+    two = build_attn_metadata(pool, [9, 9], [1, 4], num_query_nodes=[3, 2])      # neighbouring portions of one sequence
+    assert two.positions.tolist() == [1, 2, 3, 4, 5] and torch.equal(two.slots, pool.slot_map[pool.state(9).row, 1:6])
 
 
 def test_pools_and_batches_plan_their_slots():
