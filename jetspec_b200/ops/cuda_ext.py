@@ -1579,16 +1579,19 @@ def plan_slots(past_lens, counts, seq_rows, free_pages, page_size: int, slot_map
         _refuse("past_lens, counts, seq_rows and mapped_lens differ in length")
     if B > 65535 or page_size < 1 or rows < 0:
         _refuse(f"plan_slots(B={B}, page_size={page_size}, rows={rows})")
-    whole = rows + 3 & ~3              # results start on 16-byte boundaries
-    buf = slot_map.new_empty(2 * whole + 2 * (B + 1))
-    at = buf.data_ptr()
-    positions, _, slots, _, cu_q, cu_pages = buf.split_with_sizes((rows, whole - rows, rows, whole - rows, B + 1, B + 1))
+    pad = -rows & 3                    # positions and slots start on 16-byte boundaries
+    buf = slot_map.new_empty(2 * (rows + B + 1) + pad)
+    at, ends = buf.data_ptr(), 4 * (2 * rows + pad)
+    if pad:
+        positions, _, slots, cu_q, cu_pages = buf.split_with_sizes((rows, pad, rows, B + 1, B + 1))
+    else:
+        positions, slots, cu_q, cu_pages = buf.split_with_sizes((rows, rows, B + 1, B + 1))
     # Blocks a request: 4096 positions each, as every block sums the requests before it anew (128 requests: 4.1 us, with 1024 positions 6.1),
     # and no more blocks than the SMs hold at once (8 of 256 threads; 256 prompts: 14 us, with 4 14.9, with 32 22).
     chunks = max(1, min(8 * SM_COUNT // max(1, B), max_len // 4096))
     rc = _entry("js_slot_plan", "pppppppppppiiiiiiip")(
         past_lens.data_ptr(), counts.data_ptr(), mapped.data_ptr(), seq_rows.data_ptr(), free_pages.data_ptr(), slot_map.data_ptr(),
-        at + 8 * whole, at + 8 * whole + 4 * (B + 1), at, at + 4 * whole, _status_at(index), B, free_pages.numel(), page_size,
+        at + ends, at + ends + 4 * (B + 1), at, at + 4 * (rows + pad), _status_at(index), B, free_pages.numel(), page_size,
         max_seqs, max_len, rows, chunks, _stream_at(index))
     if rc:
         _check(rc, "js_slot_plan")
