@@ -6,15 +6,22 @@
 // own keys [P, L), and the parts are joined.  Where every sequence's rows fill tiles of their own there is nothing to gain by that, and a
 // sequence's rows take both ranges in one go.
 //
-// Work is a line of units, a unit being 80 keys for a pair of row tiles: items (pair of tiles, KV head) one after the other, an
-// item's units in key order behind a few that stand for what it costs beside them.  Every CTA takes an equal piece of the line, so lengths, which only the device knows, balance by
-// themselves; where a piece begins or ends inside an item its parts go through a workspace and attn_shared_merge_kernel.
+// Work is a line of units, a unit being 96 keys for a pair of row tiles: items (pair of tiles, KV head) one after the other, an
+// item's units in key order behind a few that stand for what it costs beside them.  Every CTA takes an equal piece of the line, so
+// lengths, which only the device knows, balance by themselves; where a piece begins or ends inside an item its parts go through a
+// workspace and attn_shared_merge_kernel.
 //
-// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warps 8 and 11 issue the MMAs of either product, warps 9 and 10 load K and V (and Q) by
-// TMA (boxes of 16 rows where slots follow one another, gathers of four rows where not).  A job is one row tile against 80 keys; jobs alternate between the
-// groups: the two tiles of a pair on the same keys, or, for a single tile, every other block of keys.  Tensor memory holds
-// scores (80 columns), probabilities as bf16 (40; the second MMA's A operand) and output (128) of both groups, so that a group's next scores
-// are there while it weighs its last ones.  Every wait is bounded (status word).
+// A CTA: two softmax groups (warps 0-3, 4-7; one row a thread), warps 8 and 11 issue the MMAs of either product, warps 9 and 10
+// load K and V (and Q) by TMA (boxes of 16 rows where slots follow one another, gathers of four rows where not).  A job is one row
+// tile against 96 keys; jobs alternate between the groups: the two tiles of a pair on the same keys, or, for a single tile, every
+// other block of keys.  The groups use one set of score columns in turn: a group has its row in registers 300 cycles after the
+// scores are there, and then the next job's may overwrite them.  Every wait is bounded (status word).
+//
+// What bounds it: the first product takes the time of 128 keys for any fewer (512 cycles, its operand of 128 rows is read from
+// shared memory whatever the columns), the second 64 cycles for 16 keys, and the softmax of a group about 500 issue slots and 770
+// cycles of the special function unit a job, both groups on the same schedulers.  16 trees of 128 nodes behind 8192 keys (floor
+// 176 us): 245 - 279 us, by what the power cap leaves; with 80 keys and scores of their own for each group 262 - 293, with 128 keys
+// (which spill) 306, with 64 keys and probabilities in two buffers 336; a quarter of the exponentials as polynomials 299.
 #include "gemm_common.cuh"
 
 #include <math.h>
@@ -24,16 +31,14 @@ namespace js {
 
 constexpr int SD = 128;              // head dim
 constexpr int SROWS = 128;           // rows of a tile
-constexpr int SKEYS = 80;            // keys of a unit: scores (80 columns) and probabilities (40) of a group fit 128 columns side by side
-constexpr int SSLOTS = 8;            // ring of K and V tiles, in turn
-constexpr int kItemCost = 6;         // what an item costs beside its jobs, in jobs: setting out, and results out of tensor memory
+constexpr int SKEYS = 96;            // keys of a unit
+constexpr int KSLOTS = 3, VSLOTS = 3, SSLOTS = KSLOTS + VSLOTS;      // rings of K and V tiles
+constexpr int kItemCost = 8;         // what an item costs beside its jobs, in jobs: setting out, and results out of tensor memory
 constexpr int kQTile = SROWS * 256, kKTile = SKEYS * 256;      // bytes of a Q, K or V tile: 2 halves x rows x 128 B
 constexpr int SWARPS = 12, STHREADS = 32 * SWARPS;      // three warps to a quarter of the SM: 168 registers a thread
 constexpr int kSharedSmem = 2 * kQTile + SSLOTS * kKTile + 512;
-// Of eight pairs of exponentials, those computed on the FMA pipe: 16 trees of 128 nodes 332 us without, 321, 316, 325 and 329 us with 1 to 4
-// (the special function unit alone takes 640 cycles a job, the MMAs 730).
-constexpr int kOnFma = 2;
-constexpr int kColP = SKEYS, kColO = 256;      // tensor memory: scores of group g from column 128 g, its probabilities behind them, its output from 256 + 128 g
+// Tensor memory: scores of a job in columns 0-95, which the groups use in turn; probabilities of group g from 128 + 64 g, its output from 256 + 128 g
+constexpr int kColP = 128, kColO = 256;
 
 struct SharedAttn {
   const __nv_bfloat16* q;      // (T, Hq, 128), ldq elements between tokens
@@ -180,17 +185,6 @@ JS_DEVICE void sa_store32(void* to, const uint32_t* v) {
                "r"(v[6]), "r"(v[7])
                : "memory");
 }
-JS_DEVICE void sa_tmem_ld16(uint32_t taddr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr) : "memory");
-}
-JS_DEVICE void sa_tmem_st8(uint32_t taddr, const uint32_t* r) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-               ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
-}
 JS_DEVICE void sa_tmem_st32(uint32_t taddr, const uint32_t* r) {
   sa_tmem_st16(taddr, r);
   sa_tmem_st16(taddr + 16, r + 16);
@@ -222,27 +216,6 @@ JS_DEVICE uint64_t sa_add2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
-}
-// 2^x for both of a pair on the FMA pipe, x <= 0: the nearest integer goes to the exponent, the rest f through the cubic that is 1 at 0 and
-// nearest to 2^f in relative error over [-1/2, 1/2] (1.0e-4, a fortieth of half a bf16 step).  x is cut at -127, which gives 0.
-JS_DEVICE void sa_exp2_pair(uint64_t x, float& lo, float& hi) {
-  constexpr float kRound = 12582912.f;           // 1.5 * 2^23: the sum's low bits are the integer
-  float a, b;
-  sa_unpack(x, a, b);
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(a));      // -127
-  asm("max.NaN.f32 %0, %0, 0fC2FE0000;" : "+f"(b));
-  x = sa_pack(a, b);
-  const uint64_t t = sa_add2(x, sa_pack(kRound, kRound));
-  const uint64_t n = sa_add2(t, sa_pack(-kRound, -kRound));
-  const uint64_t f = sa_fma2(n, sa_pack(-1.f, -1.f), x);
-  uint64_t y = sa_fma2(f, sa_pack(0.05500864f, 0.05500864f), sa_pack(0.2422105f, 0.2422105f));
-  y = sa_fma2(y, f, sa_pack(0.69328291f, 0.69328291f));
-  y = sa_fma2(y, f, sa_pack(1.f, 1.f));
-  float ta, tb, ya, yb;
-  sa_unpack(t, ta, tb);
-  sa_unpack(y, ya, yb);
-  lo = __int_as_float((__float_as_int(ta) << 23) + __float_as_int(ya));
-  hi = __int_as_float((__float_as_int(tb) << 23) + __float_as_int(yb));
 }
 JS_DEVICE void sa_tma_heads(uint32_t dst, const CUtensorMap* m, uint64_t* bar, int x, int head, int token) {
   asm volatile(
@@ -416,7 +389,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     const CUtensorMap *box = values ? &maps.v16 : &maps.k16, *one = values ? &maps.v1 : &maps.k1;
     // One tile ahead: the slots of the next one, which may be another sequence's, are asked for before this one is issued.
     struct Tile {
-      int slot[3], row0, keys;                  // keys: to the end of what the item sees, from the tile's first
+      int slot[SKEYS / 32], row0, keys;                  // keys: to the end of what the item sees, from the tile's first
       int token, h, sides;                      // a segment's first tile: its Q tiles (sides 0: another tile)
     };
     const int* slots = nullptr;
@@ -438,7 +411,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       t.h = w.h;
       t.sides = at > 0 ? 0 : w.two ? 2 : 1;
 #pragma unroll
-      for (int part = 0; part < 3; ++part) t.slot[part] = __ldg(slots + min(first + 32 * part + lane, end - 1));      // keys past the end repeat the last one
+      for (int part = 0; part < SKEYS / 32; ++part) t.slot[part] = __ldg(slots + min(first + 32 * part + lane, end - 1));      // keys past the end repeat the last one
       if (++at < w.nt) return true;
       sa_done(w);
       return open();
@@ -446,7 +419,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     Tile tile, next{};
     bool have = open(), more = have && ask(tile), ok = true;
     int uses = 0;                               // Q buffers filled so far: buffer uses % 2
-    for (int n = values; have; n += 2) {
+    for (int n = 0; have; ++n) {
       have = more;
       if (more) more = ask(next);
       for (int side = 0; values && side < tile.sides && ok; ++side, ++uses) {
@@ -468,9 +441,9 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       // Groups of 16 keys: those in one page load as a box, others four rows at a time, and those behind the last key not at all (the
       // second product leaves them out, and the scores of the first are masked).
       unsigned paged = 0;
-      int page[6];
+      int page[SKEYS / 16];
 #pragma unroll
-      for (int part = 0; part < 3; ++part) {
+      for (int part = 0; part < SKEYS / 32; ++part) {
         int& slot = tile.slot[part];
         if (slot < 0 || slot >= p.S) { report(p.status, kBadSlot); slot = 0; }
         const int first = __shfl_sync(0xffffffffu, slot, lane & 16);
@@ -483,13 +456,13 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         page[2 * part + 1] = tile.row0 + __shfl_sync(0xffffffffu, slot, 16);
       }
       const int groups = min(SKEYS / 16, (tile.keys + 15) / 16);
-      const int s = n % SSLOTS;
-      if (!sa_wait(&kv_empty[s], ((n / SSLOTS) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up)) break;
+      const int s = values ? KSLOTS + n % VSLOTS : n % KSLOTS;
+      if (!sa_wait(&kv_empty[s], ((n / (values ? VSLOTS : KSLOTS)) & 1) ^ 1, p.status, kTimeoutEmpty, gave_up)) break;
       const uint32_t dst = smem_u32(sKV + s * kKTile);
       if (elect_one()) {
         mbar_expect_tx(&kv_full[s], groups * 4096);
 #pragma unroll
-        for (int part = 0; part < 5; ++part) {
+        for (int part = 0; part < SKEYS / 16; ++part) {
           if (part >= groups || !((paged >> part) & 1u)) continue;
           sa_tma_box(dst + part * 2048, box, &kv_full[s], 0, page[part]);
           sa_tma_box(dst + part * 2048 + SKEYS * 128, box, &kv_full[s], 64, page[part]);
@@ -499,7 +472,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const unsigned rest = ((1u << groups) - 1u) & ~paged;
       if (rest != 0) {
 #pragma unroll
-        for (int part = 0; part < 5; ++part) {
+        for (int part = 0; part < SKEYS / 16; ++part) {
           if (!((rest >> part) & 1u)) continue;
 #pragma unroll
           for (int g = 4 * part; g < 4 * part + 4; ++g) {
@@ -518,7 +491,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     }
   } else if (warp == 8) {
     // ================================================================ issuer of the first product: S = Q K^T of a job once the group's scores before it are read
-    // (An issuer's waits and MMAs of a job take 700 cycles, about as long as the MMAs run: one warp for both products held them up.)
+    // (One warp for both products held the MMAs up: its waits take as long as they run.)
     constexpr uint32_t idesc = umma_idesc_bf16(SROWS, SKEYS);
     const uint64_t q_desc = umma_desc_sw128(smem_u32(sQ)), k_desc = umma_desc_sw128(smem_u32(sKV));
     int n = 0, tile = 0, use = 0;               // jobs; K tiles and Q buffers of the segments before
@@ -526,16 +499,16 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     while (ok && sa_next(p, w)) {
       const int sides = w.two ? 2 : 1, jobs = w.nt * sides;
       for (int job = 0; job < jobs; ++job, ++n) {
-        const int g = n & 1, side = w.two ? job & 1 : 0, buf = (use + side) & 1, slot = 2 * (tile + (w.two ? job >> 1 : job)), s = slot % SSLOTS;
+        const int g = n & 1, side = w.two ? job & 1 : 0, buf = (use + side) & 1, slot = tile + (w.two ? job >> 1 : job), s = slot % KSLOTS;
         if (job < sides && !(ok = sa_wait(&q_full[buf], ((use + side) >> 1) & 1, p.status, kTimeoutFull, gave_up))) break;
-        if (side == 0 && !(ok = sa_wait(&kv_full[s], (slot / SSLOTS) & 1, p.status, kTimeoutFull, gave_up))) break;
-        if (n >= 2 && !(ok = sa_wait(&s_read[g], ((n >> 1) - 1) & 1, p.status, kTimeoutAccum, gave_up))) break;
+        if (side == 0 && !(ok = sa_wait(&kv_full[s], (slot / KSLOTS) & 1, p.status, kTimeoutFull, gave_up))) break;
+        if (n > 0 && !(ok = sa_wait(&s_read[g ^ 1], ((n - 1) >> 1) & 1, p.status, kTimeoutAccum, gave_up))) break;
         tc_fence_after();
         if (elect_one()) {
           const uint64_t a = q_desc + static_cast<uint64_t>(buf * (kQTile >> 4)), b = k_desc + static_cast<uint64_t>(s * (kKTile >> 4));
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_f16(tmem + g * 128, a + (k >> 2) * (SROWS * 128 >> 4) + 2 * (k & 3), b + (k >> 2) * (SKEYS * 128 >> 4) + 2 * (k & 3), idesc, k != 0);
+            umma_f16(tmem, a + (k >> 2) * (SROWS * 128 >> 4) + 2 * (k & 3), b + (k >> 2) * (SKEYS * 128 >> 4) + 2 * (k & 3), idesc, k != 0);
           umma_commit(&s_full[g]);
           if (side == sides - 1) umma_commit(&kv_empty[s]);
           if (job + sides >= jobs) umma_commit(&q_empty[buf]);
@@ -556,8 +529,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       const int end = sa_end(p, w.s, w.b, w.pair);
       const int sides = w.two ? 2 : 1, jobs = w.nt * sides;
       for (int job = 0; job < jobs; ++job, ++n) {
-        const int g = n & 1, slot = 2 * (tile + (w.two ? job >> 1 : job)) + 1, s = slot % SSLOTS;
-        if (!(ok = sa_wait(&kv_full[s], (slot / SSLOTS) & 1, p.status, kTimeoutFull, gave_up))) break;
+        const int g = n & 1, slot = tile + (w.two ? job >> 1 : job), s = KSLOTS + slot % VSLOTS;
+        if (!(ok = sa_wait(&kv_full[s], (slot / VSLOTS) & 1, p.status, kTimeoutFull, gave_up))) break;
         if (!(ok = sa_wait(&p_full[g], (n >> 1) & 1, p.status, kTimeoutAccum, gave_up))) break;
         tc_fence_after();
         if (elect_one()) {
@@ -565,7 +538,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
           const int keys = end - (w.s.first + (w.first + (w.two ? job >> 1 : job)) * SKEYS);
 #pragma unroll
           for (int k = 0; k < SKEYS / 16; ++k)
-            if (16 * k < keys) sa_mma_tmem_a(tmem + kColO + g * 128, tmem + g * 128 + kColP + k * 8, b + k * (2048 >> 4), idesc, k != 0 || job >= 2);
+            if (16 * k < keys) sa_mma_tmem_a(tmem + kColO + g * 128, tmem + kColP + g * 64 + k * 8, b + k * (2048 >> 4), idesc, k != 0 || job >= 2);
           umma_commit(&pv_done[g]);
           if (!w.two || (job & 1)) umma_commit(&kv_empty[s]);
         }
@@ -578,7 +551,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     // ================================================================ softmax and epilogue: one row a thread
     const int g = warp >> 2, row = (warp & 3) * 32 + lane, tok = row / p.G, sub = row % p.G;
     const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t ts = tmem + t_lane + g * 128, to = tmem + t_lane + kColO + g * 128;
+    const uint32_t ts = tmem + t_lane, tp = ts + kColP + g * 64, to = tmem + t_lane + kColO + g * 128;
     int jobs_done = 0;                          // of this group: the phase of its barriers
     bool ok = true;
     bool more = sa_next(p, w);
@@ -595,10 +568,10 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       for (int i = w.two ? 0 : rel; i < w.nt && ok; i += w.two ? 1 : 2, ++jobs, ++jobs_done) {
         const int k0 = w.s.first + (w.first + i) * SKEYS;
         const bool all = k0 + SKEYS <= min(w.s.past, end);      // every row of the item sees the whole block
-        uint32_t see[3] = {0u, 0u, 0u};
+        uint32_t see[SKEYS / 32] = {};
         if (!all && valid) {
 #pragma unroll
-          for (int c = 0; c < 3; ++c) see[c] = sa_visible(p, w.s, prefix, end, node, bits, k0 + 32 * c);
+          for (int c = 0; c < SKEYS / 32; ++c) see[c] = sa_visible(p, w.s, prefix, end, node, bits, k0 + 32 * c);
         }
         ok = sa_wait(&s_full[g], jobs_done & 1, p.status, kTimeoutAccum, gave_up);
         if (!ok) break;
@@ -611,9 +584,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
           continue;
         }
         uint32_t sr[SKEYS];
-        tmem_ld_32x32(ts, sr);
-        tmem_ld_32x32(ts + 32, sr + 32);
-        sa_tmem_ld16(ts + 64, sr + 64);
+#pragma unroll
+        for (int c = 0; c < SKEYS; c += 32) tmem_ld_32x32(ts + c, sr + c);
         tmem_ld_wait();
         tc_fence_before();
         mbar_arrive(&s_read[g]);
@@ -634,28 +606,29 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         m_run = m_new;
         const uint64_t scale2 = sa_pack(p.scale_log2, p.scale_log2), shift2 = sa_pack(-m_safe, -m_safe);
         uint64_t sum2[4] = {0ull, 0ull, 0ull, 0ull};
-        uint32_t pr[SKEYS / 2];
 #pragma unroll
-        for (int j = 0; j < SKEYS / 2; ++j) {
-          float p0, p1;
-          const uint64_t x = sa_fma2(sa_pack(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), scale2, shift2);
-          if (j % 8 < kOnFma) {
-            sa_exp2_pair(x, p0, p1);
-          } else {
+        for (int part = 0; part < SKEYS / 32; ++part) {
+          uint32_t pr[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int j = part * 16 + i;
+            float p0, p1;
+            const uint64_t x = sa_fma2(sa_pack(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1])), scale2, shift2);
             sa_unpack(x, p0, p1);
             p0 = sa_exp2(p0);
             p1 = sa_exp2(p1);
+            sum2[j & 3] = sa_add2(sum2[j & 3], sa_pack(p0, p1));
+            const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);      // the MMA's operand: bf16, the sum keeps fp32
+            pr[i] = *reinterpret_cast<const uint32_t*>(&v);
           }
-          sum2[j & 3] = sa_add2(sum2[j & 3], sa_pack(p0, p1));
-          const __nv_bfloat162 v = __floats2bfloat162_rn(p0, p1);      // the MMA's operand: bf16, the sum keeps fp32
-          pr[j] = *reinterpret_cast<const uint32_t*>(&v);
+          if (part == 0 && jobs_done > 0) {      // this group's PV before: its probabilities are read, its output is complete
+            ok = sa_wait(&pv_done[g], (jobs_done - 1) & 1, p.status, kTimeoutAccum, gave_up);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          sa_tmem_st16(tp + 16 * part, pr);
         }
-        // this group's PV before: its probabilities are read, its output is complete
-        if (jobs_done > 0) ok = sa_wait(&pv_done[g], (jobs_done - 1) & 1, p.status, kTimeoutAccum, gave_up);
         if (!ok) break;
-        tc_fence_after();
-        sa_tmem_st32(ts + kColP, pr);
-        sa_tmem_st8(ts + kColP + 32, pr + 32);
         if (__any_sync(0xffffffffu, valid && jobs > 0 && alpha != 1.f)) {
 #pragma unroll 1
           for (int c = 0; c < SD; c += 32) {
