@@ -17,11 +17,12 @@
 // other block of keys.  The groups use one set of score columns in turn: a group has its row in registers 300 cycles after the
 // scores are there, and then the next job's may overwrite them.  Every wait is bounded (status word).
 //
-// What bounds it: the first product takes the time of 128 keys for any fewer (512 cycles, its operand of 128 rows is read from
-// shared memory whatever the columns), the second 64 cycles for 16 keys, and the softmax of a group about 500 issue slots and 770
-// cycles of the special function unit a job, both groups on the same schedulers.  16 trees of 128 nodes behind 8192 keys (floor
-// 176 us): 245 - 279 us, by what the power cap leaves; with 80 keys and scores of their own for each group 262 - 293, with 128 keys
-// (which spill) 306, with 64 keys and probabilities in two buffers 336; a quarter of the exponentials as polynomials 299.
+// What bounds it: the way of a job's scores, product to registers to the next job's product, with the second product of the job
+// before in between: 1,380 cycles a job of 128 rows x 96 keys, of which the tensor pipe is busy for 770 (56 %), the special function
+// unit for 800 (58 %) and the schedulers for 620 (45 %).  16 trees of 128 nodes behind
+// 8192 keys (floor 176 us): 255 us, 293 under the power cap.  Against it, in turn on one GPU: 80 keys and scores of their own for each
+// group 312 (293 here), scores of their own and one set of probabilities 269 (260 here), 128 keys (which spill) 306 (279 here), 64
+// keys and probabilities in two buffers 336 (279 here), a quarter of the exponentials as polynomials 299 (279 here).
 #include "gemm_common.cuh"
 
 #include <math.h>
