@@ -7,14 +7,15 @@
 // A temperature below 1e-5 is a point mass at the lowest most likely index.
 //
 // chain_stats_kernel reads the rows of some drafts (maximum, sum of exponentials) and decides about them; chain_token_kernel draws
-// the token, a cluster per sequence.  Where reading every row would take long, the first kernel runs for draft 0 of all sequences,
-// then 1, 2, 3-4, 5-8 and the rest, so that rows behind a rejection are not read.  Sums that only decide `u q < p` are fp32 (a
-// decision is off by some 1e-7 of a probability); the running sum that a token is found in is fp64, as its index would change with
+// the token, a cluster per sequence.  A block of the first kernel asks whether an earlier draft of its sequence is known to be
+// rejected before it reads; blocks start in the order of their drafts, eight at a time, so that most rows behind a rejection are not
+// read (64 chains of 4 to 16 drafts over 151936 fp32 values 146 us; all drafts at a time 187, four 155; six launches for draft 0, 1,
+// 2, 3-4, 5-8 and the rest 182, as each starts and ends with SMs that have nothing in flight).  Sums that only decide `u q < p` are fp32
+// (a decision is off by some 1e-7 of a probability); the running sum that a token is found in is fp64, as its index would change with
 // every rounding among 150,000 terms.
 //
-// What bounds it: few sequences, latency (one chain of 3 drafts over 151936 fp32 values 26 us, 12 us in either kernel); many, reading
-// (64 chains of 4 to 16 drafts 182 us, of which six launches that read only needed rows take 120, a third of the copy rate: each
-// starts and ends with SMs that have nothing in flight) and the fp64 pipe with the table's banks (the draw, 60 us).
+// What bounds it: few sequences, latency (one chain of 3 drafts 26 us, 12 us in either kernel); many, reading (90 of those 146 us) and
+// the fp64 pipe with the table's banks (the draw, 60 us).
 #include "common.cuh"
 
 #include <math.h>
@@ -29,6 +30,7 @@ template <typename T>
 struct StatShape { static constexpr int kThreads = 256, kResident = 4; };
 template <>
 struct StatShape<float> { static constexpr int kThreads = 128, kResident = 6; };
+constexpr int kAhead = 8;            // drafts of a sequence that blocks of their own read
 constexpr int kChainThreads = 512;
 constexpr float kGreedyBelow = 1e-5f;
 constexpr int kNoneRejected = 0x7fffffff;
@@ -124,9 +126,9 @@ JS_DEVICE float warp_max_f32(float v) {
   asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
-// One chunk of the rows of drafts lo + z, lo + z + Z, ... below hi of a sequence: block (chunk, sequence, z).
+// One chunk of the rows of drafts z, z + Z, ... of a sequence: block (chunk, sequence, z).
 template <typename T>
-__global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResident) chain_stats_kernel(ChainParams p, int lo, int hi) {
+__global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResident) chain_stats_kernel(ChainParams p) {
   constexpr int N = 16 / sizeof(T), kStatThreads = StatShape<T>::kThreads, kStatBlocks = kChunkBytes / 16 / kStatThreads, kWarps = kStatThreads / 32;
   __shared__ float tops[2][kWarps], sums[2][kWarps];
   __shared__ int where[2], go;
@@ -134,11 +136,10 @@ __global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResiden
   pdl_launch_dependents();
   int first;
   const int n = chain_span(p, b, first);
-  pdl_wait();                                  // what the launch before decided; ahead of any return, so that launches end in their order
-  if (lo + static_cast<int>(blockIdx.z) > n) return;
+  if (static_cast<int>(blockIdx.z) > n) return;
   const double temps[2] = {chain_temp(p.temp, p.temp_all, b), chain_temp(p.draft_temp, p.draft_temp_all, b)};
   const float scales[2] = {chain_scale(temps[0]), chain_scale(temps[1])};
-  for (int i = lo + blockIdx.z; i < hi && i <= n; i += gridDim.z) {
+  for (int i = blockIdx.z; i <= n; i += gridDim.z) {
     // Behind a known rejection nobody needs the rows; whether they are read all the same goes by time, results do not.
     __syncthreads();
     if (tid == 0) go = kNoneRejected - *reinterpret_cast<volatile int*>(p.rejected + b) >= i;
@@ -474,30 +475,8 @@ static int launch_token(const ChainParams& p, cudaStream_t stream) {
 
 template <typename T>
 static int launch_chain(const ChainParams& p, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.blockDim = dim3(StatShape<T>::kThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 0;                            // the first launch waits for everything before it
-  auto launch = [&](int lo, int hi, int z) {
-    cfg.gridDim = dim3(p.chunks, p.B, z);
-    const bool good = cudaLaunchKernelEx(&cfg, chain_stats_kernel<T>, p, lo, hi) == cudaSuccess;
-    cfg.numAttrs = 1;
-    return good;
-  };
-  const int all = 0x7fffffff;
-  const int mean = p.D / p.B + 1;
-  // Launches in turn cost about 3 us each, so they pay where reading all rows takes several times that.
-  if (static_cast<double>(p.V) * sizeof(T) * (2.0 * p.D + p.B) < 160e6) {
-    if (!launch(0, all, mean < 64 ? mean : 64)) return -4;
-  } else {
-    for (int lo = 0, hi = 1; lo < 9; lo = hi, hi = lo < 3 ? lo + 1 : lo < 5 ? 5 : lo < 9 ? 9 : all)
-      if (!launch(lo, hi, hi - lo)) return -4;
-    if (!launch(9, all, 4)) return -4;
-  }
+  chain_stats_kernel<T><<<dim3(p.chunks, p.B, kAhead), StatShape<T>::kThreads, 0, stream>>>(p);
+  if (cudaGetLastError() != cudaSuccess) return -4;
   // As many CTAs a sequence as are there at once, two an SM (16 is more than a portable cluster has): 16 sequences 56 us with 16, 61 with 8, 68 with
   // 4; 64 sequences 184 us with 4, 193 with 8, 214 with 2.
   constexpr int kAtOnce = 2 * 148;
