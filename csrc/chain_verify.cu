@@ -77,10 +77,15 @@ JS_DEVICE float chain_exp2(float x) {
   return y;
 }
 
-struct RowStat { float m, s; int at; };      // maximum, sum of the exponentials relative to it, lowest index of the maximum
+JS_DEVICE float chain_max(float a, float b) {      // NaN if one is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+struct RowStat { float m, s; int at; };      // maximum (NaN if a logit is), sum of the exponentials relative to it, lowest index of the maximum
 JS_DEVICE RowStat join(const RowStat& a, const RowStat& b, float scale) {
   RowStat r;
-  r.m = fmaxf(a.m, b.m);
+  r.m = chain_max(a.m, b.m);
   r.at = a.m > b.m ? a.at : b.m > a.m ? b.at : min(a.at, b.at);
   const float base = chain_base(r.m, scale);
   r.s = (a.m == r.m ? a.s : a.s != 0.f ? a.s * chain_exp2(chain_base(a.m, scale) - base) : 0.f) +
@@ -100,7 +105,7 @@ JS_DEVICE RowStat warp_join(RowStat r, float scale) {
 JS_DEVICE double chain_prob(float x, int index, double temp, const RowStat& st) {
   if (temp < kGreedyBelow) return index == st.at ? 1.0 : 0.0;
   const float scale = chain_scale(temp);
-  return st.s > 0.f ? exp2(static_cast<double>(x) * scale - chain_base(st.m, scale)) / st.s : 0.0;
+  return st.s != 0.f ? exp2(static_cast<double>(x) * scale - chain_base(st.m, scale)) / st.s : 0.0;      // NaN beside a logit of +inf
 }
 
 // A row as the 16-byte blocks that hold it: a copy starts and ends with a block, and never leaves the blocks that the row has a part in.
@@ -118,12 +123,12 @@ struct ChainRow {
 
 JS_DEVICE float chain_max3(float a, float b, float c) {
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 JS_DEVICE float warp_max_f32(float v) {
   float r;
-  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
   return r;
 }
 // One chunk of the rows of drafts z, z + Z, ... of a sequence: block (chunk, sequence, z).
@@ -253,6 +258,9 @@ __global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResiden
       __syncwarp();
     }
     if (lane != 0) continue;
+    // a row with a NaN says as little as one without a logit above -inf
+    if (st.m != st.m) st = RowStat{-INFINITY, 0.f, 0x7fffffff};
+    if (sd.m != sd.m) sd = RowStat{-INFINITY, 0.f, 0x7fffffff};
     tstat[0] = make_float4(st.m, st.s, __int_as_float(st.at), 0.f);
     if (i == n) continue;
     dstat[0] = make_float4(sd.m, sd.s, __int_as_float(sd.at), 0.f);

@@ -349,7 +349,7 @@ GREEDY_BELOW = 1e-5      # temperatures below it mean the most likely token
 
 def chain_probabilities(logits: torch.Tensor, temperature: float) -> torch.Tensor:
     """fp64 ``softmax(logits / T)`` of one row; a point mass at the lowest most likely index for ``T < 1e-5``; zeros where no logit
-    is above -inf."""
+    is above -inf, or one is NaN."""
     x = logits.double()
     top = x.max()
     if not bool(top > -math.inf):
@@ -372,8 +372,9 @@ def verify_chains(target_logits: torch.Tensor, draft_logits: torch.Tensor, draft
     then distributed like the target's own.  ``temperature`` and ``draft_temperature`` (default: the same) are numbers or ``(B,)``
     tensors; below 1e-5 they mean the lowest most likely token.  The rows of a sequence behind its first rejection do not matter.
 
-    A row without any logit above -inf accepts nothing; its next token is -1.  Where rounding leaves nothing of ``max(p - q, 0)``
-    the target's most likely token is taken.  Returns ``(accepted (B,) int32, next token (B,) int64)``.
+    A target row without any logit above -inf, or with a NaN, accepts nothing; its next token is -1.  Such a draft row says nothing:
+    what the target can say at all is accepted.  Where rounding leaves nothing of ``max(p - q, 0)`` the target's most likely token
+    is taken.  Returns ``(accepted (B,) int32, next token (B,) int64)``.
     """
     B = cu_drafts.numel() - 1
     cu = cu_drafts.tolist()

@@ -1,0 +1,61 @@
+"""Operators of a batched serving step where they are easily wrong: rows that are not numbers, very large vocabularies and values, views at odd
+addresses, padded batches, long items of attention, lengths past the slot map.
+"""
+import math
+
+import pytest
+import torch
+
+from jetspec_b200 import ops
+from jetspec_b200.ops import reference as ref
+from test_serving_ops import I32, attend, attention_case, attention_close, attention_exact, clean, i32, kernel_refuses  # noqa: F401
+
+gpu = pytest.mark.gpu
+INF, NAN = math.inf, math.nan
+
+
+# ------------------------------------------------------------------ verification of chains
+def one_chain(target, draft, x, u, v, dtype=torch.float32, **kw):
+    """A chain of one sequence, on the CPU and on the GPU: what the two say."""
+    args = [torch.stack(target).to(dtype), torch.stack(draft).to(dtype) if draft else target[0].new_zeros(0, target[0].numel()).to(dtype),
+            i32(*x), i32(0, len(x)), torch.tensor(u), torch.tensor([v])]
+    got = ops.verify_chains(*[a.cuda() for a in args], **kw)
+    return tuple(int(t) for t in ref.verify_chains(*args, **kw)), tuple(int(t) for t in got)
+
+
+def test_verify_chains_of_rows_that_are_not_numbers():
+    """A NaN in a target row: nothing is accepted, no token.  In a draft row: it says nothing, like an empty row."""
+    p = torch.tensor([0.5, 0.25, 0.25]).log()
+    q = torch.tensor([0.25, 0.5, 0.25]).log()
+    bad = torch.tensor([1.0, NAN, 2.0])
+    call = lambda target, draft, x, u, v, **kw: tuple(int(t) for t in ops.verify_chains(
+        torch.stack(target), torch.stack(draft), i32(*x), i32(0, len(x)), torch.tensor(u), torch.tensor([v]), **kw))
+    for kw in (dict(), dict(temperature=0.0)):
+        assert call([bad, p], [q], [0], [.0], .5, **kw) == (0, -1)
+        assert call([p, bad], [p], [0], [.9], .5, **kw) == (1, -1)
+    assert call([p, p], [bad], [2], [.9], .3) == (1, 0)
+
+
+@gpu
+@pytest.mark.parametrize("V,dtype", [(3, torch.float32), (4099, torch.float32), (70001, torch.bfloat16)])
+def test_verify_chains_kernel_of_rows_that_are_not_numbers(clean, V, dtype):
+    g = torch.Generator().manual_seed(V)
+    p, q = (torch.randn(V, generator=g) * 2 for _ in "pq")
+    x = int(p.argmax())
+    for at in (0, V // 2, V - 1):
+        bad, far = p.clone(), p.clone()
+        bad[at] = NAN
+        far[at] = INF
+        for kw in (dict(), dict(temperature=0.0), dict(draft_temperature=0.0), dict(temperature=0.6, draft_temperature=2.0)):
+            for target, draft in (([bad, p], [q]), ([p, bad], [p]), ([p, p], [bad]), ([bad, bad], [bad]), ([far, p], [q]), ([p, far], [p]),
+                                  ([p, p], [far]), ([far, far], [far])):
+                for u in (0.0, 0.9):
+                    want, got = one_chain(target, draft, [x], [u], 0.4, dtype, **kw)
+                    assert got == want, (at, kw, u)
+    # beside sequences whose rows are sound
+    target = torch.stack([p, p, bad, p, p]).to(dtype)
+    args = [target, torch.stack([p, q]).to(dtype), i32(x, x), i32(0, 1, 2, 2), torch.tensor([.9, .0]), torch.tensor([.3, .6, .8])]
+    want, got = ref.verify_chains(*args), ops.verify_chains(*[a.cuda() for a in args])
+    assert [t.tolist() for t in got] == [t.tolist() for t in want] and want[0].tolist() == [1, 0, 0] and want[1].tolist()[1] == -1
+
+
