@@ -272,9 +272,12 @@ __global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResiden
   }
 }
 
-// 2^(t / 512) for t from -512,000 to 0: t = n + r, a table of 2^(j/512) and the series of 2^(r/512) to the second power, |r| <= 1/2
+// 2^(t / 512) for t from -512 * 1000 to 0 (results stay above the smallest normal number, 2^-1022): t = n + r, a table of 2^(j/512) and the series of 2^(r/512) to the second power, |r| <= 1/2
 // (P. Tang's table-driven scheme): relative error below 6e-11, of either sign.
 constexpr int kExpTable = 512;
+// Probabilities are cut at 2^-900 of the most likely one's: divided by a sum of up to 2^28 terms they stay in the table's domain, and that many of them
+// add up to less than 2^-860, below which a sum counts as zero.
+constexpr double kCut = -900.0 * kExpTable, kNoSum = 0x1p-860;
 JS_DEVICE double exp2_table(double t, const double* table) {
   constexpr double kRound = 6755399441055744.0;              // 1.5 * 2^52: the integer part of the sum's low word
   constexpr double c1 = 0.69314718055994531 / kExpTable;
@@ -323,9 +326,8 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
   const int skip = point ? d_at : -1;
   const double ts = kExpTable * 1.4426950408889634 / tt, ds = kExpTable * 1.4426950408889634 / td;
   double tc = -tstat.x * ts, dc = both ? -dstat.x * ds : 0.0;
-  // logits below these have a probability under 2^-1000; they are cut there, and sums too small for any other count as zero
-  const float t_least = fmaxf(static_cast<float>((-1000.0 * kExpTable - tc) / ts), -3.4e38f);
-  const float d_least = fmaxf(static_cast<float>((-1000.0 * kExpTable - dc) / ds), -3.4e38f);
+  const float t_least = fmaxf(static_cast<float>((kCut - tc) / ts), -3.4e38f);      // logits below these are cut
+  const float d_least = fmaxf(static_cast<float>((kCut - dc) / ds), -3.4e38f);
   auto ep = [&](float v) { return exp2_table(fma(static_cast<double>(fmaxf(v, t_least)), ts, tc), table); };
   auto eq = [&](float v) { return exp2_table(fma(static_cast<double>(fmaxf(v, d_least)), ds, dc), table); };
   // A CTA takes a slice of the vocabulary and a warp a slice of that, so sums follow the order of the indices.
@@ -352,7 +354,7 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
   auto block_sum = [&](double v, double* to) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (lane == 0) to[warp] = v > 1e-290 ? v : 0.0;      // (2^-963)
+    if (lane == 0) to[warp] = v > kNoSum ? v : 0.0;
     __syncthreads();
     v = 0.0;
     for (int w = 0; w < kWarps; ++w) v += to[w];

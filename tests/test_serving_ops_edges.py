@@ -59,3 +59,22 @@ def test_verify_chains_kernel_of_rows_that_are_not_numbers(clean, V, dtype):
     assert [t.tolist() for t in got] == [t.tolist() for t in want] and want[0].tolist() == [1, 0, 0] and want[1].tolist()[1] == -1
 
 
+@gpu
+def test_verify_chains_kernel_of_a_vocabulary_of_millions(clean):
+    """Sums beyond 2^24 beside masked entries: what is left of ``p - q`` are the two tokens that only the draft masked."""
+    V = 2 ** 24 + 19
+    target, draft = torch.zeros(2, V, device="cuda"), torch.zeros(1, V, device="cuda")
+    target[0, 11], target[0, 12] = -INF, -INF
+    draft[0, 5], draft[0, 9] = -INF, -INF
+    for v, want in ((0.0, 5), (0.49, 5), (0.51, 9)):
+        accepted, token = ops.verify_chains(target, draft, i32(11, device="cuda"), i32(0, 1, device="cuda"), torch.tensor([0.5], device="cuda"),
+                                            torch.tensor([v], device="cuda"))
+        assert (accepted.tolist(), token.tolist()) == ([0], [want])
+    for v in (0.0, 0.25, 0.999):      # behind an accepted draft: the last row, all alike
+        accepted, token = ops.verify_chains(target, draft, i32(7, device="cuda"), i32(0, 1, device="cuda"), torch.tensor([0.5], device="cuda"),
+                                            torch.tensor([v], device="cuda"))
+        v32 = float(torch.tensor(v))
+        # the running sum is off by 6e-11 of itself at most, 0.001 of a token here
+        assert accepted.tolist() == [1] and abs(int(token) - int(v32 * V)) <= 1
+
+
