@@ -59,7 +59,8 @@ JS_DEVICE float chain_f<float>(float v) { return v; }
 template <>
 JS_DEVICE float chain_f<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
-JS_DEVICE double chain_temp(const float* each, double all, int b) { return each != nullptr ? each[b] : all; }
+constexpr double kLog2e = 1.4426950408889634, kHottest = 1e30;      // temperatures end there
+JS_DEVICE double chain_temp(const float* each, double all, int b) { return fmin(each != nullptr ? each[b] : all, kHottest); }
 
 // drafts of sequence b: first and number (bad offsets are cut to what is there)
 JS_DEVICE int chain_span(const ChainParams& p, int b, int& first) {
@@ -67,10 +68,10 @@ JS_DEVICE int chain_span(const ChainParams& p, int b, int& first) {
   return max(0, min(p.cu[b + 1], p.D) - first);
 }
 
-// log2(e) / T.  Its rounding to fp32 is a change of the temperature by about 2^-23 of itself, for the sum and the drafted token alike.
-JS_DEVICE float chain_scale(double temp) { return temp < kGreedyBelow ? 1.f : 1.44269504f / static_cast<float>(temp); }
-// What a row's exponents are relative to: its maximum in the log2 domain, rounded the same way wherever it is needed.
-JS_DEVICE float chain_base(float m, float scale) { return __fmul_rn(m, scale); }
+// log2(e) / T.  Exponents of a row's sum are (x - maximum) * scale, subtracted first: so nothing overflows, and a row that a large finite mask
+// fills says what it says (one operation a value more than a rounded base costs 64 sequences 2 of 149 us).  An exponent of -e bits is off by 4 e 2^-24
+// at most: half a step each for T, the scale, the difference and the product.
+JS_DEVICE float chain_scale(double temp) { return temp < kGreedyBelow ? 1.f : static_cast<float>(kLog2e) / static_cast<float>(temp); }
 JS_DEVICE float chain_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -87,9 +88,8 @@ JS_DEVICE RowStat join(const RowStat& a, const RowStat& b, float scale) {
   RowStat r;
   r.m = chain_max(a.m, b.m);
   r.at = a.m > b.m ? a.at : b.m > a.m ? b.at : min(a.at, b.at);
-  const float base = chain_base(r.m, scale);
-  r.s = (a.m == r.m ? a.s : a.s != 0.f ? a.s * chain_exp2(chain_base(a.m, scale) - base) : 0.f) +
-        (b.m == r.m ? b.s : b.s != 0.f ? b.s * chain_exp2(chain_base(b.m, scale) - base) : 0.f);
+  r.s = (a.m == r.m ? a.s : a.s != 0.f ? a.s * chain_exp2((a.m - r.m) * scale) : 0.f) +
+        (b.m == r.m ? b.s : b.s != 0.f ? b.s * chain_exp2((b.m - r.m) * scale) : 0.f);
   return r;
 }
 JS_DEVICE RowStat warp_join(RowStat r, float scale) {
@@ -104,8 +104,7 @@ JS_DEVICE RowStat warp_join(RowStat r, float scale) {
 // probability of the element at `index`, whose logit is `x`
 JS_DEVICE double chain_prob(float x, int index, double temp, const RowStat& st) {
   if (temp < kGreedyBelow) return index == st.at ? 1.0 : 0.0;
-  const float scale = chain_scale(temp);
-  return st.s != 0.f ? exp2(static_cast<double>(x) * scale - chain_base(st.m, scale)) / st.s : 0.0;      // NaN beside a logit of +inf
+  return st.s != 0.f ? exp2((static_cast<double>(x) - st.m) * (kLog2e / temp)) / st.s : 0.0;      // NaN beside a logit of +inf
 }
 
 // A row as the 16-byte blocks that hold it: a copy starts and ends with a block, and never leaves the blocks that the row has a part in.
@@ -211,12 +210,11 @@ __global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResiden
       tops2[row] = top;
       float sum = 0.f;
       if (top != -INFINITY) {
-        const float base = -chain_base(top, scales[row]);
         float e[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int q = 0; q < kStatBlocks; ++q)
 #pragma unroll
-          for (int c = 0; c < N; ++c) e[c & 3] += chain_exp2(fmaf(value(row, q, c), scales[row], base));
+          for (int c = 0; c < N; ++c) e[c & 3] += chain_exp2((value(row, q, c) - top) * scales[row]);
         sum = (e[0] + e[1]) + (e[2] + e[3]);
         if (temps[row] < kGreedyBelow) {       // only a point mass wants to know where the maximum is
 #pragma unroll
@@ -272,12 +270,12 @@ __global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResiden
   }
 }
 
-// 2^(t / 512) for t from -512 * 1000 to 0 (results stay above the smallest normal number, 2^-1022): t = n + r, a table of 2^(j/512) and the series of 2^(r/512) to the second power, |r| <= 1/2
+// 2^(t / 512) for t from -512 * 1020 to 0 (results stay above the smallest normal number, 2^-1022): t = n + r, a table of 2^(j/512) and the series of 2^(r/512) to the second power, |r| <= 1/2
 // (P. Tang's table-driven scheme): relative error below 6e-11, of either sign.
 constexpr int kExpTable = 512;
-// Probabilities are cut at 2^-900 of the most likely one's: divided by a sum of up to 2^28 terms they stay in the table's domain, and that many of them
-// add up to less than 2^-860, below which a sum counts as zero.
-constexpr double kCut = -900.0 * kExpTable, kNoSum = 0x1p-860;
+// Probabilities are cut below 2^-890 of the most likely one's, and count there as something from 2^-990 to 2^-890: divided by a sum of up to 2^28
+// terms they stay in the table's domain, and that many of them add up to less than 2^-860, below which a sum counts as zero.
+constexpr double kCut = -890.0 * kExpTable, kNoSum = 0x1p-860;
 JS_DEVICE double exp2_table(double t, const double* table) {
   constexpr double kRound = 6755399441055744.0;              // 1.5 * 2^52: the integer part of the sum's low word
   constexpr double c1 = 0.69314718055994531 / kExpTable;
@@ -287,6 +285,19 @@ JS_DEVICE double exp2_table(double t, const double* table) {
   const double e = fma(r, fma(r, c1 * c1 / 2.0, c1), 1.0) * table[n & (kExpTable - 1)];
   return __hiloint2double(__double2hiint(e) + ((n >> 9) << 20), __double2loint(e));
 }
+
+// Table steps a logit, and half the logit at which a row is cut, rounded down (logits are halved, so that the cut of any finite maximum is finite and
+// -inf lies below it).  Where the next value below the maximum has 2^-100 of its probability or less, that is as good as nothing: the slope stops
+// there, so that rounding takes the cut down by 2^-100 at most.
+struct ChainAxis {
+  double slope;
+  float least;
+  JS_DEVICE ChainAxis(float top, double temp) {
+    const double step = top == -3.402823466e38f ? 0x1p104 : static_cast<double>(top) - nextafterf(top, -INFINITY);
+    slope = fmin(kExpTable * kLog2e / temp, 100.0 * kExpTable / step);
+    least = __double2float_rd(0.5 * (top + kCut / slope));
+  }
+};
 
 // CLUSTER CTAs share a sequence's last row.
 template <typename T, int CLUSTER>
@@ -324,12 +335,10 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
   // (p <= 1) and nothing elsewhere.
   const bool point = left && td < kGreedyBelow, both = left && !point && dstat.x != -INFINITY;
   const int skip = point ? d_at : -1;
-  const double ts = kExpTable * 1.4426950408889634 / tt, ds = kExpTable * 1.4426950408889634 / td;
-  double tc = -tstat.x * ts, dc = both ? -dstat.x * ds : 0.0;
-  const float t_least = fmaxf(static_cast<float>((kCut - tc) / ts), -3.4e38f);      // logits below these are cut
-  const float d_least = fmaxf(static_cast<float>((kCut - dc) / ds), -3.4e38f);
-  auto ep = [&](float v) { return exp2_table(fma(static_cast<double>(fmaxf(v, t_least)), ts, tc), table); };
-  auto eq = [&](float v) { return exp2_table(fma(static_cast<double>(fmaxf(v, d_least)), ds, dc), table); };
+  const ChainAxis ta(tstat.x, tt), da(both ? dstat.x : 0.f, td);
+  double tc = -tstat.x * ta.slope, dc = both ? -dstat.x * da.slope : 0.0;
+  auto ep = [&](float v) { return exp2_table(fma(static_cast<double>(fmaxf(0.5f * v, ta.least)), 2.0 * ta.slope, tc), table); };
+  auto eq = [&](float v) { return exp2_table(fma(static_cast<double>(fmaxf(0.5f * v, da.least)), 2.0 * da.slope, dc), table); };
   // A CTA takes a slice of the vocabulary and a warp a slice of that, so sums follow the order of the indices.
   const int lo = static_cast<long long>(p.V) * rank / CLUSTER, size = static_cast<int>(static_cast<long long>(p.V) * (rank + 1) / CLUSTER) - lo;
   auto warp_lo = [&](int w) { return lo + static_cast<int>(static_cast<long long>(size) * w / kWarps); };
@@ -394,7 +403,7 @@ __global__ void __launch_bounds__(kChainThreads, 2) chain_token_kernel(ChainPara
   }
   auto weight = [&](int i) {
     const float v = chain_f(x[i]);
-    if (!(v > t_least) || i == skip) return 0.0;
+    if (!(0.5f * v > ta.least) || i == skip) return 0.0;
     return both ? fmax(ep(v) - eq(chain_f(y[i])), 0.0) : ep(v);
   };
   sum = block_sum(sum, part);

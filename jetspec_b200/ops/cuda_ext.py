@@ -1604,8 +1604,8 @@ def _temperatures(t, B: int, index: int, name: str) -> tuple:
         if t.dtype is not torch.float32 or t.get_device() != index or not t.is_contiguous() or t.numel() != B:
             _refuse(f"{name}: expected a number or {B} fp32 values on device {index}")
         return t.data_ptr(), 0.0
-    if not 0.0 <= t < math.inf:
-        _refuse(f"{name}={t}")
+    if not 0.0 <= t <= 1e30:
+        _refuse(f"{name}={t}: expected a number from 0 to 1e30")
     return 0, t
 
 

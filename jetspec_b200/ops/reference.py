@@ -370,7 +370,7 @@ def verify_chains(target_logits: torch.Tensor, draft_logits: torch.Tensor, draft
     before it were and ``accept_u[i] * q_i(x_i) < p_i(x_i)``.  The next token is drawn by inverse CDF with ``sample_u[b]``: from
     the last row when every draft was accepted, else from ``max(p - q, 0)`` at the first one that was not; the tokens kept are
     then distributed like the target's own.  ``temperature`` and ``draft_temperature`` (default: the same) are numbers or ``(B,)``
-    tensors; below 1e-5 they mean the lowest most likely token.  The rows of a sequence behind its first rejection do not matter.
+    tensors, from 0 to 1e30; below 1e-5 they mean the lowest most likely token.  The rows of a sequence behind its first rejection do not matter.
 
     A target row without any logit above -inf, or with a NaN, accepts nothing; its next token is -1.  Such a draft row says nothing:
     what the target can say at all is accepted.  Where rounding leaves nothing of ``max(p - q, 0)`` the target's most likely token

@@ -78,3 +78,55 @@ def test_verify_chains_kernel_of_a_vocabulary_of_millions(clean):
         assert accepted.tolist() == [1] and abs(int(token) - int(v32 * V)) <= 1
 
 
+LOWEST = torch.finfo(torch.float32).min
+
+
+def large_rows(V, g):
+    """Rows of values far from zero, and the temperatures at which they say something."""
+    flat = lambda v: torch.full((V,), v)
+    some = torch.rand(V, generator=g) < 0.3
+    some[:2] = torch.tensor([True, False])
+    near = flat(2e5)
+    near[~some] = float(torch.nextafter(torch.tensor(2e5), torch.tensor(0.0)))
+    step = flat(-1e9)
+    step[~some] = -1e9 - 64
+    usual = torch.randn(V, generator=g) * 3
+    return [(flat(-1e9), 0.2), (flat(-1e9), 1.0), (step, 37.0), (flat(-1e30), 1.0), (flat(-1e30).masked_fill(some, -2e30), 0.7),
+            (flat(1e30).masked_fill(some, 0.0), 1.0), (flat(LOWEST), 1.0), (flat(LOWEST), 0.01), (flat(LOWEST).masked_fill(some, -INF), 1.0),
+            (flat(LOWEST).masked_fill(some, -INF), 1e30), (usual.masked_fill(some, LOWEST), 0.8), (usual.masked_fill(some, -1e9), 0.8),
+            (near, 2e-5), (near, 0.01), (usual * 1000, 2e-5), (usual.masked_fill(some, -INF), 1e30), (flat(-LOWEST).masked_fill(some, LOWEST), 0.5),
+            (usual * 1e29, 1e29)]
+
+
+@gpu
+@pytest.mark.parametrize("V,dtype", [(1003, torch.float32), (20001, torch.bfloat16)])
+def test_verify_chains_kernel_of_large_values(clean, V, dtype):
+    """Rows that a finite mask fills, neighbours among large values, temperatures at both ends."""
+    g = torch.Generator().manual_seed(V)
+    usual = torch.randn(V, generator=g)
+    for number, (row, hot) in enumerate(large_rows(V, g)):
+        row = row.to(dtype).float()
+        if dtype == torch.bfloat16:
+            row = row.clamp(torch.finfo(dtype).min, torch.finfo(dtype).max)      # the type's own extremes
+        x = int(row.argmax())
+        for v in (0.0, 0.3, 0.77):
+            for kw in (dict(temperature=hot), dict(temperature=torch.tensor([hot]))):
+                gpu_kw = lambda d: {k: t.cuda() if torch.is_tensor(t) else t for k, t in d.items()}
+                args = [row[None].to(dtype), row[None][:0].to(dtype), i32(), i32(0, 0), torch.zeros(0), torch.tensor([v])]
+                assert int(ops.verify_chains(*[a.cuda() for a in args], **gpu_kw(kw))[1]) == int(ref.verify_chains(*args, **kw)[1]), (number, v)
+            for u in (0.3, 0.7):
+                for target, draft, kw in (([row, row], [row], dict(temperature=hot)), ([usual, row], [row], dict(temperature=1.0, draft_temperature=hot)),
+                                          ([row, usual], [usual], dict(temperature=hot, draft_temperature=1.0))):
+                    want, got = one_chain(target, draft, [x], [u], v, dtype, **kw)
+                    assert got == want, (number, u, v, kw)
+
+
+def test_verify_chains_refuses_temperatures_without_bounds():
+    from jetspec_b200.ops import cuda_ext
+    row = torch.zeros(1, 4)
+    call = lambda **kw: cuda_ext.verify_chains(row, row[:0], i32(), i32(0, 0), torch.zeros(0), torch.zeros(1), **kw)
+    for t in (1.1e30, INF, NAN, -1.0):
+        kernel_refuses(lambda: call(temperature=t), "temperature")
+        kernel_refuses(lambda: call(draft_temperature=t), "draft_temperature")
+
+
