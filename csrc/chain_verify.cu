@@ -32,7 +32,7 @@ template <>
 struct StatShape<float> { static constexpr int kThreads = 128, kResident = 6; };
 constexpr int kAhead = 8;            // drafts of a sequence that blocks of their own read
 constexpr int kChainThreads = 512;
-constexpr float kGreedyBelow = 1e-5f;
+constexpr double kGreedyBelow = 1e-5;      // fp32 1e-5 lies below it
 constexpr int kNoneRejected = 0x7fffffff;
 
 struct ChainParams {
@@ -69,8 +69,8 @@ JS_DEVICE int chain_span(const ChainParams& p, int b, int& first) {
 }
 
 // log2(e) / T.  Exponents of a row's sum are (x - maximum) * scale, subtracted first: so nothing overflows, and a row that a large finite mask
-// fills says what it says (one operation a value more than a rounded base costs 64 sequences 2 of 149 us).  An exponent of -e bits is off by 4 e 2^-24
-// at most: half a step each for T, the scale, the difference and the product.
+// fills says what it says (one operation a value more than a rounded base costs 64 sequences 2 of 149 us).  An exponent of -e bits is off by 5 e 2^-24
+// at most: half a step each for T, log2(e), their quotient, the difference and the product.
 JS_DEVICE float chain_scale(double temp) { return temp < kGreedyBelow ? 1.f : static_cast<float>(kLog2e) / static_cast<float>(temp); }
 JS_DEVICE float chain_exp2(float x) {
   float y;

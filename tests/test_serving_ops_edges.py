@@ -130,3 +130,20 @@ def test_verify_chains_refuses_temperatures_without_bounds():
         kernel_refuses(lambda: call(draft_temperature=t), "draft_temperature")
 
 
+def greedy_threshold(device):
+    """1e-5 in fp32 lies below 1e-5: the lowest most likely token, although half of the probability is at the next one."""
+    row = torch.tensor([[-INF, 0.0, 0.0]], device=device)
+    accepted, token = ops.verify_chains(row, row[:0], i32(device=device), i32(0, 0, device=device), torch.zeros(0, device=device),
+                                        torch.tensor([0.75], device=device), temperature=torch.tensor([1e-5], device=device))
+    assert accepted.tolist() == [0] and token.tolist() == [1]
+
+
+def test_verify_chains_greedy_threshold():
+    greedy_threshold("cpu")
+
+
+@gpu
+def test_verify_chains_kernel_greedy_threshold(clean):
+    greedy_threshold("cuda")
+
+
