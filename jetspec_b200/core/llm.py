@@ -139,7 +139,9 @@ class LLM:
                 n = drafts.numel()
                 kept, nxt = ops.verify_chains(logits[0], draft_logits, drafts.to(torch.int32), torch.tensor([0, n], dtype=torch.int32, device=self.device),
                                               torch.rand(n, device=self.device), torch.rand(1, device=self.device), temperature=sp.temperature)
-                acc = int(kept)
+                acc, token = torch.cat((kept.to(nxt.dtype), nxt)).tolist()
+                if token < 0:
+                    raise RuntimeError(f"generate_chain: the target gave no logit above -inf, or a NaN, at position {past + 1 + acc}")
             else:
                 greedy = logits[0].argmax(-1)
                 agree = (drafts == greedy[:k]).to(torch.int64)

@@ -147,3 +147,27 @@ def test_verify_chains_kernel_greedy_threshold(clean):
     greedy_threshold("cuda")
 
 
+@pytest.mark.parametrize("value", [-INF, NAN])
+def test_generate_chain_of_a_target_that_says_nothing(monkeypatch, value):
+    """Logits without a number among them end the generation with an error, and no -1 is fed to the model."""
+    from jetspec_b200 import LLM, SamplingParams
+    from jetspec_b200.models import Qwen3ForCausalLM, tiny_config
+    llm = LLM(Qwen3ForCausalLM.random_init(tiny_config(), seed=0, dtype=torch.float32), device="cpu", dtype=torch.float32)
+    fed, forward = [], llm.runner.forward
+
+    def silent(ids, cache, **kw):
+        fed.append(ids)
+        logits, cache, hidden = forward(ids, cache, **kw)
+        return (logits if len(fed) == 1 else torch.full_like(logits, value)), cache, hidden
+
+    class Drafts:
+        def propose_sampled(self, context_ids, k, temperature, target_hidden=None):
+            return torch.arange(k), torch.zeros(k, 1024)
+
+    monkeypatch.setattr(llm.runner, "forward", silent)
+    torch.manual_seed(0)
+    with pytest.raises(RuntimeError, match="logit"):
+        llm.generate_chain(torch.arange(1, 8).view(1, -1), Drafts(), block_size=4, sampling_params=SamplingParams(0.8, 20))
+    assert len(fed) == 2 and all(int(ids.min()) >= 0 for ids in fed)
+
+
