@@ -879,7 +879,7 @@ extern "C" long long js_shared_attention_ws(int B, int T, int Hq, int Hkv, int m
 
 // q (T, Hq, 128) bf16, ldq elements between tokens; pools (Hkv, S, 128); slot_map (max_seqs, max_len); seq_rows, past_lens (B); cu_q (B + 1);
 // mask_bits (T, W), or null when causal; out (T, Hq * 128).  Positions [0, prefix_len) hold the same slots in all rows of the slot map that
-// are named; max_q bounds a sequence's rows.  ws: js_shared_attention_ws bytes.
+// are named; max_q bounds a sequence's rows.  ws: js_shared_attention_ws bytes.  q and the pools on 16-byte boundaries, out and ws on 32.
 extern "C" int js_shared_attention(const void* q, long long ldq, const void* k_pool, const void* v_pool, const int* slot_map, const int* seq_rows,
                                    const int* cu_q, const int* past_lens, const int* mask_bits, void* out, void* ws, long long ws_bytes,
                                    int* status, int B, int T, int Hq, int Hkv, int S, int max_seqs, int max_len, int W, int causal, float scale,
@@ -889,7 +889,9 @@ extern "C" int js_shared_attention(const void* q, long long ldq, const void* k_p
   SharedAttn p{};
   p.B = B; p.T = T; p.Hq = Hq; p.Hkv = Hkv; p.max_len = max_len;
   if (const int rc = shared_setup(&p, max_q, prefix_len, ctas)) return rc;
-  if (ldq % 8 || (reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(out) & 15)) return -12;
+  // copies start on 16-byte boundaries, results and parts leave 32 bytes at a time
+  if (ldq % 8 || ((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pool) | reinterpret_cast<uintptr_t>(v_pool)) & 15) ||
+      ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(ws)) & 31)) return -12;
   if (!causal && (mask_bits == nullptr || W < 1)) return -13;
   if (!(scale > 0.f) || S < 1 || max_seqs < 1) return -10;
   if (shared_layout(&p, reinterpret_cast<uint8_t*>(ws), max_q) > ws_bytes) return -14;

@@ -171,3 +171,20 @@ def test_generate_chain_of_a_target_that_says_nothing(monkeypatch, value):
     assert len(fed) == 2 and all(int(ids.min()) >= 0 for ids in fed)
 
 
+# ------------------------------------------------------------------ attention behind a shared prefix
+@pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of nothing: not where a mistake would launch a kernel on them")
+def test_shared_attention_entry_refuses_addresses():
+    """Results leave in stores of 32 bytes, keys and queries come in 16: the entry point turns other addresses down before it starts anything."""
+    from jetspec_b200.ops import cuda_ext
+    need = cuda_ext.shared_prefix_workspace(1, 2, 2, 1, 64, 0, 2)
+    entry = cuda_ext._entry("js_shared_attention", "plppppppppplpiiiiiiiiifiiip")
+    sound = dict(q=4096, k=4096, v=4096, out=4096, ws=4096)
+
+    def rc(**kw):
+        a = {**sound, **kw}
+        return entry(a["q"], 256, a["k"], a["v"], 4096, 4096, 4096, 4096, 0, a["out"], a["ws"], need, 4096, 1, 2, 2, 1, 64, 1, 64, 0, 1, 1.0, 0, 2,
+                     cuda_ext.SM_COUNT, None)
+
+    assert rc(out=4096 + 16) == rc(out=4096 + 8) == rc(ws=4096 + 16) == rc(q=4096 + 8) == rc(k=4096 + 8) == rc(v=4096 + 2) == -12
+
+
