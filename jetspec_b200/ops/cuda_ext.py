@@ -1520,6 +1520,8 @@ def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_le
     if (k_pool.dim() != 3 or k_pool.shape != v_pool.shape or k_pool.shape[2] != 128 or k_pool.dtype is not bf16 or v_pool.dtype is not bf16
             or not k_pool.is_contiguous() or not v_pool.is_contiguous() or k_pool.get_device() != index or v_pool.get_device() != index):
         _refuse("pools: expected contiguous bf16 (Hkv, S, 128) tensors on the queries' device")
+    if (k_pool.data_ptr() | v_pool.data_ptr()) % 16:
+        _refuse("pools: expected to start at multiples of 16 bytes")
     Hkv, S, _ = k_pool.shape
     if Hkv < 1 or S < 1 or Hq < 1 or Hq % Hkv or Hq // Hkv > 128 or Hkv * S >= 2 ** 31:
         _refuse(f"{Hq} query and {Hkv} KV heads over {S} slots")
@@ -1536,8 +1538,9 @@ def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_le
     if not (0 <= prefix_len <= max_len and max_q >= 0 and 0.0 < scale < math.inf):
         _refuse(f"prefix_len={prefix_len} of {max_len}, max_q={max_q}, scale={scale}")
     max_q = max(max_q, 1)
-    if q.stride(2) != 1 or q.stride(1) != 128 or q.stride(0) % 8 or q.stride(0) < Hq * 128 or q.data_ptr() % 16:
-        q = q.contiguous()
+    ldq = q.stride(0) if T > 1 else Hq * 128      # one token: its stride says nothing
+    if q.stride(2) != 1 or q.stride(1) != 128 or ldq % 8 or ldq < Hq * 128 or q.data_ptr() % 16:
+        q, ldq = q.clone(memory_format=torch.contiguous_format), Hq * 128      # also off its boundary, where contiguous() changes nothing
     if out is None:
         out = torch.empty(T, Hq * 128, dtype=bf16, device=q.device)
     elif out.shape != (T, Hq * 128) or out.dtype is not bf16 or not out.is_contiguous() or out.get_device() != index or out.data_ptr() % 32:
@@ -1550,7 +1553,7 @@ def shared_prefix_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_le
     elif ws.dtype is not torch.uint8 or not ws.is_contiguous() or ws.get_device() != index or ws.numel() < need or ws.data_ptr() % 32:
         _refuse(f"ws: expected {need} contiguous bytes on the queries' device")
     rc = _entry("js_shared_attention", "plppppppppplpiiiiiiiiifiiip")(
-        q.data_ptr(), q.stride(0), k_pool.data_ptr(), v_pool.data_ptr(), slot_map.data_ptr(), seq_rows.data_ptr(), cu_q.data_ptr(),
+        q.data_ptr(), ldq, k_pool.data_ptr(), v_pool.data_ptr(), slot_map.data_ptr(), seq_rows.data_ptr(), cu_q.data_ptr(),
         past_lens.data_ptr(), bits, out.data_ptr(), ws.data_ptr(), ws.numel(), _status_at(index), B, T, Hq, Hkv, S, max_seqs, max_len, words,
         1 if causal else 0, scale, prefix_len, max_q, SM_COUNT, _stream_at(index))
     if rc:

@@ -188,3 +188,28 @@ def test_shared_attention_entry_refuses_addresses():
     assert rc(out=4096 + 16) == rc(out=4096 + 8) == rc(ws=4096 + 16) == rc(q=4096 + 8) == rc(k=4096 + 8) == rc(v=4096 + 2) == -12
 
 
+@gpu
+def test_shared_prefix_attention_of_views_at_odd_addresses(clean):
+    """Queries that start off a 16-byte boundary, one token whose stride says nothing, pools that no copy can read."""
+    c = attention_case(3, 8, 2, 70, [0, 9], [2, 3], True, device="cuda")
+    want = attention_exact(c)
+    flat = torch.zeros(c["q"].numel() + 8, dtype=torch.bfloat16, device="cuda")
+    for shift in (1, 4):
+        q = flat[shift:shift + c["q"].numel()].view(c["q"].shape)
+        q.copy_(c["q"])
+        attention_close(attend({**c, "q": q}), want)
+    one = attention_case(4, 8, 2, 70, [5], [1], True, device="cuda")
+    want = attention_exact(one)
+    for stride in (0, 5, 1027, 8 * 128 + 4):
+        q = one["q"].as_strided((1, 8, 128), (stride, 128, 1))
+        attention_close(attend({**one, "q": q}), want)
+
+
+def test_shared_prefix_attention_refuses_pools_off_their_boundary():
+    from jetspec_b200.ops import cuda_ext
+    c = attention_case(0, 4, 2, 20, [0, 5], [4, 3], False)
+    for name in ("k_pool", "v_pool"):
+        odd = torch.zeros(c[name].numel() + 1, dtype=torch.bfloat16)[1:].view(c[name].shape)
+        kernel_refuses(lambda: cuda_ext.shared_prefix_attention(**{**c, "max_q": 4, name: odd}), "16 bytes")
+
+
