@@ -317,6 +317,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
   for (int b = tid; blockIdx.x == 0 && b < p.B; b += STHREADS) {
     const SaSeq s = sa_seq(p, b);
     if (s.n > 0 && s.past < p.prefix) report(p.status, kShortPrefix);
+    const int past = p.past_lens[b];           // s.past is cut to the slot map's columns: a sequence that does not fit in them loses keys
+    if (s.n > 0 && (past < 0 || past > p.max_len - s.n)) report(p.status, kBadSlot);
   }
   const int mine = tid < p.B ? sa_total(p, tid) * p.Hkv : 0;
   int total;

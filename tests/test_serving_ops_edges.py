@@ -213,3 +213,25 @@ def test_shared_prefix_attention_refuses_pools_off_their_boundary():
         kernel_refuses(lambda: cuda_ext.shared_prefix_attention(**{**c, "max_q": 4, name: odd}), "16 bytes")
 
 
+@gpu
+def test_shared_prefix_attention_reports_rows_past_the_slot_map(clean):
+    """Positions that the slot map has no columns for, and lengths below zero: reported, as slot planning does."""
+    for past in (0, 1):                   # with a prefix of its own, and without
+        c = attention_case(6, 8, 2, 64 * (1 - past), [0, 7, 0, 3], [1, 1, 1, 1], True, device="cuda")
+        most = c["slot_map"].shape[1]
+        attend({**c, "past_lens": c["past_lens"] * 0 + most - 1})
+        clean.check_status("cuda")
+        for lens in ((most, most - 1, most - 1, most - 1), (most - 1, most - 1, most - 1, most + 5), (most - 1, 2 ** 31 - 1, most - 1, most - 1)):
+            attend({**c, "past_lens": i32(*lens, device="cuda")})
+            with pytest.raises(RuntimeError, match="slot"):
+                clean.check_status("cuda")
+    c = attention_case(6, 8, 2, 0, [0, 7], [1, 1], True, device="cuda")
+    attend({**c, "past_lens": i32(-1, 7, device="cuda")})
+    with pytest.raises(RuntimeError, match="slot"):
+        clean.check_status("cuda")
+    # a sequence without rows has no positions: whatever its length says
+    c = attention_case(6, 8, 2, 64, [0, 7, 0], [1, 0, 1], True, device="cuda")
+    want = attention_exact(c)
+    attention_close(attend({**c, "past_lens": torch.where(i32(0, 1, 0, device="cuda") > 0, 10 ** 6, c["past_lens"]).to(I32)}), want)
+
+
