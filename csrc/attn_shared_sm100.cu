@@ -77,7 +77,7 @@ JS_DEVICE SaSeq sa_seq(const SharedAttn& p, int b) {
     s.n = max(0, min(p.cu_q[p.B], p.T));
     s.past = s.end = p.prefix;
     s.first = 0;
-    s.row = p.seq_rows[0];
+    s.row = 0;                 // sa_prefix_row says
   } else {
     s.q_begin = min(max(0, p.cu_q[b]), p.T);
     s.n = max(0, min(p.cu_q[b + 1], p.T) - s.q_begin);
@@ -87,6 +87,15 @@ JS_DEVICE SaSeq sa_seq(const SharedAttn& p, int b) {
     s.row = p.seq_rows[b];
   }
   return s;
+}
+// The slot-map row that the prefix is read through: the first sequence's that has rows (others may have none any more).  A whole warp asks.
+JS_DEVICE int sa_prefix_row(const SharedAttn& p) {
+  const int lane = threadIdx.x & 31;
+  for (int base = 0; base < p.B; base += 32) {
+    const unsigned some = __ballot_sync(0xffffffffu, base + lane < p.B && sa_seq(p, base + lane).n > 0);
+    if (some != 0) return p.seq_rows[base + __ffs(some) - 1];
+  }
+  return -1;
 }
 // keys a pair of tiles sees end here
 JS_DEVICE int sa_end(const SharedAttn& p, const SaSeq& s, int b, int pair) {
@@ -396,6 +405,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       int token, h, sides;                      // a segment's first tile: its Q tiles (sides 0: another tile)
     };
     const int* slots = nullptr;
+    if (w.left > 0 && w.b < 0) w.s.row = sa_prefix_row(p);      // a walk that takes prefix items starts with them
     int at = 0;                                 // tile of the segment
     auto open = [&] {
       at = 0;

@@ -337,7 +337,7 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     """:func:`paged_tree_attention` of a batch whose sequences share their first ``prefix_len`` positions.
 
     Every ``past_lens[b] >= prefix_len``, and the rows ``seq_rows`` of the slot map hold the same slots up to there (the kernel reads the
-    prefix through the first of them).  Rows behind the last sequence (``cu_q[-1]`` and on) are zero.  ``scale`` is positive.  A sequence
+    prefix through the first sequence with rows of its own; of the others nothing is read).  Rows behind the last sequence (``cu_q[-1]`` and on) are zero.  ``scale`` is positive.  A sequence
     that is shorter than the prefix, or longer than a row of the slot map, is an error: the kernel sets the device's status word.
     """
     out = paged_tree_attention(q, k_pool, v_pool, slot_map, seq_rows, cu_q, past_lens, mask_bits, scale, causal)

@@ -235,3 +235,19 @@ def test_shared_prefix_attention_reports_rows_past_the_slot_map(clean):
     attention_close(attend({**c, "past_lens": torch.where(i32(0, 1, 0, device="cuda") > 0, 10 ** 6, c["past_lens"]).to(I32)}), want)
 
 
+@gpu
+@pytest.mark.parametrize("idle", [1, 3, 40])
+def test_shared_prefix_attention_behind_idle_sequences(clean, idle):
+    """A batch whose first sequences have no rows, and slot-map rows that are not theirs any more."""
+    c = attention_case(8, 8, 2, 200, [4, 0, 30], [1, 2, 1], True, device="cuda")
+    want = attention_exact(c)
+    n = c["cu_q"].numel() - 1
+    for row in (0, -1, 10 ** 6):          # slots outside the pool, and no row at all
+        rows = torch.cat((i32(*[row] * idle, device="cuda"), c["seq_rows"]))
+        cu = torch.cat((c["cu_q"].new_zeros(idle), c["cu_q"]))
+        past = torch.cat((c["past_lens"].new_zeros(idle), c["past_lens"]))
+        assert rows.numel() == n + idle
+        attention_close(attend({**c, "seq_rows": rows, "cu_q": cu, "past_lens": past}), want)
+        clean.check_status("cuda")
+
+
