@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(SlotPlan p) {
     plan_need(p, j, past, count, held, need);
     q += count;
     pages += need;
-    again |= p.rows[j] == row;
+    again |= p.rows[j] == row && (count > 0 || need > 0);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kPlanThreads) slot_plan_kernel(SlotPlan p) {
     if (b == p.B - 1) { p.cu_q[p.B] = capped_int(q + count); p.cu_pages[p.B] = capped_int(pages + need); }
   }
   const bool sound = row >= 0 && row < p.max_seqs && seen_row == 0;      // a slot-map row serves one request
-  if (b < p.B && !sound && first == 0) report(p.status, kBadSlot);
+  if (b < p.B && !sound && first == 0 && (count > 0 || need > 0)) report(p.status, kBadSlot);      // without rows and pages it only fills up a batch
   const unsigned page = p.page;
   // page `k` of the request's new ones
   auto granted = [&](unsigned k) {

@@ -420,7 +420,8 @@ def plan_slots(past_lens: torch.Tensor, counts: torch.Tensor, seq_rows: torch.Te
     Returns ``(cu_q (B + 1,), positions (rows,), slots (rows,), cu_pages (B + 1,))``, int32: offsets of the new rows, position and
     slot of each, and offsets of the pages taken (``cu_pages[-1]`` in all).  Rows behind the last request have position 0 and
     slot -1.  A slot is -1 too where the free pages ran out, a position is past the slot map, or a slot-map row is out of range or an
-    earlier request's; the kernel then also sets the device's status word (:func:`jetspec_b200.ops.cuda_ext.check_status`).
+    earlier request's; the kernel then also sets the device's status word (:func:`jetspec_b200.ops.cuda_ext.check_status`).  A request
+    that gets neither rows nor pages may name any row: batches are filled up with such.
     """
     B, (max_seqs, max_len), dev = past_lens.numel(), slot_map.shape, slot_map.device
     past, count = past_lens.long().clamp_min(0), counts.long().clamp_min(0)
@@ -429,7 +430,7 @@ def plan_slots(past_lens: torch.Tensor, counts: torch.Tensor, seq_rows: torch.Te
     offsets = lambda n: torch.cat((n.new_zeros(1), n.cumsum(0)))
     cu_q, cu_pages = offsets(count), offsets(need)
     row = seq_rows.long()
-    known = (row[:, None] == row[None, :]).tril(-1).any(1)
+    known = ((row[:, None] == row[None, :]) & ((count > 0) | (need > 0))).tril(-1).any(1)
     sound = (row >= 0) & (row < max_seqs) & ~known
     pages = torch.cat((free_pages.long(), free_pages.new_full((1,), -1).long()))
 

@@ -251,3 +251,33 @@ def test_shared_prefix_attention_behind_idle_sequences(clean, idle):
         clean.check_status("cuda")
 
 
+# ------------------------------------------------------------------ slot planning
+def padded_plan(device):
+    """Requests that fill a batch up: no rows, no pages, any slot-map row.  Nothing about them is wrong."""
+    t = lambda *v: i32(*v, device=device)
+    slot_map = torch.zeros(3, 32, dtype=I32, device=device)
+    cu_q, positions, slots, cu_pages = ops.plan_slots(t(8, 4, 8, 0, 0, 8), t(0, 1, 4, 0, 0, 0), t(2, 1, 2, -1, -1, 1), t(7, 9), 4, slot_map, 7)
+    assert cu_q.tolist() == [0, 0, 1, 5, 5, 5, 5] and cu_pages.tolist() == [0, 0, 1, 2, 2, 2, 2]
+    assert positions.tolist() == [4, 8, 9, 10, 11, 0, 0] and slots.tolist() == [28, 36, 37, 38, 39, -1, -1]
+
+
+def test_plan_slots_of_a_padded_batch():
+    padded_plan("cpu")
+
+
+@gpu
+def test_plan_slots_kernel_of_a_padded_batch(clean):
+    padded_plan("cuda")
+    clean.check_status("cuda")
+    e = i32(device="cuda")
+    ops.plan_slots(i32(4, 4, device="cuda"), i32(0, 4, device="cuda"), i32(9, 9, device="cuda"), i32(1, 2, device="cuda"), 4,
+                   torch.zeros(3, 32, dtype=I32, device="cuda"), 4, mapped_lens=i32(4, 8, device="cuda"))
+    with pytest.raises(RuntimeError, match="status 5"):      # rows there are, and their request's slot-map row is not
+        clean.check_status("cuda")
+    ops.plan_slots(i32(4, device="cuda"), i32(0, device="cuda"), i32(9, device="cuda"), i32(1, 2, device="cuda"), 4,
+                   torch.zeros(3, 32, dtype=I32, device="cuda"), 0, mapped_lens=i32(0, device="cuda"))
+    with pytest.raises(RuntimeError, match="status 5"):      # a page was granted, and its slots have nowhere to go
+        clean.check_status("cuda")
+    assert e.numel() == 0
+
+
