@@ -753,9 +753,10 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attn_shared_merge_kernel(con
   int c0 = 0, own = 0, item = 0, own_begin = 0;      // first CTA and number of CTAs with a part of the sequence's own keys
   if (units > 0) {
     item = sa_item(p, s, b, pair, h);
-    const int u = own_begin = p.plan[1 + item];
-    c0 = (u + kItemCost) / piece;
-    own = (u + kItemCost + ((units - 1) << two)) / piece - c0 + 1;
+    // On the line, whatever the plan says: a CTA that a wait ran out in leaves its items' places unwritten, and nothing is read past the parts.
+    const int u = own_begin = min(max(p.plan[1 + item], 0), p.ctas * piece - 1);
+    c0 = min((u + kItemCost) / piece, p.ctas - 1);
+    own = min((u + kItemCost + ((units - 1) << two)) / piece, p.ctas - 1) - c0 + 1;
     item -= p.prefix_items;
   }
   if (own == 1 && two && p.prefix == 0) return;       // written by its CTA

@@ -2,6 +2,8 @@
 addresses, padded batches, long items of attention, lengths past the slot map.
 """
 import math
+import random
+import re
 
 import pytest
 import torch
@@ -279,5 +281,38 @@ def test_plan_slots_kernel_of_a_padded_batch(clean):
     with pytest.raises(RuntimeError, match="status 5"):      # a page was granted, and its slots have nowhere to go
         clean.check_status("cuda")
     assert e.numel() == 0
+
+
+# ------------------------------------------------------------------ attention when a wait has run out: that cannot be staged on a GPU
+def shared_attention_source():
+    from jetspec_b200.ops import cuda_ext
+    source = next(s for s in cuda_ext.sources() if s.endswith("attn_shared_sm100.cu"))
+    return re.sub(r"//.*", "", open(source).read())
+
+
+def test_shared_attention_merge_stays_in_its_workspace():
+    """The merge finds a sequence's parts by where the plan says that its item begins, which a CTA whose wait ran out has not written.  Its
+    expressions, on any number: the CTAs are some that there are.  On places of a line as the plan has them, the bounds change nothing."""
+    text = shared_attention_source()
+    own = re.search(r"const int u = own_begin = (.*);\s*c0 = (.*);\s*own = (.*);", text).groups()
+    python = [re.sub(r"(?<!/)/(?!/)", "//", re.sub(r"p\.plan\[1 \+ item\]", "said", e)).replace("p.ctas", "ctas") for e in own]
+
+    def parts(said, piece, units, two, ctas=148, cost=8):
+        env = dict(said=said, piece=piece, units=units, two=two, ctas=ctas, kItemCost=cost, min=min, max=max)
+        for name, expression in zip(("u", "c0", "own"), python):
+            env[name] = eval(expression, env)
+            assert -2 ** 31 <= env[name] < 2 ** 31
+        return env["u"], env["c0"], env["own"]
+
+    rng = random.Random(0)
+    for _ in range(2000):
+        piece, units, two = rng.choice([1, 7, 900, 13_000_000]), rng.randint(1, 2000), rng.randint(0, 1)
+        u, c0, own = parts(rng.choice([-2 ** 31, -1, 2 ** 31 - 1, rng.randint(-2 ** 31, 2 ** 31 - 1)]), piece, units, two)
+        assert 0 <= c0 < 148 and 1 <= own <= 148 - c0
+        length = (units << two) + 8
+        if length <= 148 * piece:
+            begin = rng.randint(0, 148 * piece - length)
+            u, c0, own = parts(begin, piece, units, two)
+            assert (u, c0, own) == (begin, (begin + 8) // piece, (begin + 8 + ((units - 1) << two)) // piece - (begin + 8) // piece + 1)
 
 
