@@ -68,6 +68,13 @@ JS_DEVICE int sa_wait(uint64_t* bar, uint32_t parity, int* status, int code, uin
   return mbar_wait_warp(bar, parity, status, code, gave_up);
 }
 
+// The last uses of a ring of barriers: what a warp has started has ended before its CTA leaves, also where another wait ran out first.
+template <int SLOTS>
+JS_DEVICE void sa_settle(uint64_t* ring, int uses, int* status, int code) {
+#pragma unroll 1
+  for (int j = max(0, uses - SLOTS); j < uses; ++j) mbar_wait(&ring[j % SLOTS], (j / SLOTS) & 1, status, code);
+}
+
 // ---------------------------------------------------------------- the line of units
 struct SaSeq { int q_begin, n, past, first, end, row; };      // rows, committed keys, key range, slot-map row
 JS_DEVICE SaSeq sa_seq(const SharedAttn& p, int b) {
@@ -431,8 +438,8 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
     };
     Tile tile, next{};
     bool have = open(), more = have && ask(tile), ok = true;
-    int uses = 0;                               // Q buffers filled so far: buffer uses % 2
-    for (int n = 0; have; ++n) {
+    int uses = 0, n = 0;                        // Q buffers filled so far: buffer uses % 2; tiles issued
+    for (; have; ++n) {
       have = more;
       if (more) more = ask(next);
       for (int side = 0; values && side < tile.sides && ok; ++side, ++uses) {
@@ -502,6 +509,9 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       }
       tile = next;
     }
+    static_assert(KSLOTS == VSLOTS, "one ring size for both loaders");
+    sa_settle<KSLOTS>(values ? kv_full + KSLOTS : kv_full, n, p.status, kTimeoutFull);
+    if (values) sa_settle<2>(q_full, uses, p.status, kTimeoutFull);
   } else if (warp == 8) {
     // ================================================================ issuer of the first product: S = Q K^T of a job once the group's scores before it are read
     // (One warp for both products held the MMAs up: its waits take as long as they run.)
@@ -532,6 +542,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       use += sides;
       sa_done(w);
     }
+    sa_settle<2>(s_full, n, p.status, kTimeoutAccum);
   } else if (warp == 11) {
     // ================================================================ issuer of the second product: O += P V
     constexpr uint32_t idesc = umma_idesc_bf16(SROWS, SD) | (1u << 16);
@@ -560,6 +571,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
       tile += w.nt;
       sa_done(w);
     }
+    sa_settle<2>(pv_done, n, p.status, kTimeoutAccum);
   } else {
     // ================================================================ softmax and epilogue: one row a thread
     const int g = warp >> 2, row = (warp & 3) * 32 + lane, tok = row / p.G, sub = row % p.G;
@@ -705,6 +717,7 @@ __global__ void __launch_bounds__(STHREADS, 1) attn_shared_kernel(const SharedAt
         }
       }
     }
+    sa_tmem_st_wait();
   }
 
   tc_fence_before();

@@ -316,3 +316,20 @@ def test_shared_attention_merge_stays_in_its_workspace():
             assert (u, c0, own) == (begin, (begin + 8) // piece, (begin + 8 + ((units - 1) << two)) // piece - (begin + 8) // piece + 1)
 
 
+def test_shared_attention_settles_what_it_started():
+    """A role whose wait runs out leaves its loop with copies or products in flight.  Every ring that a warp starts something on is waited for
+    behind the loops, use by use, ahead of the barrier that the CTA's tensor memory is given back behind."""
+    text = shared_attention_source()
+    body = re.search(r"void sa_settle\(.*?\n}", text, re.S).group()
+    assert "int j = max(0, uses - SLOTS); j < uses; ++j" in body and "mbar_wait(&ring[j % SLOTS], (j / SLOTS) & 1," in body
+    loaders, scores, outputs, softmax = re.split(r"\} else if \(warp == 8\) \{|\} else if \(warp == 11\) \{|\n  \} else \{\n",
+                                                 text[text.index("if (warp == 9 || warp == 10)"):text.index("attn_shared_merge_kernel")])[:4]
+    settled = lambda role: re.findall(r"sa_settle<(.*?), p\.status", role)
+    assert settled(loaders) == ["KSLOTS>(values ? kv_full + KSLOTS : kv_full, n", "2>(q_full, uses"]
+    assert settled(scores) == ["2>(s_full, n"] and settled(outputs) == ["2>(pv_done, n"]
+    end = softmax[softmax.rindex("sa_tmem_st_wait()"):]
+    assert "tcgen05" not in end and end.index("__syncthreads()") < end.index("tmem_dealloc")
+    for role, commits in ((scores, "umma_commit(&s_full[g])"), (outputs, "umma_commit(&pv_done[g])")):      # a commit of that ring for every use
+        assert role.count(commits) == 1 and "++job, ++n" in role
+
+
