@@ -333,3 +333,71 @@ def test_shared_attention_settles_what_it_started():
         assert role.count(commits) == 1 and "++job, ++n" in role
 
 
+# ------------------------------------------------------------------ attention: many items a CTA, many sequences
+def line_of_work(c):
+    """Restated from the kernel's description: the segments of every CTA on the line of items, as (units of the segment, units of the item,
+    both tiles of the pair have rows, of the prefix)."""
+    keys, cost, ctas = 96, 8, 148
+    T, hq, _ = c["q"].shape
+    hkv = c["k_pool"].shape[0]
+    npt = 128 // (hq // hkv)
+    cu, past = c["cu_q"].tolist(), c["past_lens"].tolist()
+    B = len(past)
+    shared = 4 * T <= 3 * max(B * npt, T + B * npt // 2)
+    prefix = c["prefix_len"] // 16 * 16 if shared else 0
+    seqs = ([(cu[-1], prefix, prefix, 0, True)] if prefix else []) + [(cu[b + 1] - cu[b], past[b], past[b] + cu[b + 1] - cu[b], prefix, False)
+                                                                      for b in range(B)]
+    items = []
+    for n, committed, end, first, common in seqs:
+        for pair in range(-(-n // (2 * npt))):
+            last = min(end, committed + (pair + 1) * 2 * npt) if c["causal"] and not common else end
+            units, two = -(-max(0, last - first) // keys), n - pair * 2 * npt > npt
+            items += [(units, two, common)] * (hkv * (units > 0))
+    total = sum((u << two) + cost for u, two, _ in items)
+    piece = max(1, -(-total // ctas))
+    segments, at = [[] for _ in range(ctas)], 0
+    begins = lambda t, two: (max(0, t - cost) + two) >> two
+    for units, two, common in items:
+        length = (units << two) + cost
+        for cta in range(at // piece, (at + length - 1) // piece + 1):
+            lo, hi = max(at, cta * piece) - at, min(at + length, (cta + 1) * piece) - at
+            part = begins(hi, two) - begins(lo, two)
+            if part > 0:
+                segments[cta].append((part, units, two, common))
+        at += length
+    return segments
+
+
+LONG = dict(heads=64, kv_heads=16, prefix=600, behind=[(37 * i) % 400 for i in range(16)], counts=[64 + (29 * i) % 65 for i in range(16)])
+MANY = [(500, 40, 4), (769, 16, 2)]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_long_items_come_whole(causal):
+    """What the test on the GPU below is about: CTAs with several items that they finish alone, of several units, beside items that are cut."""
+    segments = line_of_work(attention_case(7, causal=causal, **LONG))
+    whole = [[s for s in cta if s[0] == s[1] and s[2]] for cta in segments]
+    assert sum(len(w) >= 2 and min(s[1] for s in w) >= 7 for w in whole) >= 20 and not any(s[3] for cta in segments for s in cta)
+    assert sum(s[0] < s[1] for cta in segments for s in cta) >= 50
+
+
+@gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_shared_prefix_attention_of_long_items(clean, causal):
+    c = attention_case(7, causal=causal, device="cuda", **LONG)
+    want = attention_exact(c)
+    got = attend(c, max_q=128)
+    attention_close(got, want)
+    assert torch.equal(got, attend(c, max_q=128))
+
+
+@gpu
+@pytest.mark.parametrize("B,heads,kv", MANY)
+def test_shared_prefix_attention_of_many_sequences(clean, B, heads, kv):
+    """More sequences than a CTA has threads: their lengths are summed in rounds."""
+    c = attention_case(B, heads, kv, 150, [(13 * i) % 60 for i in range(B)], [1 + (i % 7 == 3) for i in range(B)], True, device="cuda", slack=1.0)
+    want = attention_exact(c)
+    attention_close(attend(c, max_q=2), want)
+    attention_close(attend({**c, "prefix_len": 0}, max_q=2), want)
+
+
