@@ -20,9 +20,9 @@
 // What bounds it: the way of a job's scores, product to registers to the next job's product, with the second product of the job
 // before in between: 1,380 cycles a job of 128 rows x 96 keys, of which the tensor pipe is busy for 770 (56 %), the special function
 // unit for 800 (58 %) and the schedulers for 620 (45 %).  16 trees of 128 nodes behind
-// 8192 keys (floor 176 us): 255 us, 293 under the power cap.  Against it, in turn on one GPU: 80 keys and scores of their own for each
-// group 312 (293 here), scores of their own and one set of probabilities 269 (260 here), 128 keys (which spill) 306 (279 here), 64
-// keys and probabilities in two buffers 336 (279 here), a quarter of the exponentials as polynomials 299 (279 here).
+// 8192 keys (floor 176 us): 254 us, 300 under the power cap.  Times of other forms relative to it, each timed in turn with it: 80 keys and
+// scores of their own for each group 1.06, scores of their own and one set of probabilities 1.03, 128 keys (which spill) 1.10, 64 keys
+// and probabilities in two buffers 1.20, a quarter of the exponentials as polynomials 1.07.
 #include "gemm_common.cuh"
 
 #include <math.h>
@@ -873,7 +873,11 @@ static long long shared_layout(SharedAttn* p, uint8_t* ws, int max_q) {
 }
 
 // Attending to the prefix for all rows together pays where sequences leave much of their own tiles empty: tiles of all rows together
-// against those of B sequences, whose last ones are half full on average.
+// against those of B sequences, whose last ones are half full on average.  Together / alone, us: 64 x 1 row behind 8192 keys 53 / 317, 8 x 1
+// behind 1024 17.6 / 22; 16 trees (32 over 8 heads) behind 2048 of 16 rows 34 / 41, of 32 46 / 47, of 48 58 / 56 (the last that go
+// together), of 64 66 / 58, of 128 behind 8192 289 / 265; 6 prompts of 33 - 901 rows 236 / 188.  It knows nothing of lengths, and misses
+// some: 16 trees of 96 rows behind 8192 keys would gain (220 / 266), two of 16 behind 4096 lose (43 / 34); below some 100 keys and for one
+// sequence it makes no difference (8 x 1 row behind 64 keys 17.3 / 17.4, one row 15.5 / 15.4).
 static bool shared_pays(int B, int T, int npt) {
   const long long together = T, own = std::max(static_cast<long long>(B) * npt, T + static_cast<long long>(B) * npt / 2);
   return 4 * together <= 3 * own;

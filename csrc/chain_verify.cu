@@ -4,18 +4,19 @@
 // place, and one more target row stands behind the last draft.  With p_i = softmax(target row i / T), q_i = softmax(draft row i / Td):
 // x_i is accepted when all before it were and u_i q_i(x_i) < p_i(x_i).  With a drafts accepted, the next token is drawn by
 // inverse CDF with v from p_n when a == n, else from max(p_a - q_a, 0): the committed tokens are then samples of the target.
-// A temperature below 1e-5 is a point mass at the lowest most likely index.
+// A temperature below 1e-5 is a point mass at the lowest most likely index.  A row with a NaN says as little as one without a logit above -inf.
 //
 // chain_stats_kernel reads the rows of some drafts (maximum, sum of exponentials) and decides about them; chain_token_kernel draws
 // the token, a cluster per sequence.  A block of the first kernel asks whether an earlier draft of its sequence is known to be
 // rejected before it reads; blocks start in the order of their drafts, eight at a time, so that most rows behind a rejection are not
-// read (64 chains of 4 to 16 drafts over 151936 fp32 values 146 us; all drafts at a time 187, four 155; six launches for draft 0, 1,
-// 2, 3-4, 5-8 and the rest 182, as each starts and ends with SMs that have nothing in flight).  Sums that only decide `u q < p` are fp32
-// (a decision is off by some 1e-7 of a probability); the running sum that a token is found in is fp64, as its index would change with
-// every rounding among 150,000 terms.
+// read (64 chains of 4 to 16 drafts over 151936 fp32 values 149 us; four at a time 157, sixteen 150, all 170).  Sums that only decide
+// `u q < p` are fp32: a probability is off by some 1e-6 of itself at most (a term e bits below the maximum by 3.5 e 2^-24 of itself, the
+// hardware's exponential by 2^-22, what is added up by a few 2^-24); the drafted token's own exponential is fp64.  The running sum
+// that a token is found in is fp64, as its index would change with every rounding among 150,000 terms.
 //
-// What bounds it: few sequences, latency (one chain of 3 drafts 26 us, 12 us in either kernel); many, reading (90 of those 146 us) and
-// the fp64 pipe with the table's banks (the draw, 60 us).
+// What bounds it: few sequences, latency (one chain of 3 drafts 25 us, 12 us in either kernel); many, reading (90 of those 149 us) and
+// the draw (60 us), whose warps wait for values, barriers of the cluster and fp64 chains (16 sequences: fp64 pipe 30 % of the time that
+// an SM has work, 47 % on the busiest SM).
 #include "common.cuh"
 
 #include <math.h>
@@ -23,8 +24,8 @@
 
 namespace js {
 
-// A block of the first kernel reads 16 KB of either row at once.  fp32: 128 threads, six blocks an SM (64 sequences 192 us, 208 with four of 256
-// threads); bf16 has twice the values, that want the registers of 256 threads (16 sequences 61 us, 81 with 128).
+// A block of the first kernel reads 16 KB of either row at once.  fp32: 128 threads, six blocks an SM (64 sequences 149 us, 167 with four of 256
+// threads); bf16 has twice the values, that want the registers of 256 threads (16 sequences 55 us, 74 with 128).
 constexpr int kChunkBytes = 16384;
 template <typename T>
 struct StatShape { static constexpr int kThreads = 256, kResident = 4; };
@@ -496,8 +497,8 @@ template <typename T>
 static int launch_chain(const ChainParams& p, cudaStream_t stream) {
   chain_stats_kernel<T><<<dim3(p.chunks, p.B, kAhead), StatShape<T>::kThreads, 0, stream>>>(p);
   if (cudaGetLastError() != cudaSuccess) return -4;
-  // As many CTAs a sequence as are there at once, two an SM (16 is more than a portable cluster has): 16 sequences 56 us with 16, 61 with 8, 68 with
-  // 4; 64 sequences 184 us with 4, 193 with 8, 214 with 2.
+  // As many CTAs a sequence as are there at once, two an SM (16 is more than a portable cluster has).  us with 16, 8, 4 and 2: one sequence 25, 29, 38,
+  // 56; 16 sequences 54, 59, 63, 86; 48 (32001 words) 54, 39, 38, 39; 64 184, 158, 149, 170.
   constexpr int kAtOnce = 2 * 148;
   if (p.B * 16 <= kAtOnce) return launch_token<T, 16>(p, stream);
   return p.B * 8 <= kAtOnce ? launch_token<T, 8>(p, stream) : launch_token<T, 4>(p, stream);

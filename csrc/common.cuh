@@ -31,7 +31,7 @@ enum : int {
   kTimeoutTopk = 11,      // vocabulary-parallel top-k: a rank's record never arrived
   kEpOverflow = 12,       // more rows for one expert (or one rank) than the receive slab / the grouped launch covers
   kNoPage = 13,           // slot plan: the free pages ran out
-  kRowsOverflow = 14,     // slot plan: more new rows than the row buffers hold
+  kRowsOverflow = 14,     // more new rows than the caller's bound (the rows of a slot plan, a sequence's rows in shared-prefix attention)
   kBadToken = 15,         // a drafted token outside the vocabulary
   kShortPrefix = 16,      // a sequence that is shorter than the prefix it shares
 };
