@@ -271,12 +271,12 @@ __global__ void __launch_bounds__(StatShape<T>::kThreads, StatShape<T>::kResiden
   }
 }
 
-// 2^(t / 512) for t from -512 * 1020 to 0 (results stay above the smallest normal number, 2^-1022): t = n + r, a table of 2^(j/512) and the series of 2^(r/512) to the second power, |r| <= 1/2
-// (P. Tang's table-driven scheme): relative error below 6e-11, of either sign.
+// 2^(t / 512) for t from -512 * 1020 to 0 (results stay above the smallest normal number, 2^-1022): t = n + r, a table of 2^(j/512) and the
+// series of 2^(r/512) to the second power, |r| <= 1/2 (P. Tang's table-driven scheme): relative error below 6e-11, of either sign.
 constexpr int kExpTable = 512;
-// Probabilities are cut below 2^-890 of the most likely one's, and count there as something from 2^-990 to 2^-890: divided by a sum of up to 2^28
-// terms they stay in the table's domain, and that many of them add up to less than 2^-860, below which a sum counts as zero.
-constexpr double kCut = -890.0 * kExpTable, kNoSum = 0x1p-860;
+// Probabilities are cut below 2^-790 of the most likely one's, and count there as something from 2^-990 to 2^-790: divided by a sum of up to 2^28
+// terms they stay in the table's domain, and that many of them add up to less than 2^-760, below which a sum counts as zero.
+constexpr double kCut = -790.0 * kExpTable, kNoSum = 0x1p-760;
 JS_DEVICE double exp2_table(double t, const double* table) {
   constexpr double kRound = 6755399441055744.0;              // 1.5 * 2^52: the integer part of the sum's low word
   constexpr double c1 = 0.69314718055994531 / kExpTable;
@@ -289,7 +289,7 @@ JS_DEVICE double exp2_table(double t, const double* table) {
 
 // Table steps a logit, and half the logit at which a row is cut, rounded down (logits are halved, so that the cut of any finite maximum is finite and
 // -inf lies below it).  Where the next value below the maximum has 2^-100 of its probability or less, that is as good as nothing: the slope stops
-// there, so that rounding takes the cut down by 2^-100 at most.
+// there, so that rounding takes the cut down by 2^-200 at most (below a negative power of two values lie twice as far from each other as above).
 struct ChainAxis {
   double slope;
   float least;

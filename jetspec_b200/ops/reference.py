@@ -375,7 +375,7 @@ def verify_chains(target_logits: torch.Tensor, draft_logits: torch.Tensor, draft
 
     A target row without any logit above -inf, or with a NaN, accepts nothing; its next token is -1.  Such a draft row says nothing:
     what the target can say at all is accepted.  Where rounding leaves nothing of ``max(p - q, 0)`` the target's most likely token
-    is taken.  Returns ``(accepted (B,) int32, next token (B,) int64)``.
+    is taken; where it adds up to less than some 1e-10 (a draft from ``q`` is rejected there as rarely) the kernel's rounding decides.  Returns ``(accepted (B,) int32, next token (B,) int64)``.
     """
     B = cu_drafts.numel() - 1
     cu = cu_drafts.tolist()

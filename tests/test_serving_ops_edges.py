@@ -173,6 +173,21 @@ def test_generate_chain_of_a_target_that_says_nothing(monkeypatch, value):
     assert len(fed) == 2 and all(int(ids.min()) >= 0 for ids in fed)
 
 
+@gpu
+def test_verify_chains_kernel_cuts_across_a_power_of_two(clean):
+    """A maximum just above a negative power of two, at a temperature that sets neighbouring values worlds apart: the values below it, and
+    with them what the cut is rounded by, lie twice as far from each other."""
+    V, top = 2 ** 24 + 19, -(2.0 ** 14 - 2.0 ** -9)
+    assert float(torch.tensor(top)) == top and float(torch.nextafter(torch.tensor(top), torch.tensor(0.0))) == top + 2.0 ** -10
+    target, draft = torch.full((2, V), top, device="cuda"), torch.full((1, V), top, device="cuda")
+    target[0, 11], target[0, 12] = -INF, -1e5
+    draft[0, 5], draft[0, 9] = -INF, -1e5
+    for v, want in ((0.0, 5), (0.49, 5), (0.51, 9)):
+        accepted, token = ops.verify_chains(target, draft, i32(11, device="cuda"), i32(0, 1, device="cuda"), torch.tensor([0.5], device="cuda"),
+                                            torch.tensor([v], device="cuda"), temperature=1e-5)
+        assert (accepted.tolist(), token.tolist()) == ([0], [want])
+
+
 # ------------------------------------------------------------------ attention behind a shared prefix
 @pytest.mark.skipif(torch.cuda.is_available(), reason="addresses of nothing: not where a mistake would launch a kernel on them")
 def test_shared_attention_entry_refuses_addresses():
