@@ -286,7 +286,6 @@ def test_plan_slots_of_a_padded_batch():
 def test_plan_slots_kernel_of_a_padded_batch(clean):
     padded_plan("cuda")
     clean.check_status("cuda")
-    e = i32(device="cuda")
     ops.plan_slots(i32(4, 4, device="cuda"), i32(0, 4, device="cuda"), i32(9, 9, device="cuda"), i32(1, 2, device="cuda"), 4,
                    torch.zeros(3, 32, dtype=I32, device="cuda"), 4, mapped_lens=i32(4, 8, device="cuda"))
     with pytest.raises(RuntimeError, match="status 5"):      # rows there are, and their request's slot-map row is not
@@ -295,7 +294,6 @@ def test_plan_slots_kernel_of_a_padded_batch(clean):
                    torch.zeros(3, 32, dtype=I32, device="cuda"), 0, mapped_lens=i32(0, device="cuda"))
     with pytest.raises(RuntimeError, match="status 5"):      # a page was granted, and its slots have nowhere to go
         clean.check_status("cuda")
-    assert e.numel() == 0
 
 
 # ------------------------------------------------------------------ attention when a wait has run out: that cannot be staged on a GPU
@@ -414,5 +412,3 @@ def test_shared_prefix_attention_of_many_sequences(clean, B, heads, kv):
     want = attention_exact(c)
     attention_close(attend(c, max_q=2), want)
     attention_close(attend({**c, "prefix_len": 0}, max_q=2), want)
-
-
